@@ -1,4 +1,4 @@
-"""Access to libscmx.so (the C ABI declared in include/scmx.h): `native()` is what the wrappers call, tensors in, one native
+"""Access to libscmx.so (the C ABI declared in include/scmx.h and scmx_cache.h): `native()` is what the wrappers call, tensors in, one native
 call per launch (csrc/torch_binding.cpp); `load()` the whole ABI through ctypes, for the queries and for foreign callers,
 with `call`, `ptr` and `stream` to check a status and to make arguments of tensors.
 There is no fallback: a missing or incomplete library raises, and so does every call that returns a negative status."""
@@ -72,6 +72,15 @@ SIGNATURES = {
     "scmx_quantize_family": (_I, [_FMT, _P, _I, _L, _I, _P, _P, _P, _P]),
     "scmx_quantize_sc": (_I, [_P, _I, _L, _I, _I, _P, _P, _P, _P]),
 }
+# the same of include/scmx_cache.h
+CACHE_SIGNATURES = {
+    "scmx_cache_write": (_I, [_P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _I, _P]),
+    "scmx_cache_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "scmx_cache_keep": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
+    "scmx_attn_tree": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _I, _I, _I, _I, _F, _P, _I, _P]),
+    "scmx_verify_workspace": (_Z, [_I, _I, _I]),
+    "scmx_verify_drafts": (_I, [_P, _P, _P, _I, _P, C.c_double, _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P]),
+}
 
 _lib = None
 
@@ -84,7 +93,7 @@ def load():
             raise RuntimeError(f"{LIB_PATH} is missing: build it with `python {os.path.join(HERE, 'build.py')}` "
                                "(there is no CPU or PyTorch fallback for these kernels)")
         lib = C.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | CACHE_SIGNATURES).items():
             fn = getattr(lib, name)       # AttributeError if the library lacks a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = lib

@@ -11,7 +11,8 @@ LIB = os.path.join(HERE, "libscmx.so")
 BINDING = os.path.join(HERE, "_binding.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 SOURCES = ["gemm_rows.hip", "gemm_blocked.hip", "gemm_grouped.hip", "gemm_rows_idle.hip", "gemm.hip", "api.hip",
-           "gemm_skinny.hip", "gemv.hip", "rowops.hip", "quantize.hip", "attn.hip", "attn_prefill.hip", "linear_bf16.hip", "silu_table.hip"]
+           "gemm_skinny.hip", "gemv.hip", "rowops.hip", "quantize.hip", "attn.hip", "attn_prefill.hip", "linear_bf16.hip", "silu_table.hip",
+           "cache.hip", "attn_tree.hip", "verify.hip"]
 # packed FP32 instructions are kept off (they have misbehaved on this hardware pool); no FMA contraction, so the
 # FP32 epilogues and norms round exactly like a plain IEEE evaluation
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt", "-Wno-unused-command-line-argument", "-fconstexpr-steps=400000000",
@@ -69,19 +70,20 @@ def build_binding():
     return BINDING
 
 
-def build_host_check(driver, out=None):
-    """The library's sources and a C++ driver of the C ABI as ONE executable whose HOST code is instrumented with
+def build_host_check(driver, out=None, sources=None):
+    """The library's sources (or those named) and a C++ driver of the C ABI as ONE executable whose HOST code is instrumented with
     AddressSanitizer and UBSan (device code is compiled as usual and never runs in this check): for machines without a
     GPU, where every entry point ends at its argument checks or at the failing launch.  Returns the executable's path."""
     hipcc = os.environ.get("HIPCC", "hipcc")
     objdir = os.path.join(HERE, "build", "host_check")
     os.makedirs(objdir, exist_ok=True)
     out = out or os.path.join(objdir, "boundary_check")
+    sources = sources or SOURCES
     san = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined", "-Xarch_host",
            "-fno-sanitize-recover=undefined", "-g", "-fno-omit-frame-pointer"]
     flags = [f for f in FLAGS if f != "-O3"] + ["-O1"]
-    objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in SOURCES]
-    cmds = [[hipcc, *flags, *san, "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)]
+    objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in sources]
+    cmds = [[hipcc, *flags, *san, "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(sources, objs)]
     dobj = os.path.join(objdir, "driver.o")
     cmds.append([hipcc, "-x", "hip", *flags, *san, "-c", driver, "-o", dobj])
     with ThreadPoolExecutor(4) as ex:

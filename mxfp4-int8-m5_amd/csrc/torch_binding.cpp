@@ -1,5 +1,5 @@
 // Python binding of the C ABI for torch tensors: `_binding`, a module whose functions are the entry points of
-// include/scmx.h that enqueue work (and four of its queries), under the same names and with the same arguments except the
+// include/scmx.h and scmx_cache.h that enqueue work (and five of their queries), under the same names and with the same arguments except the
 // last.  A pointer argument takes a tensor (contiguous, on the GPU), None or an integer address; a format argument an object
 // whose buffer is the scmx_format; the stream is the caller's current one and is not passed.  A negative status raises.
 //
@@ -17,7 +17,7 @@
 #include <type_traits>
 #include <utility>
 
-#include "../../include/scmx.h"
+#include "../../include/scmx_cache.h"
 
 namespace {
 
@@ -258,8 +258,10 @@ PyMODINIT_FUNC PyInit__binding() {
         ENTRY(scmx_quantize_sc), ENTRY(scmx_quantize_family),
         QUERY(scmx_linear_w4a8_workspace), QUERY(scmx_gemv_rows_workspace), QUERY(scmx_mm_w4a8_prefers_blocked),
         QUERY(scmx_moe_mm_takes_slots),
+        ENTRY(scmx_cache_write), ENTRY(scmx_cache_read), ENTRY(scmx_cache_keep), ENTRY(scmx_attn_tree), ENTRY(scmx_verify_drafts),
+        QUERY(scmx_verify_workspace),
         {"gemv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&gemv)), METH_FASTCALL, nullptr},
-        EMPTY(bf16, BFloat16), EMPTY(i8, Char), EMPTY(u8, Byte), EMPTY(i32, Int), EMPTY(f32, Float),
+        EMPTY(bf16, BFloat16), EMPTY(i8, Char), EMPTY(u8, Byte), EMPTY(i32, Int), EMPTY(i64, Long), EMPTY(f32, Float),
         {nullptr, nullptr, 0, nullptr}};
     module_def.m_methods = methods;
     return PyModule_Create(&module_def);
