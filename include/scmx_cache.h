@@ -40,12 +40,15 @@ int scmx_cache_read(const int8_t* kcache, const int8_t* vcache, const float* ksc
 int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d, int cache_rows, const int32_t* path,
                     const int32_t* count, int T, const int64_t* pos_dev, int64_t pos0, void* stream);
 
-/* Attention of the T nodes of a tree: out bf16 [T, hq * d] = softmax(q . K^T * scale) V, q bf16 [T, hq, d].  Every node sees
+/* Attention of the T nodes of a tree: out bf16 [T, hq * d] = softmax(q . K^T * scale) V, q bf16 [T, hq, d], hq / hk up to 4096.  Every node sees
  * the rows below pos; row pos + j is seen by node i if bit j of mask[i] is set (mask NULL: j <= i, a chain).  A node that sees
  * nothing gets zeros; what a node does not see does not reach its result, infinities and NaN among it.  T = 1 is the decode
  * step's attention over an 8-bit cache.  With pos_dev, a position whose rows do not fit the cache gives zeros.
  * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16, 32 or 64 query rows; more than one needs
- * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches. */
+ * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches.
+ * scmx_attn_tree_splits: how many to take for n rows in all (the cache's, where the position is on the device); 1 for arguments that
+ * scmx_attn_tree refuses. */
+int scmx_attn_tree_splits(int T, int n, int hq, int hk, int d);
 int scmx_attn_tree(const uint16_t* q, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
                    const int64_t* mask, const int64_t* pos_dev, int64_t pos0, uint16_t* out, int T, int hq, int hk, int d,
                    int cache_rows, float scale, float* workspace, int splits, void* stream);

@@ -78,6 +78,7 @@ CACHE_SIGNATURES = {
     "scmx_cache_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "scmx_cache_keep": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
     "scmx_attn_tree": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _I, _I, _I, _I, _F, _P, _I, _P]),
+    "scmx_attn_tree_splits": (_I, [_I, _I, _I, _I, _I]),
     "scmx_verify_workspace": (_Z, [_I, _I, _I]),
     "scmx_verify_drafts": (_I, [_P, _P, _P, _I, _P, C.c_double, _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P]),
 }

@@ -24,6 +24,7 @@
 #include <math.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "../../include/scmx_cache.h"
 #include "scmx_common.h"
@@ -32,10 +33,10 @@ namespace scmx {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // scales: aligned as floats
 
-constexpr int TNT = 256, TWAVES = TNT / 64, TKEYS = 32, TXCDS = 8;
-constexpr int TTILES_MIN = 8;   // tiles a range has at least (two a wave), where there are that many
+constexpr int TKEYS = 32, TXCDS = 8, JNT = 256;
+// Waves of a workgroup: two a SIMD; rows of 256 in bf16 take the registers of two.
+static constexpr __host__ __device__ int tree_waves(int d, bool eight) { return d == 256 && !eight ? 4 : 8; }
 
 struct TreeArgs {
     const uint16_t* q;
@@ -47,45 +48,42 @@ struct TreeArgs {
     const int64_t* pos_dev;
     int64_t pos0;
     uint16_t* out;
-    float* part;      // [splits][T hq][d] sums, then [splits][T hq][2]: reference, denominator
+    float* part;      // [T hq][splits][d] sums, then [T hq][splits][2]: reference, denominator
     int T, hq, hk, rows, splits, blocks;   // blocks: of query rows
+    uint32_t by_group;                     // 2^32 / (hq / hk), rounded up: r / group as a high product, exact for r group < 2^32
     float scale;      // times log2 e
 };
 
-// The ranges of a context of n keys in all: tiles each, and how many of them have any.
-static __device__ __host__ inline int range_tiles(int n, int splits) {
+// Tiles of a range, of a context of n keys in all: one range up to two tiles a wave, then a tile a wave at least.
+static __device__ __host__ inline int range_tiles(int n, int splits, int waves) {
     const int tiles = (n + TKEYS - 1) / TKEYS, even = (tiles + splits - 1) / splits;
-    return even > TTILES_MIN ? even : TTILES_MIN;
+    return tiles <= 2 * waves ? 2 * waves : even > waves ? even : waves;
 }
 
-template <int D, int RT, bool EIGHT>
-struct Tree {
-    static constexpr int ROWB = EIGHT ? D : 2 * D;   // bytes of a cache row
-    static constexpr int KL = ROWB / 64;             // 16-byte loads of a lane from a K row
-    static constexpr int VW = ROWB / 64;             // words of a lane from a V row
-    static constexpr int DPL = D / 16;               // head-dimension indexes of a lane in V^T, and MFMAs of the second product
-    static constexpr int ROWS = 16 * RT;
-    // What one tile of keys is loaded into.
-    struct Raw {
-        u32x4 k[2][KL];
-        uint32_t v[8][VW];
-        float ks[8], vs[8];
-    };
-};
+// Broadcast of lane N of each row of 16 lanes to the row.
+template <int N>
+__device__ __forceinline__ float row_lane(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + N, 0xF, 0xF, true));
+}
+template <typename F, int... E>
+__device__ __forceinline__ void for_eight(F&& f, std::integer_sequence<int, E...>) { (f(std::integral_constant<int, E>{}), ...); }
 
-// v_cvt_f32 of byte B of w as a signed number, as the bits of a float.
+// Byte B of w, a signed number, as the bits of a float.
 template <int B>
 __device__ __forceinline__ uint32_t byte_f32(uint32_t w) { return __float_as_uint(float(int8_t(w >> (8 * B)))); }
 
 template <int D, int RT, bool EIGHT>
-__global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
-    using W = Tree<D, RT, EIGHT>;
-    constexpr int ROWB = W::ROWB, KL = W::KL, VW = W::VW, DPL = W::DPL, SLICES = D / 32;
+__global__ __launch_bounds__(64 * tree_waves(D, EIGHT), tree_waves(D, EIGHT) / 4) void attn_tree_kernel(const TreeArgs a) {
+    constexpr int ROWB = EIGHT ? D : 2 * D;   // bytes of a cache row
+    constexpr int KL = ROWB / 64;             // 16-byte loads of a lane from a K row
+    constexpr int VW = ROWB / 64;             // words of a lane from a V row
+    constexpr int DPL = D / 16;               // head-dimension indexes of a lane in V^T, and MFMAs of the second product
+    constexpr int ROWS = 16 * RT, SLICES = D / 32, WAVES = tree_waves(D, EIGHT), NT = 64 * WAVES;
     constexpr float NEG = -__builtin_inff();
     // how far scores may pass the reference, and where it is put below the largest score (both in powers of two)
     constexpr float PASS = EIGHT ? 6.0f : 8.0f, BELOW = EIGHT ? 8.0f : 0.0f;
-    __shared__ float s_o[TWAVES][W::ROWS][D + 4];
-    __shared__ float s_m[TWAVES][W::ROWS], s_l[TWAVES][W::ROWS];
+    __shared__ float s_o[WAVES][ROWS][D + 4];
+    __shared__ float2 s_ml[WAVES][ROWS];   // reference, denominator
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
     // blocks of the query rows of one range and KV head run on one XCD, behind one L2
@@ -93,33 +91,111 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
     const int block = in / TXCDS, combo = turn * TXCDS + in % TXCDS;
     if (combo >= a.hk * a.splits) return;
     const int kvh = combo % a.hk, range = combo / a.hk, group = a.hq / a.hk, rows_all = a.T * group;
-    const int row0 = block * W::ROWS;
-    const auto out_row = [&](int r) { return size_t(r / group) * a.hq + size_t(kvh) * group + r % group; };   // of [T, hq]
+    const int row0 = block * ROWS;
+    const auto token = [&](int r) { return group == 1 ? r : int(__umulhi(uint32_t(r), a.by_group)); };
+    const auto out_row = [&](int r) { return size_t(token(r)) * a.hq + size_t(kvh) * group + (r - token(r) * group); };   // of [T, hq]
 
     const int64_t pos64 = a.pos_dev ? a.pos_dev[0] : a.pos0;
     if (pos64 < 0 || pos64 > int64_t(a.rows) - a.T) {   // (a device-resident position that the host could not see)
         if (range == 0)
-            for (int i = tid; i < W::ROWS * D; i += TNT)
+            for (int i = tid; i < ROWS * D; i += NT)
                 if (row0 + i / D < rows_all) a.out[out_row(row0 + i / D) * D + i % D] = 0;
         return;
     }
     const int pos = int(pos64), n = pos + a.T, tiles = (n + TKEYS - 1) / TKEYS;
-    const int per = range_tiles(n, a.splits);
+    const int per = range_tiles(n, a.splits, WAVES);
     const int first = range * per, last = min(tiles, first + per);
     if (first >= last) return;   // an empty range: the join knows
     const bool whole = per >= tiles;
 
+    const uint8_t* kb = a.k + size_t(kvh) * a.rows * ROWB;
+    const uint8_t* vb = a.v + size_t(kvh) * a.rows * ROWB;
+    u32x4 kr[2][KL];
+    uint32_t vr[8][VW];
+    float sc = 0.0f;   // 8 bits: lanes 0..7 of a row of 16 hold the K scales of the row's eight keys, 8..15 the V scales
+    // (The last row stands in for the ones behind it, which are not read.  A branch that spares full tiles the minima costs the loads'
+    // overlap: 40000 rows in one range 237 -> 260 us.)
+    const auto load_k = [&](int tile) __attribute__((always_inline)) {
+        const int base = tile * TKEYS;
+        const auto row = [&](int i) { return min(i, n - 1 - base); };
+        const uint8_t* kt = kb + size_t(base) * ROWB;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const unsigned at = unsigned(row(16 * h + ln) * ROWB + 16 * g);
+#pragma unroll
+            for (int u = 0; u < KL; ++u) kr[h][u] = *reinterpret_cast<const u32x4*>(kt + at + 64 * u);
+        }
+        if constexpr (EIGHT) {
+            const float* from = (ln < 8 ? a.ks : a.vs) + size_t(kvh) * a.rows + base;
+            sc = from[row(16 * (ln / 4 % 2) + 4 * g + ln % 4)];
+        }
+    };
+    const auto load_v = [&](int tile) __attribute__((always_inline)) {
+        const int base = tile * TKEYS;
+        const auto row = [&](int i) { return min(i, n - 1 - base); };
+        const uint8_t* vt = vb + size_t(base) * ROWB;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint8_t* p = vt + unsigned(row(16 * (e / 4) + 4 * g + e % 4) * ROWB + ROWB / 16 * ln);
+            if constexpr (VW == 1) {
+                vr[e][0] = *reinterpret_cast<const uint32_t*>(p);
+            } else if constexpr (VW == 2) {
+                const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+                vr[e][0] = w[0];
+                vr[e][1] = w[1];
+            } else {
+#pragma unroll
+                for (int u = 0; u < VW / 4; ++u) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(p + 16 * u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vr[e][4 * u + i] = w[i];
+                }
+            }
+        }
+    };
+    // The queries.  32 rows, or rows of 256, come through LDS: read by every wave for itself, as 64-byte pieces of 16 rows an
+    // instruction, they held up the first keys by 1.5 us (16 tokens, 300 rows: 10.9 -> 8.9 us); 16 rows of 128 do not (6.6, direct 6.2).
+    constexpr bool QLDS = RT > 1 || D > 128;
+    constexpr int QPIECES = ROWS * D / 8, QROW = D + 8;   // 16-byte pieces; LDS row in values
+    constexpr int QPER = (QPIECES + NT - 1) / NT;         // a thread (the ones left over bring some again)
+    __shared__ __attribute__((aligned(16))) uint16_t s_q[QLDS ? ROWS * QROW : 1];
+    const auto q_at = [&](int s) { return EIGHT ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };   // slice s of a lane, in K's order
     bf16x8 qf[RT][SLICES];
+    u32x4 qraw[QPER];
+    if constexpr (QLDS) {
+#pragma unroll
+        for (int i = 0; i < QPER; ++i) {
+            const int c = (tid + NT * i) % QPIECES;
+            qraw[i] = *reinterpret_cast<const u32x4*>(a.q + out_row(min(row0 + c / (D / 8), rows_all - 1)) * D + c % (D / 8) * 8);
+        }
+    }
     uint64_t seen[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(row0 + 16 * rt + ln, rows_all - 1);
-        const uint16_t* qp = a.q + out_row(r) * D;
+        const int i = token(min(row0 + 16 * rt + ln, rows_all - 1));
+        seen[rt] = (a.mask ? uint64_t(a.mask[i]) : ~0ull >> (63 - i)) & ~0ull >> (64 - a.T);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const int start = first + wave < last ? first + wave : last - 1;   // (a wave without a tile loads one and uses none)
+    load_k(start);
+    if constexpr (!QLDS) {
+        const uint16_t* qp = a.q + out_row(min(row0 + ln, rows_all - 1)) * D;
 #pragma unroll
-        for (int s = 0; s < SLICES; ++s)
-            qf[rt][s] = *reinterpret_cast<const bf16x8*>(qp + (EIGHT ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g));
-        const int i = r / group;
-        seen[rt] = a.mask ? uint64_t(a.mask[i]) : ~0ull >> (63 - i);
+        for (int s = 0; s < SLICES; ++s) qf[0][s] = *reinterpret_cast<const bf16x8*>(qp + q_at(s));
+    }
+    load_v(start);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (QLDS) {
+#pragma unroll
+        for (int i = 0; i < QPER; ++i) {
+            const int c = (tid + NT * i) % QPIECES;
+            *reinterpret_cast<u32x4*>(s_q + c / (D / 8) * QROW + c % (D / 8) * 8) = qraw[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int s = 0; s < SLICES; ++s) qf[rt][s] = *reinterpret_cast<const bf16x8*>(s_q + (16 * rt + ln) * QROW + q_at(s));
     }
     f32x4 o[RT][DPL], ones[RT];   // ones: sums of the rounded weights (bf16)
     float m[RT], l[RT];
@@ -132,114 +208,62 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
         l[rt] = 0.0f;
     }
 
-    const uint8_t* kb = a.k + size_t(kvh) * a.rows * ROWB;
-    const uint8_t* vb = a.v + size_t(kvh) * a.rows * ROWB;
-    const float* ksb = EIGHT ? a.ks + size_t(kvh) * a.rows : nullptr;
-    const float* vsb = EIGHT ? a.vs + size_t(kvh) * a.rows : nullptr;
-
-    auto load_at = [&](typename W::Raw& t, int base, auto row) __attribute__((always_inline)) {   // row(i): row i of the tile, as one that is there
-        const uint8_t* kt = kb + size_t(base) * ROWB;
-        const uint8_t* vt = vb + size_t(base) * ROWB;
+    // K of the next tile is requested when this one's scores stand, V when its product does: each has the other half of the
+    // step to arrive, and no second set of registers.
+    for (int tile = first + wave; tile < last; tile += WAVES) {
+        const int base = tile * TKEYS, next = min(tile + WAVES, last - 1);
+        const bool tail = base + TKEYS > pos;   // the tile reaches into the tree, or past the last row
+        // ---- scores
+        f32x4 s[RT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int u = 0; u < KL; ++u) t.k[h][u] = *reinterpret_cast<const u32x4*>(kt + unsigned(row(16 * h + ln) * ROWB + 64 * u + 16 * g));
+        for (int sl = 0; sl < SLICES; ++sl)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint8_t* p = vt + unsigned(row(16 * (e / 4) + 4 * g + e % 4) * ROWB + ROWB / 16 * ln);
-            if constexpr (VW == 1) {
-                t.v[e][0] = *reinterpret_cast<const uint32_t*>(p);
-            } else if constexpr (VW == 2) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-                t.v[e][0] = w[0];
-                t.v[e][1] = w[1];
-            } else {
-#pragma unroll
-                for (int u = 0; u < VW / 4; ++u) {
-                    const u32x4 w = *reinterpret_cast<const u32x4*>(p + 16 * u);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t.v[e][4 * u + i] = w[i];
-                }
-            }
-        }
-    };
-    auto load = [&](typename W::Raw& t, int tile) __attribute__((always_inline)) {
-        const int base = tile * TKEYS;
-        if (base + TKEYS <= n) {
-            load_at(t, base, [](int i) { return i; });
-            if constexpr (EIGHT) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4u a4 = *reinterpret_cast<const f32x4u*>(ksb + base + 16 * h + 4 * g), b4 = *reinterpret_cast<const f32x4u*>(vsb + base + 16 * h + 4 * g);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        t.ks[4 * h + r] = a4[r];
-                        t.vs[4 * h + r] = b4[r];
-                    }
-                }
-            }
-        } else {   // the last tile: rows behind the last one are not read
-            const auto there = [&](int i) { return min(i, n - 1 - base); };
-            load_at(t, base, there);
-            if constexpr (EIGHT) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = base + there(16 * (e / 4) + 4 * g + e % 4);
-                    t.ks[e] = ksb[at];
-                    t.vs[e] = vsb[at];
-                }
-            }
-        }
-    };
-
-    auto work = [&](typename W::Raw& t, int tile, auto tail) __attribute__((always_inline)) {
-        constexpr bool TAIL = decltype(tail)::value;   // the tile reaches into the tree, or past the last row
-        const int base = tile * TKEYS;
-        // ---- scores, in powers of two
-        float x[RT][8], iv[8];
-        {
-            f32x4 s[RT][2];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int sl = 0; sl < SLICES; ++sl)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    bf16x8 kf;
-                    if constexpr (EIGHT) {
-                        const uint32_t w0 = t.k[h][sl / 2][2 * (sl & 1)], w1 = t.k[h][sl / 2][2 * (sl & 1) + 1];
-                        const u32x4 p = {perm(byte_f32<1>(w0), byte_f32<0>(w0), 0x07060302u), perm(byte_f32<3>(w0), byte_f32<2>(w0), 0x07060302u),
-                                         perm(byte_f32<1>(w1), byte_f32<0>(w1), 0x07060302u), perm(byte_f32<3>(w1), byte_f32<2>(w1), 0x07060302u)};
-                        kf = __builtin_bit_cast(bf16x8, p);
-                    } else {
-                        kf = __builtin_bit_cast(bf16x8, t.k[h][sl]);
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][sl], s[rt][h], 0, 0, 0);
-                }
-            float kscale[8], lv[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                kscale[e] = EIGHT ? t.ks[e] * a.scale : a.scale;
+            for (int h = 0; h < 2; ++h) {
+                bf16x8 kf;
                 if constexpr (EIGHT) {
-                    // a row of zeros (scale 0) counts in the denominator alone
-                    t.vs[e] = t.vs[e] == 0.0f ? 1.0f : t.vs[e];
-                    lv[e] = __builtin_amdgcn_logf(t.vs[e]);
-                    iv[e] = __builtin_amdgcn_rcpf(t.vs[e]);
-                    if constexpr (TAIL) iv[e] = iv[e] == iv[e] ? iv[e] : 1.0f;   // (0 times NaN: the nodes that do not see the row)
+                    const uint32_t w0 = kr[h][sl / 2][2 * (sl & 1)], w1 = kr[h][sl / 2][2 * (sl & 1) + 1];
+                    const u32x4 p = {perm(byte_f32<1>(w0), byte_f32<0>(w0), 0x07060302u), perm(byte_f32<3>(w0), byte_f32<2>(w0), 0x07060302u),
+                                     perm(byte_f32<1>(w1), byte_f32<0>(w1), 0x07060302u), perm(byte_f32<3>(w1), byte_f32<2>(w1), 0x07060302u)};
+                    kf = __builtin_bit_cast(bf16x8, p);
+                } else {
+                    kf = __builtin_bit_cast(bf16x8, kr[h][sl]);
                 }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[rt][sl], s[rt][h], 0, 0, 0);
             }
+        const float scales = sc;
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- in powers of two; masked
+        float x[RT][8], inverse = 0.0f;
+        if constexpr (EIGHT) {
+            const float vscale = scales == 0.0f && ln >= 8 ? 1.0f : scales;   // a row of zeros (scale 0) counts in the denominator alone
+            const float both = ln < 8 ? scales * a.scale : __builtin_amdgcn_logf(vscale);
+            inverse = __builtin_amdgcn_rcpf(vscale);
+            inverse = inverse == inverse ? inverse : 1.0f;   // (0 times NaN: the nodes that do not see the row)
+            for_eight([&](auto e) __attribute__((always_inline)) {
+                constexpr int E = decltype(e)::value;
+                const float k = row_lane<E>(both), lv = row_lane<8 + E>(both);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) x[rt][E] = __builtin_fmaf(s[rt][E / 4][E % 4], k, lv);
+            }, std::make_integer_sequence<int, 8>{});
+        } else {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[rt][e] = EIGHT ? __builtin_fmaf(s[rt][e / 4][e % 4], kscale[e], lv[e]) : s[rt][e / 4][e % 4] * kscale[e];
-                    if constexpr (TAIL) {
-                        const int key = base + 16 * (e / 4) + 4 * g + e % 4, j = key - pos;
-                        const bool vis = j < 0 || (j < a.T && (seen[rt] >> (j & 63) & 1));
-                        x[rt][e] = vis ? x[rt][e] : NEG;
-                    }
-                }
+                for (int e = 0; e < 8; ++e) x[rt][e] = s[rt][e / 4][e % 4] * a.scale;
+        }
+        if (tail) {
+            const int below = pos - base;   // rows of the tile before the tree (negative: rows of the tree before the tile, up to 63)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {   // bit k: key k of the tile is seen; shifted to the lane's first key
+                const uint32_t window = uint32_t(below > 0 ? seen[rt] << below | ((1ull << below) - 1) : seen[rt] >> -below) >> (4 * g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[rt][e] = window & (1u << (16 * (e / 4) + e % 4)) ? x[rt][e] : NEG;
+            }
         }
         // ---- the reference moves where a score passes it
         bool any = false;
@@ -275,10 +299,7 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
         for (int rt = 0; rt < RT; ++rt) {
             const float shift = m[rt] == NEG ? 0.0f : m[rt];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[rt][e] = __builtin_amdgcn_exp2f(x[rt][e] - shift);
-                if constexpr (EIGHT) l[rt] = __builtin_fmaf(x[rt][e], iv[e], l[rt]);
-            }
+            for (int e = 0; e < 8; ++e) x[rt][e] = __builtin_amdgcn_exp2f(x[rt][e] - shift);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (EIGHT) {
@@ -289,23 +310,39 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
                 }
             }
         }
+        if constexpr (EIGHT) {
+            for_eight([&](auto e) __attribute__((always_inline)) {
+                constexpr int E = decltype(e)::value;
+                const float iv = row_lane<8 + E>(inverse);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) l[rt] = __builtin_fmaf(x[rt][E], iv, l[rt]);
+            }, std::make_integer_sequence<int, 8>{});
+        }
         // ---- the tree's rows in bf16: a row that is not finite must not reach (0 times infinity) the queries that do not see it
-        if constexpr (TAIL && !EIGHT) {
-            uint32_t bad = 0;
+        if (!EIGHT && tail) {
+            uint32_t odd[8], any_odd = 0;   // not zero: some value of the row is an infinity or NaN (the exponent's carry)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int j = base + 16 * (e / 4) + 4 * g + e % 4 - pos;
-                bool odd = false;
+                odd[e] = 0;
 #pragma unroll
-                for (int w = 0; w < VW; ++w) odd |= (t.v[e][w] & 0x7F80u) == 0x7F80u || (t.v[e][w] & 0x7F800000u) == 0x7F800000u;
-                const bool gone = j >= a.T;   // behind the last row: a copy of that
-                const uint64_t b = __builtin_amdgcn_ballot_w64(odd && j >= 0 && !gone);
-                const uint32_t of = uint32_t((b & 0xFFFFu) != 0) | uint32_t((b >> 16 & 0xFFFFu) != 0) << 1 | uint32_t((b >> 32 & 0xFFFFu) != 0) << 2 |
-                                    uint32_t((b >> 48) != 0) << 3;
-                bad |= of << (4 * e);
-                if (gone || (of >> g & 1)) {
+                for (int w = 0; w < VW; ++w) {
+                    odd[e] |= (vr[e][w] & 0x7F807F80u) + 0x00800080u;
+                    vr[e][w] = j < a.T ? vr[e][w] : 0;   // behind the last row: a copy of that
+                }
+                odd[e] = j >= 0 && j < a.T ? odd[e] & 0x80008000u : 0;
+                any_odd |= odd[e];
+            }
+            uint32_t bad = 0;
+            if (__builtin_amdgcn_ballot_w64(any_odd != 0)) {
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) t.v[e][w] = 0;
+                for (int e = 0; e < 8; ++e) {
+                    const uint64_t b = __builtin_amdgcn_ballot_w64(odd[e] != 0);
+                    const uint32_t of = uint32_t((b & 0xFFFFu) != 0) | uint32_t((b >> 16 & 0xFFFFu) != 0) << 1 | uint32_t((b >> 32 & 0xFFFFu) != 0) << 2 |
+                                        uint32_t((b >> 48) != 0) << 3;
+                    bad |= of << (4 * e);
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) vr[e][w] = of >> g & 1 ? 0 : vr[e][w];
                 }
             }
             if (bad) {   // rare: those rows by hand, for the queries that see them; their weights through LDS, which is free here
@@ -337,15 +374,20 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
             for (int rt = 0; rt < RT; ++rt)
                 ones[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, pf[rt]), ones[rt], 0, 0, 0);
         }
+        uint32_t pairs[2][4];   // 8 bits: bytes 0, 1 and 2, 3 of a word of two rows, side by side
 #pragma unroll
         for (int i = 0; i < DPL; ++i) {
             u32x4 w;
             if constexpr (EIGHT) {
-                // bytes i of two rows, biased by 128, beside 0x64: half precision 1024 + 128 + code
+                // half precision 1024 + 128 + code: the code biased by 128 beside the byte 0x64
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t lo = t.v[2 * e][i / 4] ^ 0x80808080u, hi = t.v[2 * e + 1][i / 4] ^ 0x80808080u;
-                    const uint32_t two = perm(hi, lo, 0x0C000C00u | uint32_t(i % 4) | uint32_t(4 + i % 4) << 16) | 0x64006400u;
+                    if (i % 4 == 0) {
+                        const uint32_t lo = vr[2 * e][i / 4] ^ 0x80808080u, hi = vr[2 * e + 1][i / 4] ^ 0x80808080u;
+                        pairs[0][e] = perm(hi, lo, 0x05010400u);
+                        pairs[1][e] = perm(hi, lo, 0x07030602u);
+                    }
+                    const uint32_t two = perm(0x64646464u, pairs[i % 4 / 2][e], i % 2 ? 0x04030402u : 0x04010400u);
                     w[e] = __builtin_bit_cast(uint32_t, half2_t(__builtin_bit_cast(half2_t, two) - half2_t{_Float16(1152.0f), _Float16(1152.0f)}));
                 }
 #pragma unroll
@@ -353,31 +395,19 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
                     o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, pf[rt]), o[rt][i], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = perm(t.v[2 * e + 1][i / 2], t.v[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                for (int e = 0; e < 4; ++e) w[e] = perm(vr[2 * e + 1][i / 2], vr[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
                     o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, pf[rt]), o[rt][i], 0, 0, 0);
             }
         }
-    };
-    typename W::Raw even, odd;
-    int tile = first + wave;
-    if (tile < last) load(even, tile);
-    const int full = min(last, pos / TKEYS);   // tiles below this one are rows that every node sees
-    while (tile + TWAVES < full) {
-        load(odd, tile + TWAVES);
-        work(even, tile, std::false_type{});
-        tile += 2 * TWAVES;
-        if (tile < last) load(even, tile);
-        work(odd, tile - TWAVES, std::false_type{});
-    }
-    for (; tile < last; tile += TWAVES) {   // up to one more of those, and the ones that reach into the tree
-        if (tile + TWAVES < last) load(odd, tile + TWAVES);
-        work(even, tile, std::true_type{});
-        even = odd;
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(next);
+        __builtin_amdgcn_sched_barrier(0);
     }
 
-    // ---- the waves meet
+    // ---- the waves meet: their references first, so that what they leave in LDS only has to be added
+    float den[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if constexpr (EIGHT) {
@@ -386,96 +416,123 @@ __global__ __launch_bounds__(TNT, 1) void attn_tree_kernel(const TreeArgs a) {
         } else {
             l[rt] = ones[rt][0];
         }
-        const int r = 16 * rt + ln;
-        if (g == 0) {
-            s_m[wave][r] = m[rt];
-            s_l[wave][r] = l[rt];
-        }
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4)
-#pragma unroll
-            for (int i = 0; i < DPL; i += 4)
-                *reinterpret_cast<f32x4*>(&s_o[wave][r][DPL * (4 * g + q4) + i]) = f32x4{o[rt][i][q4], o[rt][i + 1][q4], o[rt][i + 2][q4], o[rt][i + 3][q4]};
+        if (g == 0) s_ml[wave][16 * rt + ln] = float2{m[rt], l[rt]};
     }
     __syncthreads();
-    for (int c = tid; c < W::ROWS * (D / 4); c += TNT) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = 16 * rt + ln;
+        float2 ml[WAVES];
+        float mx = NEG;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            ml[w] = s_ml[w][r];
+            mx = fmaxf(mx, ml[w].x);
+        }
+        den[rt] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)   // (l is 0 of a wave whose keys the query does not see)
+            if (ml[w].y != 0.0f) den[rt] = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[w].x - mx), ml[w].y, den[rt]);
+        float f = l[rt] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - mx);
+        if (whole) f *= den[rt] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den[rt]);   // (0: nothing was seen)
+        else if (wave == 0 && g == 0 && row0 + r < rows_all)
+            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, den[rt]};
+        if (row0 + r < rows_all) {
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+                for (int i = 0; i < DPL; i += 4)
+                    *reinterpret_cast<f32x4*>(&s_o[wave][r][DPL * (4 * g + q4) + i]) =
+                        f32x4{o[rt][i][q4] * f, o[rt][i + 1][q4] * f, o[rt][i + 2][q4] * f, o[rt][i + 3][q4] * f};
+        }
+    }
+    __syncthreads();
+    for (int c = tid; c < ROWS * (D / 4); c += NT) {
         const int r = c / (D / 4), e = c % (D / 4) * 4;
         if (row0 + r >= rows_all) break;
-        float mx = s_m[0][r];
+        f32x4 v[WAVES];
 #pragma unroll
-        for (int w = 1; w < TWAVES; ++w) mx = fmaxf(mx, s_m[w][r]);
-        f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
-        float den = 0.0f;
+        for (int w = 0; w < WAVES; ++w) v[w] = *reinterpret_cast<const f32x4*>(&s_o[w][r][e]);
 #pragma unroll
-        for (int w = 0; w < TWAVES; ++w) {
-            if (s_l[w][r] == 0.0f) continue;   // a wave whose keys the query does not see
-            const float f = __builtin_amdgcn_exp2f(s_m[w][r] - mx);
-            const f32x4 v = *reinterpret_cast<const f32x4*>(&s_o[w][r][e]);
+        for (int w = 1; w < WAVES; ++w)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(f, v[i], num[i]);
-            den = __builtin_fmaf(f, s_l[w][r], den);
-        }
+            for (int i = 0; i < 4; ++i) v[0][i] += v[w][i];
         const size_t at = out_row(row0 + r);
-        if (whole) {
-            const float inv = den == 0.0f ? 0.0f : 1.0f / den;   // (0: nothing was seen)
-            const u32x2 w = {f32_to_bf16x2(num[0] * inv, num[1] * inv), f32_to_bf16x2(num[2] * inv, num[3] * inv)};
-            *reinterpret_cast<u32x2*>(a.out + at * D + e) = w;
-        } else {
-            const size_t all = size_t(a.T) * a.hq, slot = size_t(range) * all + at;
-            *reinterpret_cast<f32x4*>(a.part + slot * D + e) = num;
-            if (e == 0) {
-                float* ml = a.part + size_t(a.splits) * all * D + 2 * slot;
-                ml[0] = mx;
-                ml[1] = den;
-            }
-        }
+        if (whole) *reinterpret_cast<u32x2*>(a.out + at * D + e) = u32x2{f32_to_bf16x2(v[0][0], v[0][1]), f32_to_bf16x2(v[0][2], v[0][3])};
+        else *reinterpret_cast<f32x4*>(a.part + (at * a.splits + range) * D + e) = v[0];
     }
 }
 
-// Joins the ranges of each row of [T, hq]: D / 4 lanes a row.
-template <int D>
-__global__ __launch_bounds__(TNT) void attn_tree_join_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
-                                                             int splits, const int64_t* pos_dev, int64_t pos0) {
+// Joins the ranges of one row of [T, hq], a workgroup: D / 4 lanes a range, the ranges dealt to the rest.  Bound by one trip to memory:
+// all that a thread reads is requested at once.  RANGES: at most.
+template <int D, int RANGES>
+__global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
+                                                             int splits, int waves, const int64_t* pos_dev, int64_t pos0) {
+    constexpr int PARTS = JNT / (D / 4), PER = (RANGES + PARTS - 1) / PARTS;
+    __shared__ float s_num[PARTS][D];
+    const int lane = threadIdx.x & 63, p = threadIdx.x / (D / 4), e = threadIdx.x % (D / 4) * 4;
+    const float* num0 = part + size_t(blockIdx.x) * splits * D + e;
+    const float2 ml = reinterpret_cast<const float2*>(part + size_t(T) * hq * splits * D)[size_t(blockIdx.x) * splits + min(lane, splits - 1)];
+    f32x4 v[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
     const int64_t pos = pos_dev ? pos_dev[0] : pos0;
     if (pos < 0 || pos > int64_t(rows) - T) return;   // zeros, written
-    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
-    const size_t all = size_t(T) * hq, row = size_t(blockIdx.x) * (TNT / (D / 4)) + threadIdx.x / (D / 4);
-    if (ranges == 1 || row >= all) return;
-    const int e = threadIdx.x % (D / 4) * 4;
-    const float* ml = part + size_t(splits) * all * D + 2 * row;
-    constexpr float NEG = -__builtin_inff();
-    float mx = NEG;
-    for (int s = 0; s < ranges; ++s) mx = fmaxf(mx, ml[2 * s * all]);
+    const int n = int(pos) + T, per = range_tiles(n, splits, waves), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
+    if (ranges == 1) return;
+    const bool mine = lane < ranges && ml.y != 0.0f;   // (0: a range of which the query sees nothing)
+    const float mx = wave_max(mine ? ml.x : -__builtin_inff()), w = mine ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
+    const float den = wave_sum(mine ? w * ml.y : 0.0f);
     f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
-    float den = 0.0f;
-    for (int s = 0; s < ranges; ++s) {
-        const float l = ml[2 * s * all + 1], w = __builtin_amdgcn_exp2f(ml[2 * s * all] - mx);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(part + (s * all + row) * D + e);
-        if (l == 0.0f) continue;   // a range of which the query sees nothing
 #pragma unroll
-        for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(w, v[i], num[i]);
-        den = __builtin_fmaf(w, l, den);
+    for (int u = 0; u < PER; ++u) {
+        const float f = __shfl(w, min(p + u * PARTS, 63), WAVE);
+        const float there = __shfl(mine ? 1.0f : 0.0f, min(p + u * PARTS, 63), WAVE);
+        if (there != 0.0f && p + u * PARTS < 64) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(f, v[u][i], num[i]);
+        }
     }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-    const u32x2 w = {f32_to_bf16x2(num[0] * inv, num[1] * inv), f32_to_bf16x2(num[2] * inv, num[3] * inv)};
-    *reinterpret_cast<u32x2*>(out + row * D + e) = w;
+    *reinterpret_cast<f32x4*>(&s_num[p][e]) = num;
+    __syncthreads();
+    if (int(threadIdx.x) >= D / 2) return;
+    float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+        lo += s_num[q][2 * threadIdx.x];
+        hi += s_num[q][2 * threadIdx.x + 1];
+    }
+    const float inv = den == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den);
+    *reinterpret_cast<uint32_t*>(out + size_t(blockIdx.x) * D + 2 * threadIdx.x) = f32_to_bf16x2(lo * inv, hi * inv);
 }
 
 template <int D, int RT>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
     const unsigned combos = unsigned(a.hk) * a.splits, grid = (combos + TXCDS - 1) / TXCDS * TXCDS * a.blocks;
-    if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(TNT), 0, st>>>(a);
-    else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(TNT), 0, st>>>(a);
-    if (a.splits > 1) {
-        constexpr int PER = TNT / (D / 4);
-        attn_tree_join_kernel<D><<<dim3((unsigned(a.T) * a.hq + PER - 1) / PER), dim3(TNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev,
-                                                                                                  a.pos0);
-    }
+    if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(64 * tree_waves(D, a.ks)), 0, st>>>(a);
+    else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(64 * tree_waves(D, a.ks)), 0, st>>>(a);
+    if (a.splits == 1) return;
+    const auto join = [&](auto ranges) {
+        attn_tree_join_kernel<D, decltype(ranges)::value><<<dim3(unsigned(a.T) * a.hq), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, tree_waves(D, a.ks), a.pos_dev,
+                                                                                                        a.pos0);
+    };
+    if (a.splits <= 16) join(std::integral_constant<int, 16>{});
+    else join(std::integral_constant<int, 64>{});
 }
 
 }  // namespace scmx
 
 using namespace scmx;
+
+// 16-row blocks of queries a wave: two where there are that many rows and its registers hold them.
+static int tree_blocks(int qrows, int d) { return qrows <= 16 || d == 256 ? 1 : 2; }
+
+extern "C" int scmx_attn_tree_splits(int T, int n, int hq, int hk, int d) {
+    if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
+    const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), keys = (d == 256 ? 4 : 8) * TKEYS;
+    const int64_t combos = int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)), most = 256 / combos, ranges = (int64_t(n) + keys - 1) / keys;
+    return n <= 2 * keys || most < 1 ? 1 : int(ranges < most ? (ranges < 64 ? ranges : 64) : most < 64 ? most : 64);
+}
 
 extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
                               const int64_t* mask, const int64_t* pos_dev, int64_t pos0, uint16_t* out, int T, int hq, int hk, int d,
@@ -484,8 +541,9 @@ extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void*
         set_error("attn_tree: null pointer argument (an 8-bit cache has both scales, a bf16 one none)");
         return SCMX_ERR_ARG;
     }
-    if (T < 1 || T > 64 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || cache_rows < T) {
-        set_error("attn_tree: need 1..64 nodes, hq %% hk == 0 and a cache that holds the tree (T=%d hq=%d hk=%d rows=%d)", T, hq, hk, cache_rows);
+    if (T < 1 || T > 64 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || hq / hk > 4096 || cache_rows < T) {
+        set_error("attn_tree: need 1..64 nodes, hq %% hk == 0, up to 4096 query heads a KV head and a cache that holds the tree (T=%d hq=%d hk=%d rows=%d)", T, hq,
+                  hk, cache_rows);
         return SCMX_ERR_ARG;
     }
     if (d != 64 && d != 128 && d != 256) {
@@ -510,16 +568,14 @@ extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void*
     }
     const int qrows = T * (hq / hk);
     TreeArgs a{q, static_cast<const uint8_t*>(kcache), static_cast<const uint8_t*>(vcache), kscale, vscale, mask, pos_dev, pos0, out, workspace,
-               T, hq, hk, cache_rows, splits, 0, scale * 1.4426950408889634f};
-    // query rows a wave: as many as there are, up to what its registers hold (64 rows of 128, 32 of 256)
-    const int rt = qrows <= 16 ? 1 : qrows <= 32 || d == 256 ? 2 : 4;
+               T, hq, hk, cache_rows, splits, 0, uint32_t(((uint64_t(1) << 32) + hq / hk - 1) / uint64_t(hq / hk)), scale * 1.4426950408889634f};
+    const int rt = tree_blocks(qrows, d);
     a.blocks = (qrows + 16 * rt - 1) / (16 * rt);
     const hipStream_t st = (hipStream_t)stream;
     const auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         if (rt == 1) launch_tree<D, 1>(a, st);
-        else if (rt == 2) launch_tree<D, 2>(a, st);
-        else if constexpr (D < 256) launch_tree<D, 4>(a, st);
+        else if constexpr (D < 256) launch_tree<D, 2>(a, st);
     };
     if (d == 64) go(std::integral_constant<int, 64>{});
     else if (d == 128) go(std::integral_constant<int, 128>{});

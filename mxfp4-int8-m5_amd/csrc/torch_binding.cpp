@@ -1,5 +1,5 @@
 // Python binding of the C ABI for torch tensors: `_binding`, a module whose functions are the entry points of
-// include/scmx.h and scmx_cache.h that enqueue work (and five of their queries), under the same names and with the same arguments except the
+// include/scmx.h and scmx_cache.h that enqueue work (and six of their queries), under the same names and with the same arguments except the
 // last.  A pointer argument takes a tensor (contiguous, on the GPU), None or an integer address; a format argument an object
 // whose buffer is the scmx_format; the stream is the caller's current one and is not passed.  A negative status raises.
 //
@@ -10,12 +10,17 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <exception>
+#include <initializer_list>
 #include <tuple>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 #include "../../include/scmx_cache.h"
 
@@ -235,9 +240,235 @@ PyObject* gemv(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
+// ---- drafted tokens over a cache: sc_cache's and sc_draft's functions for the operands of every step, in one call as above ---------
+// (None where an operand is anything else: the caller's general way converts or refuses it.  16 tokens through 28 blocks'
+// caches, host time: 314 us with checks and allocations in Python, see sc_cache, 121 here.)
+
+// A contiguous tensor of `type` on the current device; NULL: something else.  None is not one.
+const at::Tensor* local(PyObject* o, at::ScalarType type) {
+    const at::Tensor* t = plain(o, type);
+    return t && t->get_device() == c10::hip::current_device() ? t : nullptr;
+}
+
+struct CacheTensors {
+    const at::Tensor *k, *v, *ks = nullptr, *vs = nullptr;
+    int64_t hk, rows, d;
+    float* scale(const at::Tensor* t) const { return t ? static_cast<float*>(t->data_ptr()) : nullptr; }
+};
+bool cache_of(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, CacheTensors& c) {
+    const bool eight = ks != Py_None;
+    const at::ScalarType type = eight ? at::ScalarType::Char : at::ScalarType::BFloat16;
+    c.k = local(k, type);
+    c.v = local(v, type);
+    if (!c.k || !c.v || c.k->dim() != 3 || c.k->sizes() != c.v->sizes() || eight != (vs != Py_None)) return false;
+    c.hk = c.k->size(0);
+    c.rows = c.k->size(1);
+    c.d = c.k->size(2);
+    if (eight) {
+        c.ks = local(ks, at::ScalarType::Float);
+        c.vs = local(vs, at::ScalarType::Float);
+        if (!c.ks || !c.vs) return false;
+        for (const at::Tensor* t : {c.ks, c.vs})
+            if (t->dim() != 2 || t->size(0) != c.hk || t->size(1) != c.rows) return false;
+    }
+    return c.hk <= INT32_MAX && c.rows <= INT32_MAX && c.d <= INT32_MAX;
+}
+// A position: an integer, or an int64 tensor of one value.
+bool position_of(PyObject* o, const int64_t*& dev, int64_t& at) {
+    dev = nullptr;
+    at = 0;
+    if (PyLong_CheckExact(o)) {
+        at = as_int(o);
+        return true;
+    }
+    const at::Tensor* t = local(o, at::ScalarType::Long);
+    if (!t || t->numel() != 1) return false;
+    dev = static_cast<const int64_t*>(t->data_ptr());
+    return true;
+}
+// None, or such a tensor of n values.
+template <typename T>
+bool optional_of(PyObject* o, at::ScalarType type, int64_t n, const T*& p) {
+    p = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor* t = local(o, type);
+    if (!t || t->numel() != n) return false;
+    p = static_cast<const T*>(t->data_ptr());
+    return true;
+}
+bool ints_of(PyObject* const* args, std::initializer_list<int> at) {
+    for (int i : at)
+        if (!PyLong_CheckExact(args[i])) return false;
+    return true;
+}
+at::TensorOptions like(const at::Tensor& t, at::ScalarType type) { return at::TensorOptions().dtype(type).device(t.device()); }
+void* stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+// cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, kscale, vscale, depth)
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 15) fail(PyExc_TypeError, "cache_write takes 15 arguments");
+        CacheTensors c;
+        const int64_t* dev;
+        int64_t pos;
+        const int32_t* depth;
+        if (!ints_of(args, {4, 5, 6, 7}) || !PyFloat_Check(args[3]) || !cache_of(args[8], args[9], args[12], args[13], c) || !position_of(args[10], dev, pos))
+            Py_RETURN_NONE;
+        const int64_t L = as_int(args[4]), hq = as_int(args[5]), hk = as_int(args[6]), d = as_int(args[7]);
+        const at::Tensor *y = local(args[0], at::ScalarType::BFloat16), *qn = local(args[1], at::ScalarType::BFloat16), *kn = local(args[2], at::ScalarType::BFloat16),
+                         *freq = local(args[11], at::ScalarType::Float);
+        if (!y || !qn || !kn || !freq || L < 0 || L > INT32_MAX || hq < 1 || hq > 65535 || hk != c.hk || d != c.d || y->dim() != 2 || y->size(0) < L ||
+            y->size(1) != (hq + 2 * hk) * d || qn->numel() != d || kn->numel() != d || freq->numel() != d / 2 || !optional_of(args[14], at::ScalarType::Int, L, depth))
+            Py_RETURN_NONE;
+        at::Tensor q;
+        int rc;
+        {
+            const NoGil released;
+            q = at::empty_strided({hq, L, d}, {d, hq * d, 1}, like(*y, at::ScalarType::BFloat16));
+            const auto bf = [](const at::Tensor* t) { return static_cast<const uint16_t*>(t->data_ptr()); };
+            rc = scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), float(PyFloat_AS_DOUBLE(args[3])), static_cast<uint16_t*>(q.data_ptr()), c.k->data_ptr(),
+                                  c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), int(L), int(hq), int(hk), int(d), static_cast<const float*>(freq->data_ptr()), depth, dev, pos,
+                                  int(c.rows), stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_cache_write", rc);
+        return THPVariable_Wrap(std::move(q));
+    } catch (...) {
+        return raised();
+    }
+}
+
+// attn_tree(q, kcache, vcache, pos, mask, kscale, vscale, scale, splits)
+PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 9) fail(PyExc_TypeError, "attn_tree takes 9 arguments");
+        CacheTensors c;
+        const int64_t *dev, *mask;
+        int64_t pos;
+        if (!THPVariable_Check(args[0]) || !cache_of(args[1], args[2], args[5], args[6], c) || !position_of(args[3], dev, pos) ||
+            (args[7] != Py_None && !PyFloat_Check(args[7])) || (args[8] != Py_None && !PyLong_CheckExact(args[8])))
+            Py_RETURN_NONE;
+        const at::Tensor& q = THPVariable_Unpack(args[0]);
+        if (!q.is_cuda() || q.get_device() != c10::hip::current_device() || q.scalar_type() != at::ScalarType::BFloat16 || q.dim() != 3) Py_RETURN_NONE;
+        const int64_t hq = q.size(0), T = q.size(1), d = q.size(2);   // the view of [T, hq, d] storage
+        if (T < 1 || T > 64 || hq < 1 || hq > 65535 || d != c.d || c.hk < 1 || hq % c.hk || c.rows < T || q.stride(2) != 1 || (hq > 1 && q.stride(0) != d) ||
+            (T > 1 && q.stride(1) != hq * d) || !optional_of(args[4], at::ScalarType::Long, T, mask) || pos < 0 || pos > INT32_MAX - 64)
+            Py_RETURN_NONE;
+        const int splits = args[8] != Py_None ? convert<int>(args[8]) : scmx_attn_tree_splits(int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
+        if (splits < 1 || splits > 64) Py_RETURN_NONE;
+        const float scale = args[7] == Py_None ? float(1.0 / std::sqrt(double(d))) : float(PyFloat_AS_DOUBLE(args[7]));
+        at::Tensor out, work;
+        int rc;
+        {
+            const NoGil released;
+            out = at::empty({T, hq * d}, like(q, at::ScalarType::BFloat16));
+            if (splits > 1) work = at::empty({splits * T * hq * (d + 2)}, like(q, at::ScalarType::Float));
+            rc = scmx_attn_tree(static_cast<const uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), mask, dev, pos,
+                                static_cast<uint16_t*>(out.data_ptr()), int(T), int(hq), int(c.hk), int(d), int(c.rows), scale,
+                                splits > 1 ? static_cast<float*>(work.data_ptr()) : nullptr, splits, stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_attn_tree", rc);
+        return THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        return raised();
+    }
+}
+
+// cache_read(kcache, vcache, kscale, vscale, n, row0)
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 6) fail(PyExc_TypeError, "cache_read takes 6 arguments");
+        CacheTensors c;
+        if (args[2] == Py_None || !ints_of(args, {4, 5}) || !cache_of(args[0], args[1], args[2], args[3], c)) Py_RETURN_NONE;
+        const int64_t rows = as_int(args[4]), row0 = as_int(args[5]);
+        if (rows < 0 || row0 < 0 || row0 > INT32_MAX || rows > c.rows) Py_RETURN_NONE;
+        at::Tensor k, v;
+        int rc;
+        {
+            const NoGil released;
+            k = at::empty({c.hk, rows, c.d}, like(*c.k, at::ScalarType::BFloat16));
+            v = at::empty({c.hk, rows, c.d}, like(*c.k, at::ScalarType::BFloat16));
+            rc = scmx_cache_read(static_cast<const int8_t*>(c.k->data_ptr()), static_cast<const int8_t*>(c.v->data_ptr()), c.scale(c.ks), c.scale(c.vs),
+                                 static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()), int(c.hk), int(c.d), int(c.rows), int(row0), int(rows), stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_cache_read", rc);
+        PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
+        return Py_BuildValue("(NN)", pk, pv);
+    } catch (...) {
+        return raised();
+    }
+}
+
+// cache_keep(caches, path, count, pos): True, or None
+PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 4) fail(PyExc_TypeError, "cache_keep takes 4 arguments");
+        const at::Tensor *path = local(args[1], at::ScalarType::Int), *count = local(args[2], at::ScalarType::Int);
+        const int64_t* dev;
+        int64_t pos;
+        if (!PyList_CheckExact(args[0]) || !path || !count || count->numel() != 1 || path->numel() > 64 || !position_of(args[3], dev, pos)) Py_RETURN_NONE;
+        const Py_ssize_t layers = PyList_GET_SIZE(args[0]);
+        std::vector<uint64_t> pointers;
+        pointers.reserve(size_t(layers) * 4);
+        CacheTensors c, first{};
+        for (Py_ssize_t i = 0; i < layers; ++i) {
+            PyObject* t = PyList_GET_ITEM(args[0], i);
+            if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 4) Py_RETURN_NONE;
+            c = CacheTensors();
+            if (!cache_of(PyTuple_GET_ITEM(t, 0), PyTuple_GET_ITEM(t, 1), PyTuple_GET_ITEM(t, 2), PyTuple_GET_ITEM(t, 3), c)) Py_RETURN_NONE;
+            if (i == 0) first = c;
+            else if (c.hk != first.hk || c.rows != first.rows || c.d != first.d || !c.ks != !first.ks) Py_RETURN_NONE;
+            for (const at::Tensor* x : {c.k, c.v, c.ks, c.vs})
+                if (x) pointers.push_back(reinterpret_cast<uintptr_t>(x->data_ptr()));
+        }
+        if (layers < 1 || layers > 1024) Py_RETURN_NONE;
+        const int rc = scmx_cache_keep(pointers.data(), int(layers), first.ks != nullptr, int(first.hk), int(first.d), int(first.rows),
+                                       static_cast<const int32_t*>(path->data_ptr()), static_cast<const int32_t*>(count->data_ptr()), int(path->numel()), dev, pos, stream());
+        if (rc != SCMX_OK) return status("scmx_cache_keep", rc);
+        Py_RETURN_TRUE;
+    } catch (...) {
+        return raised();
+    }
+}
+
+// verify_drafts(logits, tokens, parents, temperature, uniforms, draft, levels): what sc_draft.verify_drafts has left of its arguments
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 7) fail(PyExc_TypeError, "verify_drafts takes 7 arguments");
+        if (!THPVariable_Check(args[0]) || !PyFloat_Check(args[3]) || !PyLong_CheckExact(args[6])) Py_RETURN_NONE;
+        const bool f32 = THPVariable_Unpack(args[0]).scalar_type() == at::ScalarType::Float;
+        const at::Tensor *logits = local(args[0], f32 ? at::ScalarType::Float : at::ScalarType::BFloat16), *tokens = local(args[1], at::ScalarType::Long),
+                         *parents = local(args[2], at::ScalarType::Int);
+        if (!logits || !tokens || !parents || logits->dim() != 2) Py_RETURN_NONE;
+        const int64_t T = logits->size(0), V = logits->size(1), levels = as_int(args[6]);
+        const float *u, *draft;
+        if (T < 1 || T > 64 || V < 1 || V > INT32_MAX || levels < 0 || levels > 16 || tokens->numel() != T || parents->numel() != T ||
+            !optional_of(args[4], at::ScalarType::Float, T, u) || !optional_of(args[5], at::ScalarType::Float, T * V, draft))
+            Py_RETURN_NONE;
+        const size_t need = scmx_verify_workspace(int(T), int(V), int(levels));
+        at::Tensor path, count, next, work;
+        int rc;
+        {
+            const NoGil released;
+            path = at::empty({T}, like(*logits, at::ScalarType::Int));
+            count = at::empty({1}, like(*logits, at::ScalarType::Int));
+            next = at::empty({1}, like(*logits, at::ScalarType::Long));
+            work = at::empty({int64_t(need)}, like(*logits, at::ScalarType::Byte));
+            rc = scmx_verify_drafts(static_cast<const int64_t*>(tokens->data_ptr()), static_cast<const int32_t*>(parents->data_ptr()), logits->data_ptr(), f32, draft,
+                                    PyFloat_AS_DOUBLE(args[3]), u, static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()),
+                                    static_cast<int64_t*>(next.data_ptr()), int(T), int(V), int(levels), work.data_ptr(), need, stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_verify_drafts", rc);
+        PyObject *a = THPVariable_Wrap(std::move(path)), *b = THPVariable_Wrap(std::move(count)), *c = THPVariable_Wrap(std::move(next));
+        return Py_BuildValue("(NNN)", a, b, c);
+    } catch (...) {
+        return raised();
+    }
+}
+
 #define ENTRY(fn) \
     {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(((Call<&fn>::name = #fn), &Call<&fn>::call))), METH_FASTCALL, nullptr}
 #define QUERY(fn) {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Query<&fn>::call)), METH_FASTCALL, nullptr}
+#define FUNCTION(fn) {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&fn)), METH_FASTCALL, nullptr}
 #define EMPTY(suffix, type) \
     {"empty_" #suffix, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empty<at::ScalarType::type>)), METH_FASTCALL, nullptr}
 
@@ -259,8 +490,9 @@ PyMODINIT_FUNC PyInit__binding() {
         QUERY(scmx_linear_w4a8_workspace), QUERY(scmx_gemv_rows_workspace), QUERY(scmx_mm_w4a8_prefers_blocked),
         QUERY(scmx_moe_mm_takes_slots),
         ENTRY(scmx_cache_write), ENTRY(scmx_cache_read), ENTRY(scmx_cache_keep), ENTRY(scmx_attn_tree), ENTRY(scmx_verify_drafts),
-        QUERY(scmx_verify_workspace),
-        {"gemv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&gemv)), METH_FASTCALL, nullptr},
+        QUERY(scmx_verify_workspace), QUERY(scmx_attn_tree_splits),
+        FUNCTION(cache_write), FUNCTION(cache_read), FUNCTION(cache_keep), FUNCTION(attn_tree), FUNCTION(verify_drafts),
+        FUNCTION(gemv),
         EMPTY(bf16, BFloat16), EMPTY(i8, Char), EMPTY(u8, Byte), EMPTY(i32, Int), EMPTY(i64, Long), EMPTY(f32, Float),
         {nullptr, nullptr, 0, nullptr}};
     module_def.m_methods = methods;

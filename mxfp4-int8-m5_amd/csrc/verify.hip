@@ -38,20 +38,48 @@ struct VerifyArgs {
     float* m;          // [T][chunks]: largest logits
 };
 
-// exp(x), x <= 0, to some 1e-14: 2^n times the series of what is left, |r| <= ln 2 / 2 (r^12 / 12! = 6e-15).
-__device__ __forceinline__ double exp_neg(double x) {
-    const double n = rint(fmax(x, -700.0) * 1.4426950408889634);
-    double r = __builtin_fma(n, -0.693147180559945286, fmax(x, -700.0));
-    r = __builtin_fma(n, -2.319046813846299558e-17, r);
-    double p = 1.0 / 39916800.0;
-    constexpr double c[] = {1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
-#pragma unroll
-    for (int i = 0; i < 11; ++i) p = __builtin_fma(p, r, c[i]);
-    const double v = p * __longlong_as_double((long long)(int(n) + 1023) << 52);
+// 2^(j / 64).  The kernels copy it to LDS.
+__device__ const double EXP2_64[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+
+// exp(x), x <= 0, to some 1e-15 (2e-14 at -200): x = k ln 2 / 64 + r, |r| <= 0.0054, exp(r) by its series to r^5 (r^6 / 720 = 4e-17),
+// 2^(k / 64) from the table and the exponent.  Half of the time of the stats kernel is this arithmetic; a series to r^11 of the whole
+// fraction, without a table, took a third more instructions.
+__device__ __forceinline__ double exp_neg(double x, const double* table) {
+    const double c = fmax(x, -700.0), n = rint(c * 92.33248261893657);
+    const double r = __builtin_fma(n, -0.010830424696249145, c);
+    double p = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    const int k = int(n);
+    const double v = __longlong_as_double(__double_as_longlong(p * table[k & 63]) + ((long long)(k >> 6) << 52));
     return x < -700.0 ? 0.0 : v;
 }
 // A logit's weight relative to the largest, m: 1 for the largest itself, also where it is infinite.
-__device__ __forceinline__ double weight(float x, float m, double inv_t) { return x == m ? 1.0 : exp_neg((double(x) - double(m)) * inv_t); }
+__device__ __forceinline__ double weight(float x, float m, double inv_t, const double* table) {
+    if (!(fabsf(m) <= 3.4028234e38f)) return x == m ? 1.0 : 0.0;   // (the same for a whole row)
+    return exp_neg((double(x) - double(m)) * inv_t, table);
+}
+__device__ __forceinline__ void copy_table(double* table) {
+    if (threadIdx.x < 64) table[threadIdx.x] = EXP2_64[threadIdx.x];   // (a barrier follows before its first use)
+}
 
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -__builtin_inff(); }
 template <bool F32>
@@ -116,6 +144,8 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
     __shared__ float s_m[VNT / 64];
     __shared__ double s_z[VNT / 64];
     __shared__ int s_at[VNT / 64];
+    __shared__ double s_table[64];
+    if (!GREEDY) copy_table(s_table);
     const size_t row = blockIdx.y;
     float x[2][8], m = -__builtin_inff();
     const int v0 = blockIdx.x * VCHUNK + 8 * threadIdx.x;
@@ -151,7 +181,7 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (v0 + t * 8 * VNT + i < a.V) z += weight(x[t][i], m, a.inv_t);
+            if (v0 + t * 8 * VNT + i < a.V) z += weight(x[t][i], m, a.inv_t, s_table);
     z = group_sum64(z, s_z);
     if (threadIdx.x == 0) {
         a.m[out] = m;
@@ -171,7 +201,8 @@ __device__ __forceinline__ void next_level(double s, double& ak, double& bk) {
 template <bool F32>
 __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, int level) {
     __shared__ float s_m[VNT / 64];
-    __shared__ double s_z[VNT / 64];
+    __shared__ double s_z[VNT / 64], s_table[64];
+    copy_table(s_table);
     const int row = blockIdx.y, lane = threadIdx.x & 63;
     if (__popcll(__ballot(lane < a.T && a.parents[min(lane, a.T - 1)] == row)) < level) return;   // (the same in every wave)
     float x[2][8], q[2][8];
@@ -199,7 +230,7 @@ __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, i
     for (int c = threadIdx.x; c < a.chunks; c += VNT) m = fmaxf(m, pm[c]);
     m = group_max(m, s_m);
     double z = 0.0;
-    for (int c = threadIdx.x; c < a.chunks; c += VNT) z += pz[c] * weight(pm[c], m, a.inv_t);
+    for (int c = threadIdx.x; c < a.chunks; c += VNT) z += pz[c] * weight(pm[c], m, a.inv_t, s_table);
     double ak = 1.0 / group_sum64(z, s_z), bk = 0.0;
     for (int l = 1; l < level; ++l) {
         const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
@@ -212,7 +243,7 @@ __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, i
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (v0 + t * 8 * VNT + i < a.V) s += fmax(ak * weight(x[t][i], m, a.inv_t) - (bk + 1.0) * double(q[t][i]), 0.0);
+            if (v0 + t * 8 * VNT + i < a.V) s += fmax(ak * weight(x[t][i], m, a.inv_t, s_table) - (bk + 1.0) * double(q[t][i]), 0.0);
     s = group_sum64(s, s_z);
     if (threadIdx.x == 0) a.s[(size_t(level - 1) * a.T + row) * a.chunks + blockIdx.x] = s;
 }
@@ -232,170 +263,244 @@ __device__ __forceinline__ double group_scan(double v, double* s) {
     return v;
 }
 
-// One workgroup: the nodes' sums from the chunks', the walk (a thread, over scalars in LDS), the token after it.
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_readlane(int(b), lane), hi = __builtin_amdgcn_readlane(int(b >> 32), lane);
+    return __longlong_as_double((long long)(uint64_t(uint32_t(hi)) << 32 | uint32_t(lo)));
+}
+
+// One workgroup: the nodes' sums from the chunks', the walk, the token after it.  A chain of trips to memory and of cross-lane
+// sums: a wave takes four nodes' sums side by side, and the walk is a wave's, node c's numbers in lane c and read from there as
+// scalars (by a thread, over LDS, it took 150 cycles a node: 60 nodes 42 us in all, 8 drawn ones 21).
 template <bool F32, bool GREEDY>
 __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) {
+    constexpr int WAVES = VWALK / 64, PER = VNODES / WAVES;
     __shared__ float s_m[VNODES];
-    __shared__ double s_z[VNODES], s_e[VNODES], s_q[VNODES], s_wave[VWALK / 64];
+    __shared__ double s_z[VNODES], s_wave[WAVES], s_table[64], s_gone_e[VNODES], s_base, s_total;
+    __shared__ double s_w[GREEDY ? 1 : VNODES][64];   // the first 64 chunks' sums relative to the node's largest logit
     __shared__ double s_a[GREEDY ? 1 : VNODES][VLEVELS + 1], s_b[GREEDY ? 1 : VNODES][VLEVELS + 1];
-    __shared__ int s_best[VNODES], s_parent[VNODES], s_level[VNODES][VLEVELS + 1], s_gone[VNODES], s_last, s_lvl, s_ngone, s_lo, s_hi;
-    __shared__ int64_t s_token[VNODES];
-    __shared__ float s_u[VNODES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < a.T) {
-        s_parent[tid] = tid ? a.parents[tid] : -1;
-        s_token[tid] = a.tokens[tid];
-        if (!GREEDY) s_u[tid] = a.uniforms[tid];
+    __shared__ int s_best[VNODES], s_level[GREEDY ? 1 : VNODES][VLEVELS + 1], s_last, s_lvl, s_gones, s_chunk, s_lo, s_hi;
+    __shared__ int64_t s_gone[VNODES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (!GREEDY) copy_table(s_table);
+    // node `lane`: every wave knows the parents (it counts children), the first one the rest
+    const int parent = lane > 0 && lane < a.T ? a.parents[lane] : -1;
+    const bool node = lane > 0 && lane < a.T && parent >= 0 && parent < lane;
+    int64_t token = -1;
+    float u = 0.0f, x = 0.0f, q = 0.0f;
+    bool known = false;
+    if (wave == 0) {
+        if (node) token = a.tokens[lane];
+        known = node && token >= 0 && token < a.V;
+        if (!GREEDY) {
+            if (lane < a.T) u = a.uniforms[lane];
+            if (known) x = logit<F32>(a.logits, size_t(parent) * a.V + token);
+            if (known && a.draft) q = a.draft[size_t(parent) * a.V + token];
+        }
     }
-    __syncthreads();
-    for (int row = wave; row < a.T; row += VWALK / 64) {
-        const float* pm = a.m + size_t(row) * a.chunks;
-        float m = -__builtin_inff();
-        for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, pm[c]);
-        m = wave_max(m);
-        if (GREEDY) {
-            int at = a.V - 1;
-            for (int c = lane; c < a.chunks; c += 64)
-                if (pm[c] == m) at = min(at, reinterpret_cast<const int32_t*>(a.z)[size_t(row) * a.chunks + c]);
+    // ---- the sums of nodes wave, wave + 16, ..
+    {
+        float pm[PER], m[PER];
+        double pz[PER], z[PER];
+        int at[PER];
 #pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) at = min(at, __shfl_xor(at, off, WAVE));
-            if (lane == 0) s_best[row] = at;
-            continue;
+        for (int r = 0; r < PER; ++r) {
+            const int row = min(wave + WAVES * r, a.T - 1);
+            const size_t c = size_t(row) * a.chunks + min(lane, a.chunks - 1);
+            pm[r] = lane < a.chunks ? a.m[c] : -__builtin_inff();
+            if (GREEDY) at[r] = reinterpret_cast<const int32_t*>(a.z)[c];
+            else pz[r] = a.z[c];
+            m[r] = pm[r];
         }
-        const double* pz = a.z + size_t(row) * a.chunks;
-        double z = 0.0;
-        for (int c = lane; c < a.chunks; c += 64) z += pz[c] * weight(pm[c], m, a.inv_t);
-        z = wave_sum64(z);
-        double ak = 1.0 / z, bk = 0.0;
-        int level = 0;   // the last one that left something
-        if (lane == 0) {
-            s_m[row] = m;
-            s_z[row] = z;
-            s_a[row][0] = ak;
-            s_b[row][0] = bk;
-            s_level[row][0] = 0;
-        }
-        if (a.levels == 0) continue;
-        const int kids = min(a.levels, int(__popcll(__ballot(lane < a.T && s_parent[min(lane, a.T - 1)] == row))));
-        for (int l = 1; l <= kids; ++l) {
-            const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
-            double s = 0.0;
-            for (int c = lane; c < a.chunks; c += 64) s += ps[c];
-            s = wave_sum64(s);
-            next_level(s, ak, bk);
-            if (s > 0.0) level = l;
-            if (lane == 0) {
-                s_a[row][l] = ak;
-                s_b[row][l] = bk;
-                s_level[row][l] = level;
+        for (int c = 64 + lane; c < a.chunks; c += 64)
+#pragma unroll
+            for (int r = 0; r < PER; ++r) m[r] = fmaxf(m[r], a.m[size_t(min(wave + WAVES * r, a.T - 1)) * a.chunks + c]);
+#pragma unroll
+        for (int r = 0; r < PER; ++r) m[r] = wave_max(m[r]);
+        if (GREEDY) {
+#pragma unroll
+            for (int r = 0; r < PER; ++r) {
+                const int row = wave + WAVES * r;
+                if (row >= a.T) break;
+                int best = lane < a.chunks && pm[r] == m[r] ? at[r] : a.V - 1;
+                for (int c = 64 + lane; c < a.chunks; c += 64)
+                    if (a.m[size_t(row) * a.chunks + c] == m[r]) best = min(best, reinterpret_cast<const int32_t*>(a.z)[size_t(row) * a.chunks + c]);
+#pragma unroll
+                for (int off = 32; off >= 1; off >>= 1) best = min(best, __shfl_xor(best, off, WAVE));
+                if (lane == 0) s_best[row] = best;
+            }
+        } else {
+            __syncthreads();   // the table
+#pragma unroll
+            for (int r = 0; r < PER; ++r) {
+                z[r] = lane < a.chunks ? pz[r] * weight(pm[r], m[r], a.inv_t, s_table) : 0.0;
+                if (wave + WAVES * r < a.T) s_w[wave + WAVES * r][lane] = z[r];
+            }
+            for (int c = 64 + lane; c < a.chunks; c += 64)
+#pragma unroll
+                for (int r = 0; r < PER; ++r) {
+                    const size_t i = size_t(min(wave + WAVES * r, a.T - 1)) * a.chunks + c;
+                    z[r] += a.z[i] * weight(a.m[i], m[r], a.inv_t, s_table);
+                }
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1)
+#pragma unroll
+                for (int r = 0; r < PER; ++r) z[r] += __shfl_xor(z[r], off, WAVE);
+#pragma unroll
+            for (int r = 0; r < PER; ++r) {
+                const int row = wave + WAVES * r;
+                if (row >= a.T) break;
+                double ak = 1.0 / z[r], bk = 0.0;
+                int level = 0;   // the last one that left something
+                if (lane == 0) {
+                    s_m[row] = m[r];
+                    s_z[row] = z[r];
+                    s_a[row][0] = ak;
+                    s_b[row][0] = bk;
+                    s_level[row][0] = 0;
+                }
+                const int kids = min(a.levels, int(__popcll(__ballot(node && parent == row))));
+                for (int l = 1; l <= kids; ++l) {
+                    const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
+                    double s = 0.0;
+                    for (int c = lane; c < a.chunks; c += 64) s += ps[c];
+                    s = wave_sum64(s);
+                    next_level(s, ak, bk);
+                    if (s > 0.0) level = l;
+                    if (lane == 0) {
+                        s_a[row][l] = ak;
+                        s_b[row][l] = bk;
+                        s_level[row][l] = level;
+                    }
+                }
             }
         }
     }
     __syncthreads();
-    if (!GREEDY) {
-        if (tid > 0 && tid < a.T) {
-            const int p = s_parent[tid];
-            const int64_t x = s_token[tid];
-            const bool known = p >= 0 && p < tid && x >= 0 && x < a.V;
-            s_e[tid] = known ? weight(logit<F32>(a.logits, size_t(p) * a.V + x), s_m[p], a.inv_t) : 0.0;
-            s_q[tid] = known && a.draft ? double(a.draft[size_t(p) * a.V + x]) : 1.0;
-        }
-        __syncthreads();
-    }
-    if (tid == 0) {   // children come after their parents: one pass
-        int cur = 0, n = 1, tried = 0, gone = 0;
+    if (wave == 0) {
+        const double e = known && !GREEDY ? weight(x, s_m[max(parent, 0)], a.inv_t, s_table) : 0.0, qd = known && a.draft ? double(q) : 1.0;
+        const bool right = GREEDY && node && token == s_best[max(parent, 0)];
+        int cur = 0, tried = 0;
+        uint64_t taken = 1, gone = 0;
         double left = GREEDY ? 0.0 : s_z[0];
-        a.path[0] = 0;
-        for (int c = 1; c < a.T; ++c) {
-            if (s_parent[c] != cur) continue;
+        uint64_t kids = __ballot(node && parent == 0);
+        const uint64_t yes = __ballot(right);
+        while (kids) {   // children come after their parents
+            const int c = __builtin_ctzll(kids);
+            kids &= kids - 1;
             bool take;
             if (GREEDY) {
-                take = s_token[c] == s_best[cur];
+                take = yes >> c & 1;
             } else if (a.draft) {
-                if (tried == a.levels) continue;
-                const double r = fmax(s_a[cur][tried] * s_e[c] - s_b[cur][tried] * s_q[c], 0.0);
-                take = double(s_u[c]) * s_q[c] < r;
+                if (tried == a.levels) break;
+                const double qc = lane_of(qd, c), r = fmax(s_a[cur][tried] * lane_of(e, c) - s_b[cur][tried] * qc, 0.0);
+                take = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), c))) * qc < r;
                 ++tried;
             } else {
-                double e = s_e[c];
-                for (int i = 0; i < gone; ++i)
-                    if (s_token[s_gone[i]] == s_token[c]) e = 0.0;
-                take = double(s_u[c]) * left < e;
-                if (!take && e > 0.0 && left - e > 0.0) {
-                    left -= e;
-                    s_gone[gone++] = c;
+                const int lo = __builtin_amdgcn_readlane(int(token), c), hi = __builtin_amdgcn_readlane(int(token >> 32), c);
+                const double ec = gone & __ballot(int(token) == lo && int(token >> 32) == hi) ? 0.0 : lane_of(e, c);
+                take = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), c))) * left < ec;
+                if (!take && ec > 0.0 && left - ec > 0.0) {
+                    left -= ec;
+                    gone |= 1ull << c;
                 }
             }
             if (take) {
                 cur = c;
-                a.path[n++] = c;
-                tried = gone = 0;
+                taken |= 1ull << c;
+                gone = 0;
+                tried = 0;
                 left = GREEDY ? 0.0 : s_z[c];
+                kids = __ballot(node && parent == c);
             }
         }
-        a.count[0] = n;
-        for (int i = n; i < a.T; ++i) a.path[i] = -1;
-        if (GREEDY) a.next[0] = s_best[cur];
-        s_last = cur;
-        s_lvl = tried;
-        s_ngone = gone;
-        s_lo = VWALK;
-        s_hi = -1;
+        const int count = int(__popcll(taken));
+        const uint64_t below = (1ull << lane) - 1;
+        if (taken >> lane & 1) a.path[__popcll(taken & below)] = lane;
+        if (lane >= count && lane < a.T) a.path[lane] = -1;
+        if (gone >> lane & 1) {
+            s_gone[__popcll(gone & below)] = token;
+            s_gone_e[__popcll(gone & below)] = e;
+        }
+        if (lane == 0) {
+            a.count[0] = count;
+            if (GREEDY) a.next[0] = s_best[cur];
+        }
+        if (!GREEDY) {
+            // ---- the chunk that the next token is in: lane i sums chunks i K .. (i + 1) K - 1
+            const int lvl = s_level[cur][tried], gones = int(__popcll(gone)), K = (a.chunks + 63) / 64;
+            const auto part = [&](int c) {   // of the residual, in the units of the sums that it was taken from
+                if (c >= a.chunks) return 0.0;
+                if (lvl > 0) return a.s[(size_t(lvl - 1) * a.T + cur) * a.chunks + c];
+                double w = c < 64 ? s_w[cur][c] : a.z[size_t(cur) * a.chunks + c] * weight(a.m[size_t(cur) * a.chunks + c], s_m[cur], a.inv_t, s_table);
+                for (int i = 0; i < gones; ++i)
+                    if (s_gone[i] / VCHUNK == c) w = fmax(w - s_gone_e[i], 0.0);
+                return w;
+            };
+            double own = 0.0;
+            for (int k = 0; k < K; ++k) own += part(lane * K + k);
+            double upto = own;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const double up = __shfl_up(upto, off, WAVE);
+                if (lane >= off) upto += up;
+            }
+            const double total = lane_of(upto, 63), target = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), 0))) * total;
+            const uint64_t over = __ballot(own > 0.0 && upto > target), some = __ballot(own > 0.0);
+            const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;   // (no sum above it: the last that has any)
+            if (lane == who) {
+                double run = upto - own, base = run;
+                int chunk = lane * K;
+                for (int k = 0; k < K; ++k) {
+                    const double w = part(lane * K + k);
+                    if (w > 0.0) {
+                        chunk = lane * K + k;
+                        base = run;
+                        if (run + w > target) break;
+                    }
+                    run += w;
+                }
+                s_chunk = min(chunk, a.chunks - 1);
+                s_base = base;
+                s_total = target;
+                s_last = cur;
+                s_lvl = lvl;
+                s_gones = gones;
+                s_lo = a.V;
+                s_hi = -1;
+            }
+        }
     }
     if (GREEDY) return;
     __syncthreads();
-    const int cur = s_last, gone = s_ngone, lvl = s_level[cur][s_lvl];
+    // ---- that chunk again, four tokens a thread
+    const int cur = s_last, gones = s_gones, lvl = s_lvl;
+    const double target = s_total;
     const float m = s_m[cur];
-    double w = 0.0;
-    if (tid < a.chunks) {
-        if (lvl > 0) {
-            w = a.s[(size_t(lvl - 1) * a.T + cur) * a.chunks + tid];
-        } else {
-            w = a.z[size_t(cur) * a.chunks + tid] * weight(a.m[size_t(cur) * a.chunks + tid], m, a.inv_t);
-            for (int i = 0; i < gone; ++i)
-                if (s_token[s_gone[i]] / VCHUNK == tid) w = fmax(w - s_e[s_gone[i]], 0.0);
-        }
-    }
-    double upto = group_scan(w, s_wave);
-    double total = 0.0;
-    for (int i = 0; i < VWALK / 64; ++i) total = i ? total + s_wave[i] : s_wave[0];
-    const double target = double(s_u[0]) * total;
-    if (w > 0.0 && upto > target) atomicMin(&s_lo, tid);
-    if (w > 0.0) atomicMax(&s_hi, tid);
-    __syncthreads();
-    const int chunk = s_lo < VWALK ? s_lo : max(s_hi, 0);   // (no sum above the target: the last chunk that has any)
-    __syncthreads();
-    if (tid == chunk) {
-        s_z[0] = upto - w;
-        s_lo = a.V;
-        s_hi = -1;
-    }
-    __syncthreads();
-    // the chunk again, four tokens a thread
-    double part[4], sum = 0.0;
-    const int v0 = chunk * VCHUNK + 4 * tid;
+    double upto[4], r[4], sum = 0.0;
+    const int v0 = s_chunk * VCHUNK + 4 * tid;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int v = v0 + i;
-        double r = 0.0;
+        r[i] = 0.0;
         if (v < a.V) {
-            const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.inv_t);
-            if (lvl > 0) {   // in the units of the level's sums, which stand before their normalisation
-                r = fmax(s_a[cur][lvl - 1] * e - (s_b[cur][lvl - 1] + 1.0) * double(a.draft[size_t(cur) * a.V + v]), 0.0);
+            const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.inv_t, s_table);
+            if (lvl > 0) {   // (before its normalisation, as the chunks' sums are)
+                r[i] = fmax(s_a[cur][lvl - 1] * e - (s_b[cur][lvl - 1] + 1.0) * double(a.draft[size_t(cur) * a.V + v]), 0.0);
             } else {
-                r = e;
-                for (int j = 0; j < gone; ++j)
-                    if (s_token[s_gone[j]] == v) r = 0.0;
+                r[i] = e;
+                for (int j = 0; j < gones; ++j)
+                    if (s_gone[j] == v) r[i] = 0.0;
             }
         }
-        sum += r;
-        part[i] = sum;
-        if (r > 0.0) atomicMax(&s_hi, v);
+        sum += r[i];
+        upto[i] = sum;
+        if (r[i] > 0.0) atomicMax(&s_hi, v);
     }
-    const double before = s_z[0] + group_scan(sum, s_wave) - sum;
+    const double before = s_base + group_scan(sum, s_wave) - sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if ((i ? part[i] > part[i - 1] : part[i] > 0.0) && before + part[i] > target) atomicMin(&s_lo, v0 + i);
+        if (r[i] > 0.0 && before + upto[i] > target) atomicMin(&s_lo, v0 + i);
     __syncthreads();
     if (tid == 0) a.next[0] = s_lo < a.V ? s_lo : max(s_hi, 0);
 }

@@ -70,6 +70,9 @@ def cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, ksc
     y bf16 [>= L, (hq + 2 hk) d], or acc int32 with xscale and wscale as in sc_kernels.qkv_headnorm_rope -> q, the [hq, L, d] view of
     [L, hq, d] storage.  depth int32 [L]: token i is rotated as position pos + depth[i] (the depths of a tree's nodes; default i).
     Computed in float32, rounded once."""
+    q = _lib.native().cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, kscale, vscale, depth)
+    if q is not None:   # the operands of every step; anything else is converted or refused below
+        return q
     src = y if y is not None else acc
     _check(src is not None and src.dim() == 2 and src.shape[0] >= L >= 0 and src.shape[1] == (hq + 2 * hk) * d, "y or acc is [>= L, (hq + 2 hk) d]")
     _check(src.dtype == (BF if y is not None else torch.int32), "y is bfloat16, acc int32")
@@ -90,6 +93,9 @@ def cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, ksc
 
 def cache_read(kcache, vcache, kscale, vscale, n, row0=0):
     """Rows row0 .. row0 + n - 1 of an 8-bit cache as bf16: (k, v) [hk, n, d], what a prompt's attention takes."""
+    out = _lib.native().cache_read(kcache, vcache, kscale, vscale, n, row0)
+    if out is not None:
+        return out
     _check(kscale is not None and n >= 0, "rows of an 8-bit cache, none or more (a bf16 one is read as it is)")
     hk, rows, d = _check_cache(kcache, vcache, kscale, vscale)
     _on_device(kcache, vcache, kscale, vscale)
@@ -102,6 +108,8 @@ def cache_keep(caches, path, count, pos):
     """Row pos + j of every cache takes what row pos + path[j] held, for j < count: the accepted line of a tree moved together, all
     blocks in one launch (up to 32 of them).  caches: (kcache, vcache, kscale, vscale) a block, all of one shape and type; path int32 [T], count int32
     [1] as verify_drafts returns them.  Rows from pos + count on keep what they hold."""
+    if _lib.native().cache_keep(caches, path, count, pos):
+        return
     caches = [tuple(c) for c in caches]
     if not caches:
         return
@@ -121,10 +129,7 @@ def cache_keep(caches, path, count, pos):
 
 def attn_tree_splits(T, n, hq, hk, d):
     """Ranges that n rows are cut into for T nodes."""
-    group = T * (hq // hk)
-    rows = 16 if group <= 16 else 32 if group <= 32 or d == 256 else 64
-    combos = hk * -(-group // rows)
-    return max(1, min(64, -(-n // 256), 512 // combos))
+    return _lib.native().scmx_attn_tree_splits(T, n, hq, hk, d)
 
 
 def attn_tree(q, kcache, vcache, pos, mask=None, kscale=None, vscale=None, scale=None, splits=None):
@@ -132,6 +137,9 @@ def attn_tree(q, kcache, vcache, pos, mask=None, kscale=None, vscale=None, scale
     view that cache_write returns (any other layout is copied) -> bf16 [T, hq * d].  All see the rows below pos; token i sees row
     pos + j if bit j of mask[i] (int64 [T]; default: a chain) is set; one that sees nothing gets zeros.  splits: ranges the rows are cut
     into (default: by the sizes; by the cache's when the position is on the device)."""
+    out = _lib.native().attn_tree(q, kcache, vcache, pos, mask, kscale, vscale, scale, splits)
+    if out is not None:
+        return out
     q = q.transpose(0, 1).contiguous()   # [T, hq, d]; no copy when q already is a view of it
     T, hq, d = q.shape
     hk, rows, dc = _check_cache(kcache, vcache, kscale, vscale)

@@ -52,6 +52,9 @@ def verify_drafts(logits, tokens, parents, temperature=0.0, uniforms=None, draft
             _check(draft.dtype == torch.float32 and draft.shape == logits.shape, "draft is float32 [T, V]")
             _check(siblings is not None and 0 <= siblings, "a draft needs siblings, the most children of a node")
             levels = min(max(int(siblings), 1), MAX_SIBLINGS)
+    out = _lib.native().verify_drafts(logits, tokens, parents, temperature, uniforms, draft, levels)
+    if out is not None:
+        return out
     _on_device(logits, tokens, parents, uniforms, draft)
     n = _lib.native()
     path, count, token = n.empty_i32(logits, T), n.empty_i32(logits, 1), n.empty_i64(logits, 1)

@@ -93,10 +93,11 @@ int main() {
     };
     expect_valid(attend(64, 32, 8, 128, 100, 36, 0.1f, f32(5), 64), "attn_tree");
     expect_valid(attend(1, 16, 4, 256, 100, 0, -0.1f, nullptr, 1, f32(6), f32(7)), "attn_tree, one token, 8 bits");
-    expect_valid(attend(64, 65535, 1, 64, 2147483647, 2147483583, 0.1f, f32(5), 64), "attn_tree at the limits");
+    expect_valid(attend(64, 4096, 1, 64, 2147483647, 2147483583, 0.1f, f32(5), 64), "attn_tree at the limits");
     expect(attend(65, 32, 8, 128, 100, 0, 0.1f, nullptr, 1), SCMX_ERR_ARG, "attn_tree of 65 nodes");
     expect(attend(4, 32, 8, 128, 100, 97, 0.1f, nullptr, 1), SCMX_ERR_ARG, "attn_tree past the cache");
     expect(attend(4, 32, 7, 128, 100, 0, 0.1f, nullptr, 1), SCMX_ERR_ARG, "attn_tree, uneven heads");
+    expect(attend(4, 4097, 1, 128, 100, 0, 0.1f, nullptr, 1), SCMX_ERR_ARG, "attn_tree, 4097 heads a KV head");
     expect(attend(4, 32, 8, 128, 100, 0, 0.1f, nullptr, 2), SCMX_ERR_ARG, "attn_tree, splits without a workspace");
     expect(attend(4, 32, 8, 128, 100, 0, 0.1f, f32(5), 65), SCMX_ERR_ARG, "attn_tree, 65 splits");
     expect(attend(4, 32, 8, 128, 100, 0, __builtin_nanf(""), nullptr, 1), SCMX_ERR_ARG, "attn_tree, scale NaN");
@@ -113,6 +114,7 @@ int main() {
     expect(verify(nullptr, -1.0, f32(8), 8, 100, 0, p(6), 4096), SCMX_ERR_ARG, "verify_drafts, temperature -1");
     expect(verify(nullptr, 1.0, f32(8), 65, 100, 0, p(6), 4096), SCMX_ERR_ARG, "verify_drafts of 65 nodes");
     expect(verify(nullptr, 1.0, f32(8), 1, 4194305, 0, p(6), size_t(1) << 30), SCMX_ERR_ARG, "verify_drafts, vocabulary");
+    if (scmx_attn_tree_splits(65, 100, 8, 8, 128) != 1 || scmx_attn_tree_splits(1, 2147483647, 65535, 65535, 64) != 1) ++failures;
     if (scmx_verify_workspace(65, 100, 0) || scmx_verify_workspace(1, 0, 0) || scmx_verify_workspace(1, 100, 17) || !scmx_verify_workspace(1, 1, 0)) ++failures;
 
     std::mt19937 rng(77);
@@ -132,6 +134,10 @@ int main() {
         expect_status(scmx_attn_tree(u16(0), p(1), p(2), maybe(f32(6)), maybe(f32(7)), rng() % 2 ? i64(3) : nullptr, dev, pos, u16(4), small(), small(), small(), dim(), r(), 0.1f,
                                      maybe(f32(5)), small(), nullptr),
                       "fuzz attn_tree");
+        {
+            const int s = scmx_attn_tree_splits(small(), r(), small(), small(), dim());
+            if (s < 1 || s > 64) ++failures;
+        }
         const int T = small(), V = r(), s = int(rng() % 20);
         expect_status(scmx_verify_drafts(i64(0), i32(1), p(2), int(rng() % 2), maybe(f32(7)), rng() % 2 ? 0.0 : 0.7, maybe(f32(8)), i32(3), i32(4), i64(5), T, V, s, p(6),
                                          rng() % 2 ? scmx_verify_workspace(T, V, s) : size_t(r()), nullptr),
