@@ -61,8 +61,7 @@ __device__ const double EXP2_64[64] = {
 // 2^(k / 64) from the table and the exponent.  Half of the time of the stats kernel is this arithmetic; a series to r^11 of the whole
 // fraction, without a table, took a third more instructions.
 __device__ __forceinline__ double exp_neg(double x, const double* table) {
-    const double c = fmax(x, -700.0), n = rint(c * 92.33248261893657);
-    const double r = __builtin_fma(n, -0.010830424696249145, c);
+    const double n = rint(x * 92.33248261893657), r = __builtin_fma(n, -0.010830424696249145, x);   // (-inf: whatever, and 0 at the end)
     double p = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
     p = __builtin_fma(p, r, 1.0 / 6.0);
     p = __builtin_fma(p, r, 0.5);
@@ -72,21 +71,31 @@ __device__ __forceinline__ double exp_neg(double x, const double* table) {
     const double v = __longlong_as_double(__double_as_longlong(p * table[k & 63]) + ((long long)(k >> 6) << 52));
     return x < -700.0 ? 0.0 : v;
 }
-// A logit's weight relative to the largest, m: 1 for the largest itself, also where it is infinite.
+// A logit's weight relative to the largest, m: 1 for the largest itself, also where that is infinite.
 __device__ __forceinline__ double weight(float x, float m, double inv_t, const double* table) {
     if (!(fabsf(m) <= 3.4028234e38f)) return x == m ? 1.0 : 0.0;   // (the same for a whole row)
     return exp_neg((double(x) - double(m)) * inv_t, table);
+}
+// The same of N logits of which the first `there` are some (the others are -inf): straight code where the largest is finite.
+template <int N>
+__device__ __forceinline__ void weights(const float* x, float m, double inv_t, const double* table, int there, double* w) {
+    if (fabsf(m) <= 3.4028234e38f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = exp_neg((double(x[i]) - double(m)) * inv_t, table);
+    } else {
+        for (int i = 0; i < N; ++i) w[i] = i < there && x[i] == m ? 1.0 : 0.0;
+    }
 }
 __device__ __forceinline__ void copy_table(double* table) {
     if (threadIdx.x < 64) table[threadIdx.x] = EXP2_64[threadIdx.x];   // (a barrier follows before its first use)
 }
 
-__device__ __forceinline__ float clean(float x) { return x == x ? x : -__builtin_inff(); }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -__builtin_inff()); }   // NaN: -inf
 template <bool F32>
 __device__ __forceinline__ float logit(const void* logits, size_t at) {
     return clean(F32 ? static_cast<const float*>(logits)[at] : bf16_to_f32(static_cast<const uint16_t*>(logits)[at]));
 }
-// Eight consecutive logits from token v on (beyond the vocabulary: anything).
+// Eight consecutive logits from token v on (beyond the vocabulary: -inf).
 template <bool F32>
 __device__ __forceinline__ void logits8(const VerifyArgs& a, size_t row, int v, float* x) {
     if (a.logits_vec && v + 8 <= a.V) {
@@ -109,17 +118,55 @@ __device__ __forceinline__ void logits8(const VerifyArgs& a, size_t row, int v, 
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = v + i < a.V ? logit<F32>(a.logits, row * a.V + v + i) : 0.0f;
+    for (int i = 0; i < 8; ++i) x[i] = v + i < a.V ? logit<F32>(a.logits, row * a.V + v + i) : -__builtin_inff();
 }
 
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_readlane(int(b), lane), hi = __builtin_amdgcn_readlane(int(b >> 32), lane);
+    return __longlong_as_double((long long)(uint64_t(uint32_t(hi)) << 32 | uint32_t(lo)));
+}
+template <int CTRL>
+__device__ __forceinline__ double row_op(double v) {   // v of the lane that CTRL names; 0 where it names none
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, int(b), CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), CTRL, 0xF, 0xF, true);
+    return __longlong_as_double((long long)(uint64_t(uint32_t(hi)) << 32 | uint32_t(lo)));
+}
+// Over the wave, in every lane: within rows of 16 lanes by row operations, the four rows as scalars (a butterfly through LDS has six
+// trips of a hundred cycles, and these kernels are chains of such sums).
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, WAVE);
-    return v;
+    v += row_op<0xB1>(v);    // quad_perm 1 0 3 2
+    v += row_op<0x4E>(v);    // quad_perm 2 3 0 1
+    v += row_op<0x141>(v);   // row_half_mirror
+    v += row_op<0x140>(v);   // row_mirror
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+template <int CTRL>
+__device__ __forceinline__ float row_max(float v) {
+    const int b = __float_as_int(v);
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ float wave_max32(float v) {
+    v = row_max<0xB1>(v);
+    v = row_max<0x4E>(v);
+    v = row_max<0x141>(v);
+    v = row_max<0x140>(v);
+    const auto at = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
+    return fmaxf(fmaxf(at(0), at(16)), fmaxf(at(32), at(48)));
+}
+// Inclusive sum in lane order.
+__device__ __forceinline__ double wave_scan64(double v) {
+    v += row_op<0x111>(v);   // row_shr 1, 2, 4, 8
+    v += row_op<0x112>(v);
+    v += row_op<0x114>(v);
+    v += row_op<0x118>(v);
+    const double a = lane_of(v, 15), b = lane_of(v, 31), c = lane_of(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? a + b : (a + b) + c);
 }
 // Over the workgroup; every thread gets the result.  `s` holds one entry a wave.
 __device__ __forceinline__ float group_max(float v, float* s) {
-    v = wave_max(v);
+    v = wave_max32(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -154,8 +201,7 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (v0 + t * 8 * VNT + i < a.V) m = fmaxf(m, x[t][i]);
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, x[t][i]);
     m = group_max(m, s_m);
     const size_t out = row * a.chunks + blockIdx.x;
     if (GREEDY) {
@@ -178,10 +224,12 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
     }
     double z = 0.0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+        double w[8];
+        weights<8>(x[t], m, a.inv_t, s_table, a.V - (v0 + t * 8 * VNT), w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (v0 + t * 8 * VNT + i < a.V) z += weight(x[t][i], m, a.inv_t, s_table);
+        for (int i = 0; i < 8; ++i) z += w[i];
+    }
     z = group_sum64(z, s_z);
     if (threadIdx.x == 0) {
         a.m[out] = m;
@@ -240,33 +288,24 @@ __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, i
     }
     double s = 0.0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+        double w[8];
+        weights<8>(x[t], m, a.inv_t, s_table, a.V - (v0 + t * 8 * VNT), w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (v0 + t * 8 * VNT + i < a.V) s += fmax(ak * weight(x[t][i], m, a.inv_t, s_table) - (bk + 1.0) * double(q[t][i]), 0.0);
+        for (int i = 0; i < 8; ++i) s += fmax(ak * w[i] - (bk + 1.0) * double(q[t][i]), 0.0);   // (beyond the vocabulary q is 0)
+    }
     s = group_sum64(s, s_z);
     if (threadIdx.x == 0) a.s[(size_t(level - 1) * a.T + row) * a.chunks + blockIdx.x] = s;
 }
 
 // Inclusive sum over the workgroup's threads in thread order; `s` holds one entry a wave.
 __device__ __forceinline__ double group_scan(double v, double* s) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double up = __shfl_up(v, off, WAVE);
-        if (lane >= off) v += up;
-    }
-    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_scan64(v);
     if (lane == 63) s[wave] = v;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) v += s[w];
-    return v;
-}
-
-__device__ __forceinline__ double lane_of(double v, int lane) {
-    const long long b = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_readlane(int(b), lane), hi = __builtin_amdgcn_readlane(int(b >> 32), lane);
-    return __longlong_as_double((long long)(uint64_t(uint32_t(hi)) << 32 | uint32_t(lo)));
+    double before = lane < wave ? s[lane] : 0.0;   // (up to 16 waves)
+    return v + wave_sum64(before);
 }
 
 // One workgroup: the nodes' sums from the chunks', the walk, the token after it.  A chain of trips to memory and of cross-lane
@@ -279,7 +318,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
     __shared__ double s_z[VNODES], s_wave[WAVES], s_table[64], s_gone_e[VNODES], s_base, s_total;
     __shared__ double s_w[GREEDY ? 1 : VNODES][64];   // the first 64 chunks' sums relative to the node's largest logit
     __shared__ double s_a[GREEDY ? 1 : VNODES][VLEVELS + 1], s_b[GREEDY ? 1 : VNODES][VLEVELS + 1];
-    __shared__ int s_best[VNODES], s_level[GREEDY ? 1 : VNODES][VLEVELS + 1], s_last, s_lvl, s_gones, s_chunk, s_lo, s_hi;
+    __shared__ int s_best[VNODES], s_level[GREEDY ? 1 : VNODES][VLEVELS + 1], s_last, s_lvl, s_gones, s_chunk, s_over[WAVES], s_some[WAVES];
     __shared__ int64_t s_gone[VNODES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (!GREEDY) copy_table(s_table);
@@ -316,7 +355,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
 #pragma unroll
             for (int r = 0; r < PER; ++r) m[r] = fmaxf(m[r], a.m[size_t(min(wave + WAVES * r, a.T - 1)) * a.chunks + c]);
 #pragma unroll
-        for (int r = 0; r < PER; ++r) m[r] = wave_max(m[r]);
+        for (int r = 0; r < PER; ++r) m[r] = wave_max32(m[r]);
         if (GREEDY) {
 #pragma unroll
             for (int r = 0; r < PER; ++r) {
@@ -343,21 +382,22 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                     z[r] += a.z[i] * weight(a.m[i], m[r], a.inv_t, s_table);
                 }
 #pragma unroll
-            for (int off = 32; off >= 1; off >>= 1)
-#pragma unroll
-                for (int r = 0; r < PER; ++r) z[r] += __shfl_xor(z[r], off, WAVE);
+            for (int r = 0; r < PER; ++r) z[r] = wave_sum64(z[r]);
 #pragma unroll
             for (int r = 0; r < PER; ++r) {
                 const int row = wave + WAVES * r;
                 if (row >= a.T) break;
-                double ak = 1.0 / z[r], bk = 0.0;
-                int level = 0;   // the last one that left something
                 if (lane == 0) {
                     s_m[row] = m[r];
                     s_z[row] = z[r];
+                    s_level[row][0] = 0;
+                }
+                if (a.levels == 0) continue;
+                double ak = 1.0 / z[r], bk = 0.0;
+                int level = 0;   // the last one that left something
+                if (lane == 0) {
                     s_a[row][0] = ak;
                     s_b[row][0] = bk;
-                    s_level[row][0] = 0;
                 }
                 const int kids = min(a.levels, int(__popcll(__ballot(node && parent == row))));
                 for (int l = 1; l <= kids; ++l) {
@@ -439,12 +479,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             };
             double own = 0.0;
             for (int k = 0; k < K; ++k) own += part(lane * K + k);
-            double upto = own;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const double up = __shfl_up(upto, off, WAVE);
-                if (lane >= off) upto += up;
-            }
+            const double upto = wave_scan64(own);
             const double total = lane_of(upto, 63), target = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), 0))) * total;
             const uint64_t over = __ballot(own > 0.0 && upto > target), some = __ballot(own > 0.0);
             const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;   // (no sum above it: the last that has any)
@@ -466,8 +501,6 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 s_last = cur;
                 s_lvl = lvl;
                 s_gones = gones;
-                s_lo = a.V;
-                s_hi = -1;
             }
         }
     }
@@ -478,6 +511,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
     const double target = s_total;
     const float m = s_m[cur];
     double upto[4], r[4], sum = 0.0;
+    int some = -1, over = -1;   // the thread's last token that has any probability, its first above the target
     const int v0 = s_chunk * VCHUNK + 4 * tid;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -495,14 +529,24 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         }
         sum += r[i];
         upto[i] = sum;
-        if (r[i] > 0.0) atomicMax(&s_hi, v);
+        if (r[i] > 0.0) some = v;
     }
     const double before = s_base + group_scan(sum, s_wave) - sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (r[i] > 0.0 && before + upto[i] > target) atomicMin(&s_lo, v0 + i);
+    for (int i = 3; i >= 0; --i)
+        if (r[i] > 0.0 && before + upto[i] > target) over = v0 + i;
+    // lanes and waves hold the chunk in order: the first wave's first lane, or the last's last (atomics on one word took 15 us)
+    const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+    if (lane == 0) {
+        s_over[wave] = overs ? __builtin_amdgcn_readlane(over, __builtin_ctzll(overs)) : -1;
+        s_some[wave] = somes ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(somes)) : -1;
+    }
     __syncthreads();
-    if (tid == 0) a.next[0] = s_lo < a.V ? s_lo : max(s_hi, 0);
+    if (wave == 0) {
+        const int o = lane < WAVES ? s_over[lane] : -1, h = lane < WAVES ? s_some[lane] : -1;
+        const uint64_t any = __ballot(o >= 0), rest = __ballot(h >= 0);
+        if (lane == 0) a.next[0] = any ? __builtin_amdgcn_readlane(o, __builtin_ctzll(any)) : rest ? __builtin_amdgcn_readlane(h, 63 - __builtin_clzll(rest)) : 0;
+    }
 }
 
 }  // namespace scmx
