@@ -11,7 +11,10 @@ epilogue="gemm": scales, residual adds and SwiGLU in the GEMM's registers (bf16 
 epilogue="row":  INT32 GEMM out, then the row kernels res_norm_quant / swiglu_quant / qkv_epilogue_headnorm,
                  e2e/fused_qwen3.py:257-308.
 The decode step's fixed-shape halves can be captured in HIP graphs (graphs=True), which is what mx.compile does for
-the reference (e2e/decode.py:30-33): one graph launch replaces about ten kernel launches per layer."""
+the reference (e2e/decode.py:30-33): one graph launch replaces about ten kernel launches per layer.
+
+Beyond the reference: caches in 8 bits (make_cache(bits=8)) in every path, and DraftQwen3, a decode step that decides several
+tokens at once, a tree of drafted ones verified against the model's own probabilities."""
 import json
 import os
 from dataclasses import dataclass, fields
@@ -19,7 +22,9 @@ from dataclasses import dataclass, fields
 import torch
 import torch.nn.functional as TF
 
+from . import sc_cache as C
 from . import sc_decode as G
+from . import sc_draft
 from . import sc_format as F
 from . import sc_kernels as S
 from .sc_weights import GROUPS, PackedWeight, pack_weights
@@ -116,14 +121,21 @@ class FusedQwen3:
     def weight_bytes(self):
         return sum(w.nbytes() for _, ws in self.layers for w in ws.values())
 
-    def make_cache(self, max_len=4096):
-        return [KVCache(self.args, max_len, self.device) for _ in self.layers]
+    def make_cache(self, max_len=4096, bits=16):
+        """A cache a block, in bf16 or (bits=8) in 8 bits with a scale a row: half the bytes to keep and to read."""
+        if bits not in (8, 16):
+            raise ValueError("a cache has 16 or 8 bits")
+        return [(KVCache if bits == 16 else C.Q8Cache)(self.args, max_len, self.device) for _ in self.layers]
 
     # ---- pieces shared by prefill and decode --------------------------------------------------------------------
     def _qkv(self, c, L, nw, y=None, acc=None, xs=None, ws=None, pos=None):
         """Per-head RMSNorm of q and k, rotary embedding at positions pos..pos+L-1 (pos defaults to the cache offset;
         an int64 device tensor for graph replay) and the KV-cache append, in one kernel: returns q [hq, L, d]."""
         a = self.args
+        if isinstance(c, C.Q8Cache):
+            return C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads, a.num_key_value_heads,
+                                 a.head_dim, c.k, c.v, c.offset if pos is None else pos, self.inv_freq, c.kscale, c.vscale, acc=acc,
+                                 xscale=xs, wscale=ws)
         return S.qkv_headnorm_rope(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads,
                                    a.num_key_value_heads, a.head_dim, c.k, c.v, c.offset if pos is None else pos,
                                    self.inv_freq, acc=acc, xscale=xs, wscale=ws, token_major=L > 1)
@@ -134,12 +146,18 @@ class FusedQwen3:
         if off + L > c.k.shape[1]:
             raise ValueError("KV cache is full")
         c.offset = off + L
-        k, v = c.k[:, :off + L], c.v[:, :off + L]
-        hq, hk = q.shape[0], k.shape[0]
-        if L == 1:
+        if isinstance(c, C.Q8Cache):
+            if L <= C.MAX_NODES:   # few tokens read the 8-bit rows as they are
+                return C.attn_tree(q, c.k, c.v, off, None, c.kscale, c.vscale)
+            k, v = C.cache_read(c.k, c.v, c.kscale, c.vscale, off + L)
+        elif L == 1:
             return S.attn_decode(q, c.k, c.v, off + 1)
+        else:
+            k, v = c.k, c.v
+        hq, hk = q.shape[0], k.shape[0]
         if self.attn_kernel and q.shape[-1] == 128:   # this library's causal attention (head dim 128 only)
-            return S.attn_prefill(q, c.k, c.v, off)
+            return S.attn_prefill(q, k, v, off)
+        k, v = k[:, :off + L], v[:, :off + L]
         gqa = {"enable_gqa": True} if hq != hk and self.sdpa_gqa else {}
         if hq != hk and not self.sdpa_gqa:
             k, v = k.repeat_interleave(hq // hk, 0), v.repeat_interleave(hq // hk, 0)
@@ -264,6 +282,8 @@ class DecodeQwen3:
             y = G.gemv(xq, w.codes, w.bcodes, xs, w.wscale, w.N, 1, fmt=f.fmt)
         if self.fuse_attn:   # the attention output, not q: the token's k and v are in the cache afterwards
             a = self.args
+            if isinstance(c, C.Q8Cache):
+                return C.attn_tree(f._qkv(c, 1, nw, y=y[None], pos=pos), c.k, c.v, pos, None, c.kscale, c.vscale)
             return S.attn_decode_qkv(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, a.num_attention_heads,
                                      a.num_key_value_heads, a.head_dim, c.k, c.v, pos, f.inv_freq)
         return f._qkv(c, 1, nw, y=y[None], pos=pos)
@@ -353,7 +373,9 @@ class DecodeQwen3:
         for i, (nw, ws) in enumerate(f.layers):
             c = cache[i]
             q = self._pre(h, nw, ws["qkv"], c, self.pos)
-            h = self._post(q if self.fuse_attn else S.attn_decode(q, c.k, c.v, self.pos), h, nw, ws)
+            if not self.fuse_attn:
+                q = C.attn_tree(q, c.k, c.v, self.pos, None, c.kscale, c.vscale) if isinstance(c, C.Q8Cache) else S.attn_decode(q, c.k, c.v, self.pos)
+            h = self._post(q, h, nw, ws)
         return self._logits(h)
 
     def step(self, tok, cache):
@@ -385,6 +407,74 @@ class DecodeQwen3:
             else:
                 h = self._replay(("post", i), lambda x, r, nw=nw, ws=ws: self._post(x, r, nw, ws), [o, h])
         return self._logits(h)      # new tensors: the final norm never returns a graph's static buffer
+
+
+class DraftQwen3(DecodeQwen3):
+    """A decode step for a tree of drafted tokens from a FusedQwen3 with epilogue="gemm": all T (1..64) go through the model
+    together, in one pass over the weights, and as many of them are accepted as the model's own probabilities allow, so that a step
+    yields between one and T tokens.  tokens int64 [T]: token 0 is the sequence's newest one, not yet in the cache (a plain
+    decode step's input), the others are drafts, whose places `tree` (sc_draft.DraftTree) says.  Where the drafts come from is the caller's.
+    graphs=True captures the step, verification and the move of the accepted rows included, once per tree, cache and kind
+    of verification (temperature, with or without a draft), for as long as that cache is used; what is returned is fresh."""
+
+    def __init__(self, fused, graphs=False):
+        super().__init__(fused, graphs=graphs)
+
+    def _linear(self, x, w, epi, res=None, nw=None):
+        """A linear on a few rows x [T, K], RMSNorm with weight nw first."""
+        f = self.f
+        if x.shape[0] <= 8:   # norm and quantization in the GEMV
+            return G.gemv(x, w.codes, w.bcodes, None, w.wscale, w.N, epi, res=res, pro=1 if nw is None else 2, nw=nw, eps=f.eps, fmt=f.fmt).view(x.shape[0], -1)
+        return S.linear_w4a8(x if nw is None else S.rmsnorm(x, nw, f.eps), w.codes, w.bcodes, w.wscale, w.N, epi, res, f.fmt)
+
+    def hidden(self, tokens, tree, cache, pos):
+        """Final normed hidden states [T, D] of the tree's nodes, whose keys and values go to the caches' rows pos .. pos + T - 1 (pos: int,
+        or an int64 device tensor); the caches' offsets stay."""
+        f, a = self.f, self.args
+        h = f.embed.index_select(0, tokens)
+        for c, (nw, ws) in zip(cache, f.layers):
+            k, v, ks, vs = C.tensors(c)
+            y = self._linear(h, ws["qkv"], 1, nw=nw["input_layernorm"])
+            q = C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, tree.T, a.num_attention_heads, a.num_key_value_heads, a.head_dim,
+                              k, v, pos, f.inv_freq, ks, vs, tree.depth)
+            h = self._linear(C.attn_tree(q, k, v, pos, tree.mask, ks, vs), ws["o"], 2, h)
+            h = self._linear(self._linear(h, ws["gu"], 3, nw=nw["post_attention_layernorm"]), ws["down"], 2, h)
+        return S.rmsnorm(h, f.norm, f.eps)
+
+    def _draft_step(self, tokens, tree, cache, pos, temperature, uniforms, draft):
+        logits = self.f.logits(self.hidden(tokens, tree, cache, pos))
+        path, count, token = sc_draft.verify_drafts(logits, tokens, tree.parents, temperature, uniforms, draft, tree.siblings)
+        C.cache_keep([C.tensors(c) for c in cache], path, count, pos)
+        return path, count, token, logits
+
+    def step(self, tokens, tree, cache, temperature=0.0, uniforms=None, draft=None):
+        """-> (path, count, next, logits): path int32 [T] names the accepted nodes from node 0 on (count of them), next int64 [1] is the
+        token after them and the next step's token 0.  The caches then hold the accepted tokens and their offsets stand
+        behind them (which waits for the step).  temperature, uniforms, draft: sc_draft.verify_drafts."""
+        off, f = cache[0].offset, self.f
+        if off + tree.T > cache[0].k.shape[1]:
+            raise ValueError("KV cache is full")
+        tokens = tokens.reshape(-1)
+        if tokens.numel() != tree.T or tokens.dtype != torch.int64:
+            raise ValueError("tokens are int64, one for every node of the tree")
+        S.set_format(f.fmt)
+        if self.graphs is None:
+            out = self._draft_step(tokens, tree, cache, off, temperature, uniforms, draft)
+        else:
+            self.pos.fill_(off)
+            given = [t for t in (uniforms, draft) if t is not None]
+
+            def fn(tokens, *rest):
+                rest = list(rest)
+                u = rest.pop(0) if uniforms is not None else None
+                return self._draft_step(tokens, tree, cache, self.pos, temperature, u, rest.pop(0) if draft is not None else None)
+
+            key = ("draft", tuple(tree.parent_list), float(temperature), uniforms is not None, draft is not None)
+            out = tuple(t.clone() for t in self._replay(key, fn, [tokens, *given], owner=cache))
+        n = off + int(out[1])
+        for c in cache:
+            c.offset = n
+        return out
 
 
 # ---- from a checkpoint directory -----------------------------------------------------------------------------------
