@@ -10,6 +10,7 @@
 namespace scmx {
 
 constexpr int CNT = 256;
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct WriteArgs {
     const int32_t* acc;
@@ -30,65 +31,98 @@ struct WriteArgs {
     int rows;
 };
 
+// Operations over the LPH lanes of a head (8, 16 or 32, aligned), within rows of 16 lanes by row operations: through LDS (shuffles) a
+// head took twenty trips of a hundred cycles, one after the other.
+template <int CTRL>
+__device__ __forceinline__ float row_op(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int LPH, typename F>
+__device__ __forceinline__ float over_head(float v, F&& f) {   // f of all lanes' values, in every lane
+    v = f(v, row_op<0xB1>(v));    // quad_perm 1 0 3 2
+    v = f(v, row_op<0x4E>(v));    // quad_perm 2 3 0 1
+    v = f(v, row_op<0x141>(v));   // row_half_mirror: the other quad of eight
+    if (LPH >= 16) v = f(v, row_op<0x140>(v));   // row_mirror: the other eight of sixteen
+    if (LPH >= 32) v = f(v, __shfl_xor(v, 16, WAVE));
+    return v;
+}
+template <int LPH>
+__device__ __forceinline__ float partner(float v) {   // of the lane half a head away
+    if (LPH == 8) return row_op<0x1B>(row_op<0x141>(v));   // 7 - j, then its quad reversed: j ^ 4
+    if (LPH == 16) return row_op<0x128>(v);                // row_ror 8
+    return __shfl_xor(v, 16, WAVE);
+}
+
 // One token per blockIdx.x.  A head of D values is held by D / 8 lanes, eight consecutive values each: 16-byte loads, 16-byte
 // (bf16) or 8-byte (codes) stores, the norm's sum and the row's maximum over the lanes of the group, and the partner of a
 // rotation half a group away at the same place.  Per head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
 // The angle is formed and reduced to one turn in float64: in float32 a position of 100000 is off by 4e-3 of a radian, as much as
 // the result's rounding.  Everything else is float32 and rounded once, to bf16 or to a code.
-// Bound by reading y for a prompt, by latency (the row, then two chains of cross-lane sums) for a few tokens.
-template <int D, bool EIGHT>
+// Bound by memory for a prompt (the next head's row is requested before this one's is worked on), by latency (the row, then two
+// chains of cross-lane sums) for a few tokens.
+template <int D, bool EIGHT, bool ACC>
 __global__ __launch_bounds__(CNT) void cache_write_kernel(const WriteArgs a) {
     constexpr int LPH = D / 8, GROUPS = CNT / LPH;
     __shared__ float s_sin[D / 2], s_cos[D / 2];
     const int row = blockIdx.x, grp = threadIdx.x / LPH, j = threadIdx.x % LPH;
-    const int heads = a.hq + 2 * a.hk;
+    const int heads = a.hq + 2 * a.hk, stride = gridDim.y * GROUPS;
     const int64_t pos = a.pos_dev ? a.pos_dev[0] : a.pos0;
     const bool fits = pos >= 0 && pos <= int64_t(a.rows) - a.L;
-    float x[8];
-    auto load = [&](int g) {   // the lane's values of head g
+    // the lane's values of a head as they come, and as numbers
+    struct Raw {
+        u32x4 w[ACC ? 2 : 1];
+    };
+    const auto load = [&](int g, Raw& r) {
         const size_t at = (size_t(row) * heads + g) * D + 8 * j;
-        if (a.acc) {
-            const float xs = a.xscale[row];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = round_bf16(__fmul_rn(__fmul_rn(float(a.acc[at + i]), xs), a.wscale[g * D + 8 * j + i]));
+        if constexpr (ACC) {
+            r.w[0] = *reinterpret_cast<const u32x4u*>(a.acc + at);
+            r.w[1] = *reinterpret_cast<const u32x4u*>(a.acc + at + 4);
         } else {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(a.y + at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[2 * i] = bf16_lo(w[i]);
-                x[2 * i + 1] = bf16_hi(w[i]);
-            }
+            r.w[0] = *reinterpret_cast<const u32x4*>(a.y + at);
         }
     };
+    Raw raw;
     int g = blockIdx.y * GROUPS + grp;
-    if (g < heads) load(g);   // on its way beside the angles
+    if (g < heads) load(g, raw);   // on its way beside the angles
+    const u32x4 wq = *reinterpret_cast<const u32x4*>(a.qn + 8 * j), wk = *reinterpret_cast<const u32x4*>(a.kn + 8 * j);
     if (threadIdx.x < D / 2) {
         const double turns = double(pos + (a.depth ? a.depth[row] : row)) * double(a.inv_freq[threadIdx.x]) * 0.15915494309189535;
         sincospif(float(2.0 * (turns - rint(turns))), &s_sin[threadIdx.x], &s_cos[threadIdx.x]);
     }
     __syncthreads();
-    for (; g < heads; g += gridDim.y * GROUPS) {   // (a group is whole or absent)
-        if (g >= int(gridDim.y) * GROUPS) load(g);
+    for (; g < heads; g += stride) {   // (a group is whole or absent)
+        float x[8];
+        if constexpr (ACC) {
+            const float xs = a.xscale[row];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = round_bf16(__fmul_rn(__fmul_rn(float(int32_t(raw.w[i / 4][i % 4])), xs), a.wscale[g * D + 8 * j + i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = bf16_lo(raw.w[0][i]);
+                x[2 * i + 1] = bf16_hi(raw.w[0][i]);
+            }
+        }
+        if (g + stride < heads) load(g + stride, raw);
         const bool is_v = g >= a.hq + a.hk;
         if (!is_v) {
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-#pragma unroll
-            for (int off = LPH / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, WAVE);
+            ss = over_head<LPH>(ss, [](float p, float q) { return p + q; });
             const float inv = __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, float(D)) + a.eps));
-            const u32x4 w = *reinterpret_cast<const u32x4*>((g < a.hq ? a.qn : a.kn) + 8 * j);
+            const u32x4 w = g < a.hq ? wq : wk;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[2 * i] = x[2 * i] * inv * bf16_lo(w[i]);
                 x[2 * i + 1] = x[2 * i + 1] * inv * bf16_hi(w[i]);
             }
+            const int at = 8 * (j % (LPH / 2));
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_xor(x[i], LPH / 2, WAVE), sn = s_sin[(8 * j + i) % (D / 2)], cs = s_cos[(8 * j + i) % (D / 2)];
-                x[i] = __builtin_fmaf(x[i], cs, j < LPH / 2 ? -(other * sn) : other * sn);
+                const float other = partner<LPH>(x[i]) * s_sin[at + i];
+                x[i] = __builtin_fmaf(x[i], s_cos[at + i], j < LPH / 2 ? -other : other);
             }
         }
         if (g >= a.hq && !fits) continue;
@@ -98,8 +132,7 @@ __global__ __launch_bounds__(CNT) void cache_write_kernel(const WriteArgs a) {
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]) <= 3.4028234e38f ? fabsf(x[i]) : __builtin_inff());   // (NaN too)
-#pragma unroll
-            for (int off = LPH / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, WAVE));
+            top = over_head<LPH>(top, [](float p, float q) { return fmaxf(p, q); });
             const bool finite = top < __builtin_inff(), any = finite && top >= 0x1p-100f;
             const float inv = any ? __fdiv_rn(127.0f, top) : 0.0f;
             u32x2 w = {0, 0};
@@ -223,8 +256,10 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
     const hipStream_t st = (hipStream_t)stream;
     const auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        if (kscale) cache_write_kernel<D, true><<<grid, dim3(CNT), 0, st>>>(a);
-        else cache_write_kernel<D, false><<<grid, dim3(CNT), 0, st>>>(a);
+        if (acc && kscale) cache_write_kernel<D, true, true><<<grid, dim3(CNT), 0, st>>>(a);
+        else if (acc) cache_write_kernel<D, false, true><<<grid, dim3(CNT), 0, st>>>(a);
+        else if (kscale) cache_write_kernel<D, true, false><<<grid, dim3(CNT), 0, st>>>(a);
+        else cache_write_kernel<D, false, false><<<grid, dim3(CNT), 0, st>>>(a);
     };
     if (d == 64) go(std::integral_constant<int, 64>{});
     else if (d == 128) go(std::integral_constant<int, 128>{});
