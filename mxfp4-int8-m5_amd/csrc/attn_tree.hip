@@ -35,8 +35,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int TKEYS = 32, TXCDS = 8, JNT = 256;
-// Waves of a workgroup: two a SIMD; rows of 256 in bf16 take the registers of two.
-static constexpr __host__ __device__ int tree_waves(int d, bool eight) { return d == 256 && !eight ? 4 : 8; }
+// Waves of a workgroup.  Four, two workgroups a CU, whose starts and ends overlap; eight of one: 16 tokens, 3000 rows of 16:8 x 128, bf16
+// 12.4 -> 10.9 us, one token, 1000 rows, 8 bits 8.8 -> 7.6, 40000 rows 21.2 -> 20.8.
+constexpr int TWAVES = 4, TNT = 64 * TWAVES;
+constexpr int TONE = 16;   // tiles up to which one range takes all (four a wave): a second launch costs a microsecond more than the steps it saves
 
 struct TreeArgs {
     const uint16_t* q;
@@ -54,10 +56,10 @@ struct TreeArgs {
     float scale;      // times log2 e
 };
 
-// Tiles of a range, of a context of n keys in all: one range up to two tiles a wave, then a tile a wave at least.
-static __device__ __host__ inline int range_tiles(int n, int splits, int waves) {
+// Tiles of a range, of a context of n keys in all; at least a tile a wave.
+static __device__ __host__ inline int range_tiles(int n, int splits) {
     const int tiles = (n + TKEYS - 1) / TKEYS, even = (tiles + splits - 1) / splits;
-    return tiles <= 2 * waves ? 2 * waves : even > waves ? even : waves;
+    return tiles <= TONE ? TONE : even > TWAVES ? even : TWAVES;
 }
 
 // Broadcast of lane N of each row of 16 lanes to the row.
@@ -73,12 +75,12 @@ template <int B>
 __device__ __forceinline__ uint32_t byte_f32(uint32_t w) { return __float_as_uint(float(int8_t(w >> (8 * B)))); }
 
 template <int D, int RT, bool EIGHT>
-__global__ __launch_bounds__(64 * tree_waves(D, EIGHT), tree_waves(D, EIGHT) / 4) void attn_tree_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_kernel(const TreeArgs a) {
     constexpr int ROWB = EIGHT ? D : 2 * D;   // bytes of a cache row
     constexpr int KL = ROWB / 64;             // 16-byte loads of a lane from a K row
     constexpr int VW = ROWB / 64;             // words of a lane from a V row
     constexpr int DPL = D / 16;               // head-dimension indexes of a lane in V^T, and MFMAs of the second product
-    constexpr int ROWS = 16 * RT, SLICES = D / 32, WAVES = tree_waves(D, EIGHT), NT = 64 * WAVES;
+    constexpr int ROWS = 16 * RT, SLICES = D / 32, WAVES = TWAVES, NT = TNT;
     constexpr float NEG = -__builtin_inff();
     // how far scores may pass the reference, and where it is put below the largest score (both in powers of two)
     constexpr float PASS = EIGHT ? 6.0f : 8.0f, BELOW = EIGHT ? 8.0f : 0.0f;
@@ -103,7 +105,7 @@ __global__ __launch_bounds__(64 * tree_waves(D, EIGHT), tree_waves(D, EIGHT) / 4
         return;
     }
     const int pos = int(pos64), n = pos + a.T, tiles = (n + TKEYS - 1) / TKEYS;
-    const int per = range_tiles(n, a.splits, WAVES);
+    const int per = range_tiles(n, a.splits);
     const int first = range * per, last = min(tiles, first + per);
     if (first >= last) return;   // an empty range: the join knows
     const bool whole = per >= tiles;
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(64 * tree_waves(D, EIGHT), tree_waves(D, EIGHT) / 4
 // all that a thread reads is requested at once.  RANGES: at most.
 template <int D, int RANGES>
 __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
-                                                             int splits, int waves, const int64_t* pos_dev, int64_t pos0) {
+                                                             int splits, const int64_t* pos_dev, int64_t pos0) {
     constexpr int PARTS = JNT / (D / 4), PER = (RANGES + PARTS - 1) / PARTS;
     __shared__ float s_num[PARTS][D];
     const int lane = threadIdx.x & 63, p = threadIdx.x / (D / 4), e = threadIdx.x % (D / 4) * 4;
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __rest
     for (int u = 0; u < PER; ++u) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
     const int64_t pos = pos_dev ? pos_dev[0] : pos0;
     if (pos < 0 || pos > int64_t(rows) - T) return;   // zeros, written
-    const int n = int(pos) + T, per = range_tiles(n, splits, waves), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
+    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
     if (ranges == 1) return;
     const bool mine = lane < ranges && ml.y != 0.0f;   // (0: a range of which the query sees nothing)
     const float mx = wave_max(mine ? ml.x : -__builtin_inff()), w = mine ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
@@ -509,11 +511,11 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __rest
 template <int D, int RT>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
     const unsigned combos = unsigned(a.hk) * a.splits, grid = (combos + TXCDS - 1) / TXCDS * TXCDS * a.blocks;
-    if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(64 * tree_waves(D, a.ks)), 0, st>>>(a);
-    else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(64 * tree_waves(D, a.ks)), 0, st>>>(a);
+    if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(TNT), 0, st>>>(a);
+    else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(TNT), 0, st>>>(a);
     if (a.splits == 1) return;
     const auto join = [&](auto ranges) {
-        attn_tree_join_kernel<D, decltype(ranges)::value><<<dim3(unsigned(a.T) * a.hq), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, tree_waves(D, a.ks), a.pos_dev,
+        attn_tree_join_kernel<D, decltype(ranges)::value><<<dim3(unsigned(a.T) * a.hq), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev,
                                                                                                         a.pos0);
     };
     if (a.splits <= 16) join(std::integral_constant<int, 16>{});
@@ -529,9 +531,13 @@ static int tree_blocks(int qrows, int d) { return qrows <= 16 || d == 256 ? 1 : 
 
 extern "C" int scmx_attn_tree_splits(int T, int n, int hq, int hk, int d) {
     if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
-    const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), keys = (d == 256 ? 4 : 8) * TKEYS;
-    const int64_t combos = int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)), most = 256 / combos, ranges = (int64_t(n) + keys - 1) / keys;
-    return n <= 2 * keys || most < 1 ? 1 : int(ranges < most ? (ranges < 64 ? ranges : 64) : most < 64 ? most : 64);
+    const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), tiles = int((int64_t(n) + TKEYS - 1) / TKEYS);
+    if (tiles <= TONE) return 1;
+    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, which the join likes better (94 tiles:
+    // 24 ranges 11.3 us, 16 10.9).
+    const int64_t most = 256 / (int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)));
+    const int even = (tiles + TWAVES - 1) / TWAVES, ranges = even > 16 && even <= 32 ? 16 : even < 64 ? even : 64;
+    return most < 1 ? 1 : ranges < most ? ranges : int(most);
 }
 
 extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void* vcache, const float* kscale, const float* vscale,
