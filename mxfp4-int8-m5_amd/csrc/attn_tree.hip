@@ -508,18 +508,58 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __rest
     *reinterpret_cast<uint32_t*>(out + size_t(blockIdx.x) * D + 2 * threadIdx.x) = f32_to_bf16x2(lo * inv, hi * inv);
 }
 
+// The same for up to 8 ranges and a wave a row, four rows a workgroup: the parts of a row meet across lanes.  64 tokens of 32 heads, four
+// ranges of 6000 rows 22.9 -> 21.0 us with the attention; with 16 ranges a wave has too much in a row (one token, 4000 rows 8.5 -> 9.0).
+template <int D>
+__global__ __launch_bounds__(JNT) void attn_tree_join_rows_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
+                                                                  int splits, const int64_t* pos_dev, int64_t pos0) {
+    constexpr int LANES = D / 4, PARTS = 64 / LANES, PER = 8 / PARTS;
+    const int lane = threadIdx.x & 63, p = lane / LANES, e = lane % LANES * 4;
+    const unsigned all = unsigned(T) * hq, row = min(blockIdx.x * (JNT / 64) + threadIdx.x / 64, all - 1);   // (the last one again)
+    const float* num0 = part + size_t(row) * splits * D + e;
+    const float2 ml = reinterpret_cast<const float2*>(part + size_t(all) * splits * D)[size_t(row) * splits + min(lane % 8, splits - 1)];
+    f32x4 v[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+        if (u == 0 || u * PARTS < splits) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
+    const int64_t pos = pos_dev ? pos_dev[0] : pos0;
+    if (pos < 0 || pos > int64_t(rows) - T) return;   // zeros, written
+    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
+    if (ranges == 1) return;
+    const bool mine = lane % 8 < ranges && ml.y != 0.0f;   // (0: a range of which the query sees nothing)
+    const float mx = wave_max(mine ? ml.x : -__builtin_inff()), w = mine ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
+    const float den = wave_sum(mine && lane < 8 ? w * ml.y : 0.0f), inv = den == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den);
+    f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        if (u > 0 && u * PARTS >= splits) break;
+        const int s = p + u * PARTS;
+        const float f = __shfl(w, s, WAVE), there = __shfl(mine ? 1.0f : 0.0f, s, WAVE);
+        if (there != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(f, v[u][i], num[i]);
+        }
+    }
+#pragma unroll
+    for (int off = LANES; off < 64; off <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) num[i] += __shfl_xor(num[i], off, WAVE);
+    if (p == 0) *reinterpret_cast<u32x2*>(out + size_t(row) * D + e) = u32x2{f32_to_bf16x2(num[0] * inv, num[1] * inv), f32_to_bf16x2(num[2] * inv, num[3] * inv)};
+}
+
 template <int D, int RT>
 static void launch_tree(const TreeArgs& a, hipStream_t st) {
     const unsigned combos = unsigned(a.hk) * a.splits, grid = (combos + TXCDS - 1) / TXCDS * TXCDS * a.blocks;
     if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(TNT), 0, st>>>(a);
     else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(TNT), 0, st>>>(a);
     if (a.splits == 1) return;
-    const auto join = [&](auto ranges) {
-        attn_tree_join_kernel<D, decltype(ranges)::value><<<dim3(unsigned(a.T) * a.hq), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev,
-                                                                                                        a.pos0);
-    };
-    if (a.splits <= 16) join(std::integral_constant<int, 16>{});
-    else join(std::integral_constant<int, 64>{});
+    const unsigned rows = unsigned(a.T) * a.hq;
+    if (a.splits <= 8)
+        attn_tree_join_rows_kernel<D><<<dim3((rows + JNT / 64 - 1) / (JNT / 64)), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
+    else if (a.splits <= 16)
+        attn_tree_join_kernel<D, 16><<<dim3(rows), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
+    else
+        attn_tree_join_kernel<D, 64><<<dim3(rows), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
 }
 
 }  // namespace scmx

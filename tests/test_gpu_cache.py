@@ -191,7 +191,8 @@ def check_attention(out, q, cache, masks, pos, scale, eight):
 # one and several blocks of query rows, rows past the last query, a range per tile group and empty ranges
 ATTEND = [(1, 1, 1, 64, 0, 1), (1, 16, 8, 128, 300, None), (1, 14, 2, 64, 31, 1), (2, 2, 1, 128, 30, 2), (7, 14, 2, 64, 901, None), (16, 16, 8, 128, 1000, 3),
           (17, 2, 2, 128, 31, 1), (33, 4, 4, 128, 64, 1), (64, 8, 2, 128, 500, None), (64, 32, 2, 64, 95, 2), (5, 16, 4, 256, 256, None), (64, 4, 2, 256, 33, 2),
-          (64, 3, 3, 128, 0, 1), (40, 8, 1, 128, 1, 64), (3, 8, 8, 256, 2500, 9), (12, 5, 1, 64, 2047, 7), (1, 32, 8, 128, 5000, 20)]
+          (64, 3, 3, 128, 0, 1), (40, 8, 1, 128, 1, 64), (3, 8, 8, 256, 2500, 9), (12, 5, 1, 64, 2047, 7), (1, 32, 8, 128, 5000, 20),
+          (9, 4, 2, 128, 700, 64), (2, 6, 2, 256, 1200, 40)]
 
 
 @pytest.mark.gpu
@@ -284,6 +285,29 @@ def test_scores_that_grow_and_fall_along_the_rows(C, eight):
             c = make_cache(rnd, False, hk, pos + T, d)
             c[0][:] = (shape / d ** 0.5)[:, None].to(BF)
         check_attention(C.attn_tree(q, *c[:2], pos, None, *c[2:], splits=4), q, c, chain, pos, d ** -0.5, eight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -30, 2.0 ** 20, 2.0 ** 60])
+def test_queries_of_any_size(C, eight, size):
+    """Queries far outside half precision's range, small ones beside large ones, and one of infinities beside finite ones."""
+    T, hq, hk, d, pos = 6, 4, 2, 128, 200
+    rnd = gen(21)
+    c = make_cache(rnd, eight, hk, pos + T, d)
+    q = rnd(T, hq, d)
+    q[1] *= 2.0 ** -12
+    q = (q * size).to(BF).transpose(0, 1)
+    chain = [(1 << (i + 1)) - 1 for i in range(T)]
+    check_attention(C.attn_tree(q, *c[:2], pos, None, *c[2:], scale=0.09 / size), q, c, chain, pos, 0.09 / size, eight)
+    if size == 2.0 ** 20:
+        q = rnd(T, hq, d).to(BF).transpose(0, 1)
+        bad = q.clone()
+        bad[:, 2, 5] = float("inf")
+        a, b = (C.attn_tree(x, *c[:2], pos, None, *c[2:]) for x in (q, bad))
+        assert torch.isnan(b[2]).any()
+        b[2] = a[2]
+        check_attention(b, q, c, chain, pos, d ** -0.5, eight)
 
 
 @pytest.mark.gpu
