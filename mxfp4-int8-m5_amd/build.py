@@ -64,7 +64,7 @@ def build_binding():
     import sysconfig
     from torch.utils import cpp_extension as ext
     inc = ["-I" + p for p in [*ext.include_paths(), sysconfig.get_paths()["include"], os.path.join(ROCM, "include")]]
-    libs = ["-L" + p for p in ext.library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+    libs = ["-L" + p for p in ext.library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
     _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *inc,
           os.path.join(CSRC, "torch_binding.cpp"), "-o", BINDING, "-L" + HERE, "-l:libscmx.so", "-Wl,-rpath,$ORIGIN", *libs])
     return BINDING

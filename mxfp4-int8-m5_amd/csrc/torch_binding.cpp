@@ -10,13 +10,15 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/empty_strided.h>
+#include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
 #include <exception>
 #include <initializer_list>
+#include <optional>
 #include <tuple>
 #include <type_traits>
 #include <utility>
@@ -301,7 +303,12 @@ bool ints_of(PyObject* const* args, std::initializer_list<int> at) {
         if (!PyLong_CheckExact(args[i])) return false;
     return true;
 }
-at::TensorOptions like(const at::Tensor& t, at::ScalarType type) { return at::TensorOptions().dtype(type).device(t.device()); }
+// Outputs straight from torch's GPU allocator (every value is written; at::empty's dispatch takes half a microsecond more), and
+// workspaces without a tensor around them.
+at::Tensor fresh(const at::Tensor& like, at::ScalarType type, at::IntArrayRef size) {
+    return at::Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt));
+}
+c10::DataPtr scratch(size_t bytes) { return c10::hip::HIPCachingAllocator::get()->allocate(bytes); }
 void* stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
 // cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, kscale, vscale, depth)
@@ -324,7 +331,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
         int rc;
         {
             const NoGil released;
-            q = at::empty_strided({hq, L, d}, {d, hq * d, 1}, like(*y, at::ScalarType::BFloat16));
+            q = at::Tensor(at::detail::empty_strided_cuda({hq, L, d}, {d, hq * d, 1}, at::ScalarType::BFloat16, y->device()));
             const auto bf = [](const at::Tensor* t) { return static_cast<const uint16_t*>(t->data_ptr()); };
             rc = scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), float(PyFloat_AS_DOUBLE(args[3])), static_cast<uint16_t*>(q.data_ptr()), c.k->data_ptr(),
                                   c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), int(L), int(hq), int(hk), int(d), static_cast<const float*>(freq->data_ptr()), depth, dev, pos,
@@ -356,15 +363,15 @@ PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int splits = args[8] != Py_None ? convert<int>(args[8]) : scmx_attn_tree_splits(int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
         if (splits < 1 || splits > 64) Py_RETURN_NONE;
         const float scale = args[7] == Py_None ? float(1.0 / std::sqrt(double(d))) : float(PyFloat_AS_DOUBLE(args[7]));
-        at::Tensor out, work;
+        at::Tensor out;
         int rc;
         {
             const NoGil released;
-            out = at::empty({T, hq * d}, like(q, at::ScalarType::BFloat16));
-            if (splits > 1) work = at::empty({splits * T * hq * (d + 2)}, like(q, at::ScalarType::Float));
+            out = fresh(q, at::ScalarType::BFloat16, {T, hq * d});
+            const c10::DataPtr work = scratch(splits > 1 ? size_t(splits * T * hq * (d + 2)) * sizeof(float) : 0);
             rc = scmx_attn_tree(static_cast<const uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), mask, dev, pos,
                                 static_cast<uint16_t*>(out.data_ptr()), int(T), int(hq), int(c.hk), int(d), int(c.rows), scale,
-                                splits > 1 ? static_cast<float*>(work.data_ptr()) : nullptr, splits, stream());
+                                splits > 1 ? static_cast<float*>(work.get()) : nullptr, splits, stream());
         }
         if (rc != SCMX_OK) return status("scmx_attn_tree", rc);
         return THPVariable_Wrap(std::move(out));
@@ -385,8 +392,8 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
         int rc;
         {
             const NoGil released;
-            k = at::empty({c.hk, rows, c.d}, like(*c.k, at::ScalarType::BFloat16));
-            v = at::empty({c.hk, rows, c.d}, like(*c.k, at::ScalarType::BFloat16));
+            k = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
+            v = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
             rc = scmx_cache_read(static_cast<const int8_t*>(c.k->data_ptr()), static_cast<const int8_t*>(c.v->data_ptr()), c.scale(c.ks), c.scale(c.vs),
                                  static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()), int(c.hk), int(c.d), int(c.rows), int(row0), int(rows), stream());
         }
@@ -445,17 +452,17 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
             !optional_of(args[4], at::ScalarType::Float, T, u) || !optional_of(args[5], at::ScalarType::Float, T * V, draft))
             Py_RETURN_NONE;
         const size_t need = scmx_verify_workspace(int(T), int(V), int(levels));
-        at::Tensor path, count, next, work;
+        at::Tensor path, count, next;
         int rc;
         {
             const NoGil released;
-            path = at::empty({T}, like(*logits, at::ScalarType::Int));
-            count = at::empty({1}, like(*logits, at::ScalarType::Int));
-            next = at::empty({1}, like(*logits, at::ScalarType::Long));
-            work = at::empty({int64_t(need)}, like(*logits, at::ScalarType::Byte));
+            path = fresh(*logits, at::ScalarType::Int, {T});
+            count = fresh(*logits, at::ScalarType::Int, {1});
+            next = fresh(*logits, at::ScalarType::Long, {1});
+            const c10::DataPtr work = scratch(need);
             rc = scmx_verify_drafts(static_cast<const int64_t*>(tokens->data_ptr()), static_cast<const int32_t*>(parents->data_ptr()), logits->data_ptr(), f32, draft,
                                     PyFloat_AS_DOUBLE(args[3]), u, static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()),
-                                    static_cast<int64_t*>(next.data_ptr()), int(T), int(V), int(levels), work.data_ptr(), need, stream());
+                                    static_cast<int64_t*>(next.data_ptr()), int(T), int(V), int(levels), work.get(), need, stream());
         }
         if (rc != SCMX_OK) return status("scmx_verify_drafts", rc);
         PyObject *a = THPVariable_Wrap(std::move(path)), *b = THPVariable_Wrap(std::move(count)), *c = THPVariable_Wrap(std::move(next));
