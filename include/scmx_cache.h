@@ -36,7 +36,7 @@ int scmx_cache_read(const int8_t* kcache, const int8_t* vcache, const float* ksc
 /* Row pos + j takes what row pos + path[j] held before the call, for j < *count, in every one of `layers` caches: the accepted
  * line of a tree moved together.  path int32 [T], any order, repeats allowed; an entry outside 0 .. T - 1 leaves its row, *count
  * is held to 0 .. T.  caches: HOST array of layers * (2 or 4) device pointers, a layer's K, V (and with eight != 0 their scales),
- * read before the call returns.  layers <= 1024.  With pos_dev, a position whose rows do not fit moves nothing. */
+ * read before the call returns; no pointer twice.  layers <= 1024.  With pos_dev, a position whose rows do not fit moves nothing. */
 int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d, int cache_rows, const int32_t* path,
                     const int32_t* count, int T, const int64_t* pos_dev, int64_t pos0, void* stream);
 
@@ -44,7 +44,7 @@ int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d
  * the rows below pos; row pos + j is seen by node i if bit j of mask[i] is set (mask NULL: j <= i, a chain).  A node that sees
  * nothing gets zeros; what a node does not see does not reach its result, infinities and NaN among it.  T = 1 is the decode
  * step's attention over an 8-bit cache.  With pos_dev, a position whose rows do not fit the cache gives zeros.
- * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16, 32 or 64 query rows; more than one needs
+ * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16 or 32 query rows; more than one needs
  * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches.
  * scmx_attn_tree_splits: how many to take for n rows in all (the cache's, where the position is on the device); 1 for arguments that
  * scmx_attn_tree refuses. */

@@ -1,7 +1,7 @@
 // Attention of a tree of drafted tokens (1..64 of them) against a KV cache in bf16 or 8 bits (include/scmx_cache.h, scmx_attn_tree).
 //
 // The tokens' query heads that share a KV head are the rows of one matrix product, so that a cache row is read once for all of
-// them: row r is token r / group, head r % group of the group.  A wave owns 16, 32 or 64 rows and walks tiles of 32 keys with a running
+// them: row r is token r / group, head r % group of the group.  A wave owns 16 or 32 rows and walks tiles of 32 keys with a running
 // reference (the softmax's maximum), sums in float32.  Both products are transposed,
 //     S^T = K Q^T  (16x16x32 MFMA: rows = keys, columns = queries),   O^T = V^T P^T  (rows = head dimension, columns = queries),
 // so that a query is a lane column (lane % 16) in both, its statistics sit in the lanes that need them, and the S^T
@@ -9,7 +9,9 @@
 // 16t + 4g + r of the tile, and V is read with the same key order.  The contraction over the head dimension may take any order
 // too, and takes the one in which a lane's 16-byte load of a K row is its operand.  A lane reads DPL = d / 16 consecutive values of eight V
 // rows and turns them in registers (byte permutes); MFMA i then yields head-dimension indexes DPL * row + i.  So nothing
-// is staged: no LDS, no barrier in the loop, every wave streams its own keys with the next tile's loads in flight.
+// is staged: no LDS, no barrier in the loop, every wave streams its own keys with the next tile's loads in flight.  Bound by reading the cache from
+// some ten thousand rows on (one token, 40000 rows of 8 x 128 in 8 bits: 4.7 TB/s), by latency and two launches below, and with many
+// tokens by a step's chain of products, exponentials and conversions (64 tokens of 32 heads: a wave's tile takes 1 us).
 //
 // 8 bits: K codes become bf16 (exact; q stays as it is), the row's scale multiplies the score.  V codes become half precision
 // (exact), and the row's scale goes into the weight, w = p * scale, through the exponent: w = exp2(score + log2(scale) - reference).
@@ -56,9 +58,10 @@ struct TreeArgs {
     float scale;      // times log2 e
 };
 
+static __device__ __host__ inline int tiles_of(int n) { return n / TKEYS + (n % TKEYS != 0); }   // (n up to 2^31 - 1)
 // Tiles of a range, of a context of n keys in all; at least a tile a wave.
 static __device__ __host__ inline int range_tiles(int n, int splits) {
-    const int tiles = (n + TKEYS - 1) / TKEYS, even = (tiles + splits - 1) / splits;
+    const int tiles = tiles_of(n), even = (tiles + splits - 1) / splits;
     return tiles <= TONE ? TONE : even > TWAVES ? even : TWAVES;
 }
 
@@ -104,7 +107,7 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
                 if (row0 + i / D < rows_all) a.out[out_row(row0 + i / D) * D + i % D] = 0;
         return;
     }
-    const int pos = int(pos64), n = pos + a.T, tiles = (n + TKEYS - 1) / TKEYS;
+    const int pos = int(pos64), n = pos + a.T, tiles = tiles_of(n);
     const int per = range_tiles(n, a.splits);
     const int first = range * per, last = min(tiles, first + per);
     if (first >= last) return;   // an empty range: the join knows
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __rest
     for (int u = 0; u < PER; ++u) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
     const int64_t pos = pos_dev ? pos_dev[0] : pos0;
     if (pos < 0 || pos > int64_t(rows) - T) return;   // zeros, written
-    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
+    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = tiles_of(n), ranges = (tiles + per - 1) / per;
     if (ranges == 1) return;
     const bool mine = lane < ranges && ml.y != 0.0f;   // (0: a range of which the query sees nothing)
     const float mx = wave_max(mine ? ml.x : -__builtin_inff()), w = mine ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
@@ -524,7 +527,7 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_rows_kernel(const float* _
         if (u == 0 || u * PARTS < splits) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
     const int64_t pos = pos_dev ? pos_dev[0] : pos0;
     if (pos < 0 || pos > int64_t(rows) - T) return;   // zeros, written
-    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = (n + TKEYS - 1) / TKEYS, ranges = (tiles + per - 1) / per;
+    const int n = int(pos) + T, per = range_tiles(n, splits), tiles = tiles_of(n), ranges = (tiles + per - 1) / per;
     if (ranges == 1) return;
     const bool mine = lane % 8 < ranges && ml.y != 0.0f;   // (0: a range of which the query sees nothing)
     const float mx = wave_max(mine ? ml.x : -__builtin_inff()), w = mine ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
@@ -571,7 +574,7 @@ static int tree_blocks(int qrows, int d) { return qrows <= 16 || d == 256 ? 1 : 
 
 extern "C" int scmx_attn_tree_splits(int T, int n, int hq, int hk, int d) {
     if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
-    const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), tiles = int((int64_t(n) + TKEYS - 1) / TKEYS);
+    const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), tiles = tiles_of(n);
     if (tiles <= TONE) return 1;
     // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, which the join likes better (94 tiles:
     // 24 ranges 11.3 us, 16 10.9).

@@ -2,6 +2,7 @@
 // prompt's attention, and the accepted rows of a tree of drafts moved together (include/scmx_cache.h).
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/scmx_cache.h"
@@ -305,6 +306,13 @@ extern "C" int scmx_cache_keep(const uint64_t* caches, int layers, int eight, in
             set_error("cache_keep: layer %d has a null or misaligned pointer", i / each);
             return SCMX_ERR_ARG;
         }
+    uint64_t sorted[4 * 1024];   // the same rows moved twice at once would race
+    std::copy(caches, caches + layers * each, sorted);
+    std::sort(sorted, sorted + layers * each);
+    if (std::adjacent_find(sorted, sorted + layers * each) != sorted + layers * each) {
+        set_error("cache_keep: a cache is given twice");
+        return SCMX_ERR_ARG;
+    }
     for (int l0 = 0; l0 < layers; l0 += KEEP_LAYERS) {
         KeepArgs a{};
         const int n = layers - l0 < KEEP_LAYERS ? layers - l0 : KEEP_LAYERS;

@@ -76,7 +76,8 @@ int main() {
     expect(scmx_cache_read(i8(0), i8(1), f32(2), f32(3), u16(4), u16(5), 8, 128, 100, 4, 97, nullptr), SCMX_ERR_ARG, "cache_read past the cache");
     expect(scmx_cache_read(i8(0), i8(1), nullptr, f32(3), u16(4), u16(5), 8, 128, 100, 0, 1, nullptr), SCMX_ERR_ARG, "cache_read without a scale");
 
-    std::vector<uint64_t> t(4 * 1024, uint64_t(uintptr_t(p(3))));
+    std::vector<uint64_t> t(4 * 1024);
+    for (size_t i = 0; i < t.size(); ++i) t[i] = uint64_t(uintptr_t(p(3))) + 4096 * (i * 1531 % t.size());
     expect_valid(scmx_cache_keep(t.data(), 1024, 1, 8, 128, 100, i32(0), i32(1), 64, nullptr, 36, nullptr), "cache_keep, 1024 layers");
     expect_valid(scmx_cache_keep(t.data(), 28, 0, 8, 256, 100, i32(0), i32(1), 1, i64(2), 0, nullptr), "cache_keep");
     expect(scmx_cache_keep(t.data(), 0, 0, 8, 256, 100, i32(0), i32(1), 1, nullptr, 0, nullptr), SCMX_OK, "cache_keep of no layers");
@@ -84,9 +85,11 @@ int main() {
     expect(scmx_cache_keep(t.data(), 28, 0, 8, 256, 100, i32(0), i32(1), 64, nullptr, 37, nullptr), SCMX_ERR_ARG, "cache_keep past the cache");
     t[7] = 0;
     expect(scmx_cache_keep(t.data(), 28, 0, 8, 256, 100, i32(0), i32(1), 4, nullptr, 0, nullptr), SCMX_ERR_ARG, "cache_keep with a null layer");
+    t[7] = t[6];
+    expect(scmx_cache_keep(t.data(), 28, 0, 8, 256, 100, i32(0), i32(1), 4, nullptr, 0, nullptr), SCMX_ERR_ARG, "cache_keep with a cache twice");
     t[7] = t[6] + 4;
     expect(scmx_cache_keep(t.data(), 28, 0, 8, 256, 100, i32(0), i32(1), 4, nullptr, 0, nullptr), SCMX_ERR_ARG, "cache_keep with a misaligned layer");
-    t[7] = t[6];
+    t[7] = uint64_t(uintptr_t(p(3))) + 4096 * (7 * 1531 % t.size());
 
     const auto attend = [&](int T, int hq, int hk, int d, int rows, int64_t pos, float scale, float* work, int splits, float* ks = nullptr, float* vs = nullptr) {
         return scmx_attn_tree(u16(0), p(1), p(2), ks, vs, i64(3), nullptr, pos, u16(4), T, hq, hk, d, rows, scale, work, splits, nullptr);

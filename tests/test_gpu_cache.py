@@ -399,7 +399,8 @@ def test_what_is_refused(C):
     p, one = torch.arange(4, device="cuda", dtype=torch.int32), torch.ones(1, device="cuda", dtype=torch.int32)
     C.cache_keep([], p, one, 0)
     for o in (([(k, v, ks, vs)], p, one, 13), ([(k, v, ks, vs)], p.long(), one, 0), ([(k, v, None, None)], p, one, 0), ([(k, v, ks, vs), (b(hk, rows, d), b(hk, rows, d), None, None)], p, one, 0),
-              ([(k[:, ::2], v[:, ::2], ks[:, ::2], vs[:, ::2])], p, one, 0), ([(k, v, ks, vs)], torch.arange(65, device="cuda", dtype=torch.int32), one, 0)):
+              ([(k[:, ::2], v[:, ::2], ks[:, ::2], vs[:, ::2])], p, one, 0), ([(k, v, ks, vs)], torch.arange(65, device="cuda", dtype=torch.int32), one, 0), ([(k, v, ks, vs)] * 2, p, one, 0),
+              ([(k, k, ks, vs)], p, one, 0)):
         with pytest.raises(ValueError):
             C.cache_keep(*o)
 

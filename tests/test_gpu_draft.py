@@ -145,6 +145,25 @@ def test_random_numbers_near_a_border_and_far_tails(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [262144, 262145, 300001, 4194304])
+def test_vocabularies_of_more_chunks_than_a_wave_has_lanes(D, V):
+    T = 3 if V < 400000 else 2
+    rng = np.random.default_rng(V)
+    logits = rng.normal(size=(T, V)).astype(np.float32)
+    logits[:, -3:] += 6   # the last chunk counts
+    best = logits.argmax(1)
+    q = np.exp(logits + 0.5 * rng.normal(size=(T, V)).astype(np.float32))
+    q = (q / q.sum(1, keepdims=True)).astype(np.float32)
+    parents = [-1, 0, 0][:T]
+    for tokens in ([0, int(best[0]), 5][:T], [0, 7, V - 1][:T]):
+        assert run(D, logits, tokens, parents, torch.float32) == O.verify(logits, tokens, parents)
+        for k in range(3):
+            u = rng.random(T).astype(np.float32) * (1.0 if k else 0.01)
+            for draft in (None, q):
+                assert run(D, logits, tokens, parents, torch.float32, 1.1, u, draft, 2) == O.verify(logits, tokens, parents, 1.1, u, draft, 2)
+
+
+@pytest.mark.gpu
 def test_parents_that_are_none(D):
     """Numbers that name no earlier node are nobody's children; nothing is read outside."""
     V = 100
