@@ -351,6 +351,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             else pz[r] = a.z[c];
             m[r] = pm[r];
         }
+#pragma unroll 1
         for (int c = 64 + lane; c < a.chunks; c += 64)
 #pragma unroll
             for (int r = 0; r < PER; ++r) m[r] = fmaxf(m[r], a.m[size_t(min(wave + WAVES * r, a.T - 1)) * a.chunks + c]);
@@ -375,43 +376,50 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 z[r] = lane < a.chunks ? pz[r] * weight(pm[r], m[r], a.inv_t, s_table) : 0.0;
                 if (wave + WAVES * r < a.T) s_w[wave + WAVES * r][lane] = z[r];
             }
-            for (int c = 64 + lane; c < a.chunks; c += 64)
-#pragma unroll
-                for (int r = 0; r < PER; ++r) {
-                    const size_t i = size_t(min(wave + WAVES * r, a.T - 1)) * a.chunks + c;
-                    z[r] += a.z[i] * weight(a.m[i], m[r], a.inv_t, s_table);
-                }
 #pragma unroll
             for (int r = 0; r < PER; ++r) z[r] = wave_sum64(z[r]);
 #pragma unroll
-            for (int r = 0; r < PER; ++r) {
-                const int row = wave + WAVES * r;
-                if (row >= a.T) break;
-                if (lane == 0) {
-                    s_m[row] = m[r];
-                    s_z[row] = z[r];
-                    s_level[row][0] = 0;
+            for (int r = 0; r < PER; ++r)
+                if (lane == 0 && wave + WAVES * r < a.T) {
+                    s_m[wave + WAVES * r] = m[r];
+                    s_z[wave + WAVES * r] = z[r];
+                    s_level[wave + WAVES * r][0] = 0;
                 }
-                if (a.levels == 0) continue;
-                double ak = 1.0 / z[r], bk = 0.0;
-                int level = 0;   // the last one that left something
+        }
+    }
+    if (!GREEDY && a.chunks > 64) {   // the chunks past the lanes
+#pragma unroll 1
+        for (int row = wave; row < a.T; row += WAVES) {
+            double more = 0.0;
+#pragma unroll 1
+            for (size_t i = size_t(row) * a.chunks + 64 + lane; i < size_t(row + 1) * a.chunks; i += 64) more += a.z[i] * weight(a.m[i], s_m[row], a.inv_t, s_table);
+            more = wave_sum64(more);
+            if (lane == 0) s_z[row] += more;
+        }
+    }
+    if (!GREEDY && a.levels > 0) {
+#pragma unroll 1
+        for (int row = wave; row < a.T; row += WAVES) {
+            double ak = 1.0 / s_z[row], bk = 0.0;   // (this wave's own)
+            int level = 0;   // the last one that left something
+            if (lane == 0) {
+                s_a[row][0] = ak;
+                s_b[row][0] = bk;
+            }
+            const int kids = min(a.levels, int(__popcll(__ballot(node && parent == row))));
+#pragma unroll 1
+            for (int l = 1; l <= kids; ++l) {
+                const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
+                double s = 0.0;
+#pragma unroll 1
+                for (int c = lane; c < a.chunks; c += 64) s += ps[c];
+                s = wave_sum64(s);
+                next_level(s, ak, bk);
+                if (s > 0.0) level = l;
                 if (lane == 0) {
-                    s_a[row][0] = ak;
-                    s_b[row][0] = bk;
-                }
-                const int kids = min(a.levels, int(__popcll(__ballot(node && parent == row))));
-                for (int l = 1; l <= kids; ++l) {
-                    const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
-                    double s = 0.0;
-                    for (int c = lane; c < a.chunks; c += 64) s += ps[c];
-                    s = wave_sum64(s);
-                    next_level(s, ak, bk);
-                    if (s > 0.0) level = l;
-                    if (lane == 0) {
-                        s_a[row][l] = ak;
-                        s_b[row][l] = bk;
-                        s_level[row][l] = level;
-                    }
+                    s_a[row][l] = ak;
+                    s_b[row][l] = bk;
+                    s_level[row][l] = level;
                 }
             }
         }
@@ -478,6 +486,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 return w;
             };
             double own = 0.0;
+#pragma unroll 1
             for (int k = 0; k < K; ++k) own += part(lane * K + k);
             const double upto = wave_scan64(own);
             const double total = lane_of(upto, 63), target = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), 0))) * total;
@@ -486,7 +495,8 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             if (lane == who) {
                 double run = upto - own, base = run;
                 int chunk = lane * K;
-                for (int k = 0; k < K; ++k) {
+#pragma unroll 1
+                for (int k = 0; K > 1 && k < K; ++k) {
                     const double w = part(lane * K + k);
                     if (w > 0.0) {
                         chunk = lane * K + k;
