@@ -31,7 +31,7 @@ struct VerifyArgs {
     int32_t* count;
     int64_t* next;
     int T, V, chunks, levels;
-    double inv_t;      // 1 / temperature
+    double rate;       // 64 / (ln 2 temperature)
     bool logits_vec, draft_vec;
     double* z;         // [T][chunks]: sums of a chunk relative to its largest logit (greedy: int32, where that is)
     double* s;         // [levels][T][chunks]: S_1 ...
@@ -57,31 +57,32 @@ __device__ const double EXP2_64[64] = {
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
 
-// exp(x), x <= 0, to some 1e-15 (2e-14 at -200): x = k ln 2 / 64 + r, |r| <= 0.0054, exp(r) by its series to r^5 (r^6 / 720 = 4e-17),
-// 2^(k / 64) from the table and the exponent.  Half of the time of the stats kernel is this arithmetic; a series to r^11 of the whole
-// fraction, without a table, took a third more instructions.
-__device__ __forceinline__ double exp_neg(double x, const double* table) {
-    const double n = rint(x * 92.33248261893657), r = __builtin_fma(n, -0.010830424696249145, x);   // (-inf: whatever, and 0 at the end)
-    double p = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
+// 2^(t / 64), t <= 0, to some 1e-15 (1e-14 at t = -10000): t = k + f, |f| <= 1/2, 2^(f / 64) by the series of exp(f ln 2 / 64) to the fifth
+// power (the sixth is 4e-17), 2^(k / 64) from the table and the exponent.  Below 2^-1074: 0.  Half of the time of the stats kernel is
+// this arithmetic (60 nodes of 151936: 11.6 us; a series to the eleventh power without a table 18.5).
+__device__ __forceinline__ double exp2_64(double t, const double* table) {
+    constexpr double L = 0.010830424696249145;   // ln 2 / 64
+    t = fmax(t, -75000.0);
+    const double n = rint(t), f = t - n;
+    double p = __builtin_fma(f, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+    p = __builtin_fma(p, f, L * L * L / 6.0);
+    p = __builtin_fma(p, f, L * L / 2.0);
+    p = __builtin_fma(p, f, L);
+    p = __builtin_fma(p, f, 1.0);
     const int k = int(n);
-    const double v = __longlong_as_double(__double_as_longlong(p * table[k & 63]) + ((long long)(k >> 6) << 52));
-    return x < -700.0 ? 0.0 : v;
+    return __builtin_ldexp(p * table[k & 63], k >> 6);
 }
 // A logit's weight relative to the largest, m: 1 for the largest itself, also where that is infinite.
-__device__ __forceinline__ double weight(float x, float m, double inv_t, const double* table) {
+__device__ __forceinline__ double weight(float x, float m, double rate, const double* table) {
     if (!(fabsf(m) <= 3.4028234e38f)) return x == m ? 1.0 : 0.0;   // (the same for a whole row)
-    return exp_neg((double(x) - double(m)) * inv_t, table);
+    return exp2_64((double(x) - double(m)) * rate, table);
 }
 // The same of N logits of which the first `there` are some (the others are -inf): straight code where the largest is finite.
 template <int N>
-__device__ __forceinline__ void weights(const float* x, float m, double inv_t, const double* table, int there, double* w) {
+__device__ __forceinline__ void weights(const float* x, float m, double rate, const double* table, int there, double* w) {
     if (fabsf(m) <= 3.4028234e38f) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = exp_neg((double(x[i]) - double(m)) * inv_t, table);
+        for (int i = 0; i < N; ++i) w[i] = exp2_64((double(x[i]) - double(m)) * rate, table);
     } else {
         for (int i = 0; i < N; ++i) w[i] = i < there && x[i] == m ? 1.0 : 0.0;
     }
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         double w[8];
-        weights<8>(x[t], m, a.inv_t, s_table, a.V - (v0 + t * 8 * VNT), w);
+        weights<8>(x[t], m, a.rate, s_table, a.V - (v0 + t * 8 * VNT), w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) z += w[i];
     }
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, i
     for (int c = threadIdx.x; c < a.chunks; c += VNT) m = fmaxf(m, pm[c]);
     m = group_max(m, s_m);
     double z = 0.0;
-    for (int c = threadIdx.x; c < a.chunks; c += VNT) z += pz[c] * weight(pm[c], m, a.inv_t, s_table);
+    for (int c = threadIdx.x; c < a.chunks; c += VNT) z += pz[c] * weight(pm[c], m, a.rate, s_table);
     double ak = 1.0 / group_sum64(z, s_z), bk = 0.0;
     for (int l = 1; l < level; ++l) {
         const double* ps = a.s + (size_t(l - 1) * a.T + row) * a.chunks;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(VNT) void verify_level_kernel(const VerifyArgs a, i
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         double w[8];
-        weights<8>(x[t], m, a.inv_t, s_table, a.V - (v0 + t * 8 * VNT), w);
+        weights<8>(x[t], m, a.rate, s_table, a.V - (v0 + t * 8 * VNT), w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += fmax(ak * w[i] - (bk + 1.0) * double(q[t][i]), 0.0);   // (beyond the vocabulary q is 0)
     }
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             __syncthreads();   // the table
 #pragma unroll
             for (int r = 0; r < PER; ++r) {
-                z[r] = lane < a.chunks ? pz[r] * weight(pm[r], m[r], a.inv_t, s_table) : 0.0;
+                z[r] = lane < a.chunks ? pz[r] * weight(pm[r], m[r], a.rate, s_table) : 0.0;
                 if (wave + WAVES * r < a.T) s_w[wave + WAVES * r][lane] = z[r];
             }
 #pragma unroll
@@ -392,7 +393,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         for (int row = wave; row < a.T; row += WAVES) {
             double more = 0.0;
 #pragma unroll 1
-            for (size_t i = size_t(row) * a.chunks + 64 + lane; i < size_t(row + 1) * a.chunks; i += 64) more += a.z[i] * weight(a.m[i], s_m[row], a.inv_t, s_table);
+            for (size_t i = size_t(row) * a.chunks + 64 + lane; i < size_t(row + 1) * a.chunks; i += 64) more += a.z[i] * weight(a.m[i], s_m[row], a.rate, s_table);
             more = wave_sum64(more);
             if (lane == 0) s_z[row] += more;
         }
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
     }
     __syncthreads();
     if (wave == 0) {
-        const double e = known && !GREEDY ? weight(x, s_m[max(parent, 0)], a.inv_t, s_table) : 0.0, qd = known && a.draft ? double(q) : 1.0;
+        const double e = known && !GREEDY ? weight(x, s_m[max(parent, 0)], a.rate, s_table) : 0.0, qd = known && a.draft ? double(q) : 1.0;
         const bool right = GREEDY && node && token == s_best[max(parent, 0)];
         int cur = 0, tried = 0;
         uint64_t taken = 1, gone = 0;
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             const auto part = [&](int c) {   // of the residual, in the units of the sums that it was taken from
                 if (c >= a.chunks) return 0.0;
                 if (lvl > 0) return a.s[(size_t(lvl - 1) * a.T + cur) * a.chunks + c];
-                double w = c < 64 ? s_w[cur][c] : a.z[size_t(cur) * a.chunks + c] * weight(a.m[size_t(cur) * a.chunks + c], s_m[cur], a.inv_t, s_table);
+                double w = c < 64 ? s_w[cur][c] : a.z[size_t(cur) * a.chunks + c] * weight(a.m[size_t(cur) * a.chunks + c], s_m[cur], a.rate, s_table);
                 for (int i = 0; i < gones; ++i)
                     if (s_gone[i] / VCHUNK == c) w = fmax(w - s_gone_e[i], 0.0);
                 return w;
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         const int v = v0 + i;
         r[i] = 0.0;
         if (v < a.V) {
-            const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.inv_t, s_table);
+            const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.rate, s_table);
             if (lvl > 0) {   // (before its normalisation, as the chunks' sums are)
                 r[i] = fmax(s_a[cur][lvl - 1] * e - (s_b[cur][lvl - 1] + 1.0) * double(a.draft[size_t(cur) * a.V + v]), 0.0);
             } else {
@@ -597,7 +598,7 @@ extern "C" int scmx_verify_drafts(const int64_t* tokens, const int32_t* parents,
         return SCMX_ERR_WORKSPACE;
     }
     const size_t cells = size_t(T) * chunks;
-    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels, greedy ? 1.0 : 1.0 / temperature,
+    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels, greedy ? 1.0 : 92.33248261893657 / temperature,
                  uintptr_t(logits) % 16 == 0 && V % (logits_f32 ? 4 : 8) == 0, uintptr_t(draft) % 16 == 0 && V % 4 == 0,
                  static_cast<double*>(workspace), static_cast<double*>(workspace) + cells, nullptr};
     a.m = reinterpret_cast<float*>(a.s + cells * levels);
