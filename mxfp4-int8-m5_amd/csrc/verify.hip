@@ -165,6 +165,11 @@ __device__ __forceinline__ double wave_scan64(double v) {
     const int row = (threadIdx.x & 63) >> 4;
     return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? a + b : (a + b) + c);
 }
+// What a lane wrote to LDS before is what the wave's other lanes read after.
+__device__ __forceinline__ void wave_sees() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 // Over the workgroup; every thread gets the result.  `s` holds one entry a wave.
 __device__ __forceinline__ float group_max(float v, float* s) {
     v = wave_max32(v);
@@ -388,6 +393,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 }
         }
     }
+    wave_sees();
     if (!GREEDY && a.chunks > 64) {   // the chunks past the lanes
 #pragma unroll 1
         for (int row = wave; row < a.T; row += WAVES) {
@@ -397,6 +403,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             more = wave_sum64(more);
             if (lane == 0) s_z[row] += more;
         }
+        wave_sees();
     }
     if (!GREEDY && a.levels > 0) {
 #pragma unroll 1
@@ -471,6 +478,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             s_gone[__popcll(gone & below)] = token;
             s_gone_e[__popcll(gone & below)] = e;
         }
+        wave_sees();
         if (lane == 0) {
             a.count[0] = count;
             if (GREEDY) a.next[0] = s_best[cur];
@@ -517,47 +525,56 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
     }
     if (GREEDY) return;
     __syncthreads();
-    // ---- that chunk again, four tokens a thread
-    const int cur = s_last, gones = s_gones, lvl = s_lvl;
-    const double target = s_total;
+    // ---- that chunk again, four tokens a thread.  Its sum may be no more than the rounding of one from which all likely tokens were taken:
+    // then the first likely token of the chunks behind it, or the last of those before it.
+    const int cur = s_last, gones = s_gones, lvl = s_lvl, first = s_chunk;
+    const double target = s_total, base = s_base;
     const float m = s_m[cur];
-    double upto[4], r[4], sum = 0.0;
-    int some = -1, over = -1;   // the thread's last token that has any probability, its first above the target
-    const int v0 = s_chunk * VCHUNK + 4 * tid;
+    int chunk = first, token_at = -1;
+#pragma unroll 1
+    for (int step = 1; token_at < 0 && chunk >= 0;) {   // (the same in every thread)
+        double upto[4], r[4], sum = 0.0;
+        int some = -1, over = -1;   // the thread's last token that has any probability, its first above the target
+        const int v0 = chunk * VCHUNK + 4 * tid;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int v = v0 + i;
-        r[i] = 0.0;
-        if (v < a.V) {
-            const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.rate, s_table);
-            if (lvl > 0) {   // (before its normalisation, as the chunks' sums are)
-                r[i] = fmax(s_a[cur][lvl - 1] * e - (s_b[cur][lvl - 1] + 1.0) * double(a.draft[size_t(cur) * a.V + v]), 0.0);
-            } else {
-                r[i] = e;
-                for (int j = 0; j < gones; ++j)
-                    if (s_gone[j] == v) r[i] = 0.0;
+        for (int i = 0; i < 4; ++i) {
+            const int v = v0 + i;
+            r[i] = 0.0;
+            if (v < a.V) {
+                const double e = weight(logit<F32>(a.logits, size_t(cur) * a.V + v), m, a.rate, s_table);
+                if (lvl > 0) {   // (before its normalisation, as the chunks' sums are)
+                    r[i] = fmax(s_a[cur][lvl - 1] * e - (s_b[cur][lvl - 1] + 1.0) * double(a.draft[size_t(cur) * a.V + v]), 0.0);
+                } else {
+                    r[i] = e;
+                    for (int j = 0; j < gones; ++j)
+                        if (s_gone[j] == v) r[i] = 0.0;
+                }
             }
+            sum += r[i];
+            upto[i] = sum;
+            if (r[i] > 0.0) some = v;
         }
-        sum += r[i];
-        upto[i] = sum;
-        if (r[i] > 0.0) some = v;
-    }
-    const double before = s_base + group_scan(sum, s_wave) - sum;
+        const double before = base + group_scan(sum, s_wave) - sum;
 #pragma unroll
-    for (int i = 3; i >= 0; --i)
-        if (r[i] > 0.0 && before + upto[i] > target) over = v0 + i;
-    // lanes and waves hold the chunk in order: the first wave's first lane, or the last's last (atomics on one word took 15 us)
-    const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
-    if (lane == 0) {
-        s_over[wave] = overs ? __builtin_amdgcn_readlane(over, __builtin_ctzll(overs)) : -1;
-        s_some[wave] = somes ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(somes)) : -1;
-    }
-    __syncthreads();
-    if (wave == 0) {
+        for (int i = 3; i >= 0; --i)
+            if (r[i] > 0.0 && (chunk == first ? before + upto[i] > target : step > 0)) over = v0 + i;
+        // lanes and waves hold the chunk in order: the first wave's first lane, or the last's last (atomics on one word took 15 us)
+        const uint64_t overs = __ballot(over >= 0), somes = __ballot(some >= 0);
+        if (lane == 0) {
+            s_over[wave] = overs ? __builtin_amdgcn_readlane(over, __builtin_ctzll(overs)) : -1;
+            s_some[wave] = somes ? __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(somes)) : -1;
+        }
+        __syncthreads();
         const int o = lane < WAVES ? s_over[lane] : -1, h = lane < WAVES ? s_some[lane] : -1;
         const uint64_t any = __ballot(o >= 0), rest = __ballot(h >= 0);
-        if (lane == 0) a.next[0] = any ? __builtin_amdgcn_readlane(o, __builtin_ctzll(any)) : rest ? __builtin_amdgcn_readlane(h, 63 - __builtin_clzll(rest)) : 0;
+        token_at = any ? __builtin_amdgcn_readlane(o, __builtin_ctzll(any)) : rest ? __builtin_amdgcn_readlane(h, 63 - __builtin_clzll(rest)) : -1;
+        chunk += step;
+        if (chunk == a.chunks) {
+            step = -1;
+            chunk = first - 1;
+        }
     }
+    if (tid == 0) a.next[0] = max(token_at, 0);
 }
 
 }  // namespace scmx

@@ -145,6 +145,26 @@ def test_random_numbers_near_a_border_and_far_tails(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("there,u", [(2 * 4096 + 5, 0.0), (2 * 4096 + 5, 0.99999994), (3, 0.0), (3, 0.99999994), (4096 + 77, 0.0), (4096 + 77, 0.99999994)])
+def test_a_chunk_whose_likely_tokens_were_all_refused(D, there, u):
+    """What is left of its sum is rounding, and no token of it is ever the next one."""
+    V, T = 3 * 4096, 17
+    for seed in range(12):
+        rng = np.random.default_rng(seed)
+        logits = np.full((T, V), -np.inf, np.float32)
+        tokens = np.concatenate([[0], 4096 + rng.choice(4096, 16, replace=False)])
+        tokens = tokens[tokens != there]
+        parents = [-1] + [0] * (len(tokens) - 1)
+        logits = logits[:len(tokens)]
+        logits[0, tokens[1:]] = 3 * rng.normal(size=len(tokens) - 1)
+        logits[0, there] = 0.0
+        us = np.full(len(tokens), 0.99999994, np.float32)
+        us[0] = u
+        assert O.verify(logits, tokens, parents, 1.0, us) == ([0], there)
+        assert run(D, logits, tokens, parents, torch.float32, 1.0, us) == ([0], there), seed
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [262144, 262145, 300001, 4194304])
 def test_vocabularies_of_more_chunks_than_a_wave_has_lanes(D, V):
     T = 3 if V < 400000 else 2
