@@ -414,8 +414,9 @@ class DraftQwen3(DecodeQwen3):
     together, in one pass over the weights, and as many of them are accepted as the model's own probabilities allow, so that a step
     yields between one and T tokens.  tokens int64 [T]: token 0 is the sequence's newest one, not yet in the cache (a plain
     decode step's input), the others are drafts, whose places `tree` (sc_draft.DraftTree) says.  Where the drafts come from is the caller's.
-    graphs=True captures the step, verification and the move of the accepted rows included, once per tree, cache and kind
-    of verification (temperature, with or without a draft), for as long as that cache is used; what is returned is fresh."""
+    graphs=True captures the step, verification and the move of the accepted rows included, once per number of nodes, cache and kind
+    of verification (temperature, with or without a draft), for as long as that cache is used: the tree's shape is an input of
+    the graph like its tokens, so every step may bring another one.  What is returned is fresh."""
 
     def __init__(self, fused, graphs=False):
         super().__init__(fused, graphs=graphs)
@@ -434,20 +435,29 @@ class DraftQwen3(DecodeQwen3):
     def hidden(self, tokens, tree, cache, pos):
         """Final normed hidden states [T, D] of the tree's nodes, whose keys and values go to the caches' rows pos .. pos + T - 1 (pos: int,
         or an int64 device tensor); the caches' offsets stay."""
+        self._check_tokens(tokens, tree)
+        return self._hidden(tokens, tree.T, tree.depth, tree.mask, cache, pos)
+
+    def _check_tokens(self, tokens, tree):
+        if tokens.numel() != tree.T or tokens.dim() != 1 or tokens.dtype != torch.int64:
+            raise ValueError("tokens are int64, one for every node of the tree")
+
+    def _hidden(self, tokens, T, depth, mask, cache, pos):
         f, a = self.f, self.args
         h = f.embed.index_select(0, tokens)
         for c, (nw, ws) in zip(cache, f.layers):
             k, v, ks, vs = C.tensors(c)
             y = self._linear(h, ws["qkv"], 1, nw=nw["input_layernorm"])
-            q = C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, tree.T, a.num_attention_heads, a.num_key_value_heads, a.head_dim,
-                              k, v, pos, f.inv_freq, ks, vs, tree.depth)
-            h = self._linear(C.attn_tree(q, k, v, pos, tree.mask, ks, vs), ws["o"], 2, h)
+            q = C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, T, a.num_attention_heads, a.num_key_value_heads, a.head_dim,
+                              k, v, pos, f.inv_freq, ks, vs, depth)
+            h = self._linear(C.attn_tree(q, k, v, pos, mask, ks, vs), ws["o"], 2, h)
             h = self._linear(self._linear(h, ws["gu"], 3, nw=nw["post_attention_layernorm"]), ws["down"], 2, h)
         return S.rmsnorm(h, f.norm, f.eps)
 
-    def _draft_step(self, tokens, tree, cache, pos, temperature, uniforms, draft):
-        logits = self.f.logits(self.hidden(tokens, tree, cache, pos))
-        path, count, token = sc_draft.verify_drafts(logits, tokens, tree.parents, temperature, uniforms, draft, tree.siblings)
+    def _draft_step(self, tokens, shape, siblings, cache, pos, temperature, uniforms, draft):
+        mask, depth, parents = sc_draft.DraftTree.unpack(shape)
+        logits = self.f.logits(self._hidden(tokens, tokens.numel(), depth, mask, cache, pos))
+        path, count, token = sc_draft.verify_drafts(logits, tokens, parents, temperature, uniforms, draft, siblings)
         C.cache_keep([C.tensors(c) for c in cache], path, count, pos)
         return path, count, token, logits
 
@@ -459,22 +469,24 @@ class DraftQwen3(DecodeQwen3):
         if off + tree.T > cache[0].k.shape[1]:
             raise ValueError("KV cache is full")
         tokens = tokens.reshape(-1)
-        if tokens.numel() != tree.T or tokens.dtype != torch.int64:
-            raise ValueError("tokens are int64, one for every node of the tree")
+        self._check_tokens(tokens, tree)
+        if temperature == 0:
+            uniforms = draft = None
+        siblings = tree.siblings if draft is not None else None
         S.set_format(f.fmt)
         if self.graphs is None:
-            out = self._draft_step(tokens, tree, cache, off, temperature, uniforms, draft)
-        else:
+            out = self._draft_step(tokens, tree.packed, siblings, cache, off, temperature, uniforms, draft)
+        else:   # a graph's inputs are copied into its own, which would convert them
+            given = [(t, shape) for t, shape in ((uniforms, (tree.T,)), (draft, (tree.T, f.lm_head.shape[0]))) if t is not None]
+            if (temperature != 0 and uniforms is None) or any(t.shape != shape or t.dtype != torch.float32 for t, shape in given):
+                raise ValueError("uniforms are float32 [T], draft float32 [T, V]")
             self.pos.fill_(off)
-            given = [t for t in (uniforms, draft) if t is not None]
 
-            def fn(tokens, *rest):
-                rest = list(rest)
-                u = rest.pop(0) if uniforms is not None else None
-                return self._draft_step(tokens, tree, cache, self.pos, temperature, u, rest.pop(0) if draft is not None else None)
+            def fn(tokens, shape, uniforms=None, draft=None):
+                return self._draft_step(tokens, shape, siblings, cache, self.pos, temperature, uniforms, draft)
 
-            key = ("draft", tuple(tree.parent_list), float(temperature), uniforms is not None, draft is not None)
-            out = tuple(t.clone() for t in self._replay(key, fn, [tokens, *given], owner=cache))
+            key = ("draft", tree.T, siblings, float(temperature))
+            out = tuple(t.clone() for t in self._replay(key, fn, [tokens, tree.packed, *(t for t, _ in given)], owner=cache))
         n = off + int(out[1])
         for c in cache:
             c.offset = n

@@ -10,7 +10,8 @@ MAX_SIBLINGS = 16   # children of a node that are tried against a draft's probab
 
 class DraftTree:
     """The shape of a tree of drafted tokens: parents[i] < i, -1 for node 0, the sequence's newest token.  On the device: `parents` and
-    `depth` int32 [T], `mask` int64 [T] (a node sees itself and its line back to the root).  `siblings`: the most children of a node."""
+    `depth` int32 [T], `mask` int64 [T] (a node sees itself and its line back to the root), views of `packed`.  `siblings`: the most children
+    of a node."""
 
     def __init__(self, parents, device="cuda"):
         parents = [int(p) for p in parents]
@@ -22,9 +23,15 @@ class DraftTree:
             mask.append(mask[p] | 1 << i)
             kids[p] += 1
         self.T, self.parent_list, self.depth_list, self.siblings = len(parents), parents, depth, max(kids)
-        self.parents = torch.tensor(parents, dtype=torch.int32, device=device)
-        self.depth = torch.tensor(depth, dtype=torch.int32, device=device)
-        self.mask = torch.tensor([m - (1 << 64) if m >> 63 else m for m in mask], dtype=torch.int64, device=device)
+        mask = torch.tensor([m - (1 << 64) if m >> 63 else m for m in mask], dtype=torch.int64)
+        self.packed = torch.cat([mask.view(torch.int32), torch.tensor(depth + parents, dtype=torch.int32)]).to(device)
+        self.mask, self.depth, self.parents = self.unpack(self.packed)
+
+    @staticmethod
+    def unpack(packed):
+        """(mask, depth, parents): views of int32 [4 T]."""
+        T = packed.numel() // 4
+        return packed[:2 * T].view(torch.int64), packed[2 * T:3 * T], packed[3 * T:]
 
     @classmethod
     def chain(cls, T, device="cuda"):

@@ -123,6 +123,48 @@ def test_sampled_drafted_steps(tiny, graphs):
         assert (path[:int(count)].tolist(), int(nxt)) == want
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_every_step_may_bring_another_tree(tiny, temperature):
+    """Trees of one size that live for one step, with other tensors in their place afterwards: captured steps are the eager ones, to the bit."""
+    Q, args, state, packed = tiny
+    from mxfp4_int8_m5_amd.sc_draft import DraftTree
+    m = Q.FusedQwen3(args, state, packed)
+    runs = []
+    for graphs in (False, True):
+        rng = np.random.default_rng(5)
+        cache = m.make_cache(200, bits=8)
+        m.hidden(ids_of(args, 9, 2), cache)
+        dec, outs = Q.DraftQwen3(m, graphs=graphs), []
+        for step in range(8):
+            tree = DraftTree([-1] + [int(rng.integers(0, i)) for i in range(1, 6)])
+            u = torch.tensor(rng.random(6), dtype=torch.float32, device="cuda")
+            q = torch.tensor(rng.dirichlet(np.ones(args.vocab_size), 6), dtype=torch.float32, device="cuda") if step % 3 == 2 else None
+            tokens = torch.tensor(rng.integers(args.vocab_size, size=6), device="cuda")
+            outs += [t.cpu() for t in dec.step(tokens, tree, cache, temperature, u, q)]
+            del tree, u, q, tokens
+            junk = [torch.randint(0, 6, (n,), device="cuda", dtype=torch.int32) for n in (6, 12, 24, 6, 12, 24)]
+        runs.append(outs)
+        del junk
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_captured_step_refuses_what_an_eager_one_does(tiny):
+    Q, args, state, packed = tiny
+    from mxfp4_int8_m5_amd.sc_draft import DraftTree
+    m = Q.FusedQwen3(args, state, packed)
+    for graphs in (False, True):
+        cache = m.make_cache(40)
+        dec, tree, tokens = Q.DraftQwen3(m, graphs=graphs), DraftTree.chain(4), ids_of(args, 4, 1)
+        b = lambda *s, t=torch.float32: torch.full(s, 0.25, dtype=t, device="cuda")   # noqa: E731
+        V = args.vocab_size
+        dec.step(tokens, tree, cache, 0.5, b(4), b(4, V))
+        for bad in ((b(1), b(4, V)), (b(4, t=torch.float64), b(4, V)), (b(4), b(V)), (b(4), b(1, V)), (b(4), b(4, V, t=torch.bfloat16)), (None, b(4, V)), (None, None)):
+            with pytest.raises(ValueError):
+                dec.step(tokens, tree, cache, 0.5, *bad)
+        with pytest.raises(ValueError):
+            dec.hidden(ids_of(args, 5, 1), tree, cache, 0)
+
+
 def test_what_the_drivers_refuse(tiny):
     Q, args, state, packed = tiny
     from mxfp4_int8_m5_amd.sc_draft import DraftTree
