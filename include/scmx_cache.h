@@ -2,7 +2,7 @@
  * (device pointers, the caller's stream, no allocation, no synchronisation, no state, SCMX_ERR_* and scmx_last_error()).
  * The reference has none of these: its decode step takes one token, its cache holds the model's type.
  *
- * A cache is a K and a V tensor [hk, cache_rows, d], either bf16 (kscale = vscale = NULL) or INT8 with one float scale per row
+ * A cache is a K and a V tensor (two, not one twice) [hk, cache_rows, d], either bf16 (kscale = vscale = NULL) or INT8 with one float scale per row
  * (kscale, vscale [hk, cache_rows]): value = code * scale.  8-bit rows take d + 4 bytes where bf16 rows take 2 d.
  * A tree of drafted tokens has its T (1..64) nodes in rows pos .. pos + T - 1 behind the pos rows of the sequence, every node
  * after its parent, node 0 the sequence's newest token.  pos is *pos_dev when pos_dev != NULL (a device-resident position, so that a

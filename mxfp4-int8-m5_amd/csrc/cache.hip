@@ -249,6 +249,10 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
         set_error("cache_write: y, qn, kn, q and the caches must be 16-byte aligned");
         return SCMX_ERR_ARG;
     }
+    if (kcache == vcache || (kscale && kscale == vscale)) {
+        set_error("cache_write: K and V are one cache");
+        return SCMX_ERR_ARG;
+    }
     if (L == 0) return SCMX_OK;
     const WriteArgs a{acc, xscale, wscale, y, qn, kn, eps, q, {kcache, vcache}, {kscale, vscale}, L, hq, hk, inv_freq, depth, pos_dev, pos0, cache_rows};
     const int groups = CNT / (d / 8), turns = (hq + 2 * hk + groups - 1) / groups;

@@ -96,8 +96,9 @@ def cache_read(kcache, vcache, kscale, vscale, n, row0=0):
     out = _lib.native().cache_read(kcache, vcache, kscale, vscale, n, row0)
     if out is not None:
         return out
-    _check(kscale is not None and n >= 0, "rows of an 8-bit cache, none or more (a bf16 one is read as it is)")
+    _check(kscale is not None, "rows of an 8-bit cache (a bf16 one is read as it is)")
     hk, rows, d = _check_cache(kcache, vcache, kscale, vscale)
+    _check(0 <= n <= rows and 0 <= row0 <= rows - n, f"{n} rows from {row0} on do not fit a cache of {rows} rows")
     _on_device(kcache, vcache, kscale, vscale)
     k, v = (_lib.native().empty_bf16(kcache, hk, n, d) for _ in range(2))
     _lib.native().scmx_cache_read(kcache, vcache, kscale, vscale, k, v, hk, d, rows, int(row0), int(n))
@@ -143,7 +144,7 @@ def attn_tree(q, kcache, vcache, pos, mask=None, kscale=None, vscale=None, scale
     q = q.transpose(0, 1).contiguous()   # [T, hq, d]; no copy when q already is a view of it
     T, hq, d = q.shape
     hk, rows, dc = _check_cache(kcache, vcache, kscale, vscale)
-    _check(q.dtype == BF and dc == d and hq % hk == 0, "q is bfloat16 [hq, T, d], hq a multiple of hk")
+    _check(q.dtype == BF and dc == d and hk > 0 and hq % hk == 0, "q is bfloat16 [hq, T, d], hq a multiple of hk")
     _check(1 <= T <= MAX_NODES, "a tree has 1..64 nodes")
     _check(mask is None or (mask.dtype == torch.int64 and mask.numel() == T), "mask is int64 [T]")
     dev_pos, at = _position(pos)

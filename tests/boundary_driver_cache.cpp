@@ -55,6 +55,8 @@ int main() {
     const auto i64 = [&](int i) { return reinterpret_cast<int64_t*>(p(i)); };
     const auto i8 = [&](int i) { return reinterpret_cast<int8_t*>(p(i)); };
 
+    expect(scmx_cache_write(nullptr, nullptr, nullptr, u16(0), u16(1), u16(2), 1e-6f, u16(3), p(4), p(4), nullptr, nullptr, 1, 4, 2, 64, f32(8), nullptr, nullptr, 0, 16, nullptr),
+           SCMX_ERR_ARG, "write: keys and values in one cache");
     const auto write = [&](const uint16_t* y, float* ks, float* vs, int L, int hq, int hk, int d, int64_t pos, int rows, const int64_t* dev = nullptr) {
         return scmx_cache_write(nullptr, nullptr, nullptr, y, u16(1), u16(2), 1e-6f, u16(3), p(4), p(5), ks, vs, L, hq, hk, d, f32(8), nullptr, dev, pos, rows, nullptr);
     };

@@ -369,6 +369,20 @@ def test_other_streams_and_two_calls_at_once(C, eight):
 
 
 @pytest.mark.gpu
+def test_caches_that_are_one_or_empty_are_refused(C):
+    b = lambda *s, t=BF: torch.zeros(*s, dtype=t, device="cuda")   # noqa: E731
+    one, none = b(2, 16, 64), b(0, 16, 64)
+    with pytest.raises(ValueError, match="one cache"):
+        C.cache_write(b(4, 8 * 64), b(64), b(64), 1e-6, 4, 4, 2, 64, one, one, 0, b(32, t=torch.float32))
+    with pytest.raises(ValueError):
+        C.attn_tree(b(4, 1, 64), none, none, 0)
+    eight = b(2, 16, 64, t=torch.int8), b(2, 16, 64, t=torch.int8), b(2, 16, t=torch.float32), b(2, 16, t=torch.float32)
+    for n, row0 in ((2 ** 40, 0), (4, 13), (0, 17), (1, -1), (-1, 3)):   # before anything is allocated
+        with pytest.raises(ValueError):
+            C.cache_read(*eight, n, row0)
+
+
+@pytest.mark.gpu
 def test_what_is_refused(C):
     hq, hk, d, rows = 4, 2, 64, 16
     b = lambda *s, t=BF: torch.zeros(*s, dtype=t, device="cuda")   # noqa: E731
