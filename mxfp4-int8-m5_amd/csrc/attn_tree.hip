@@ -217,7 +217,7 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
     // step to arrive, and no second set of registers.
     for (int tile = first + wave; tile < last; tile += WAVES) {
         const int base = tile * TKEYS, next = min(tile + WAVES, last - 1);
-        const bool tail = base + TKEYS > pos;   // the tile reaches into the tree, or past the last row
+        const bool tail = base > pos - TKEYS;   // the tile reaches into the tree, or past the last row
         // ---- scores
         f32x4 s[RT][2];
 #pragma unroll
@@ -356,6 +356,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[(rt * 32 + 4 * e + g) * 16 + ln] = x[rt][e];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
                 for (; bad; bad &= bad - 1) {
                     const int at = __builtin_ctz(bad), key = base + 16 * (at / 16) + 4 * (at % 4) + at / 4 % 4;
                     const uint16_t* row = reinterpret_cast<const uint16_t*>(vb + size_t(key) * ROWB) + DPL * 4 * g;
