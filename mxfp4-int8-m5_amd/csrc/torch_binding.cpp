@@ -244,7 +244,7 @@ PyObject* gemv(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // ---- drafted tokens over a cache: sc_cache's and sc_draft's functions for the operands of every step, in one call as above ---------
 // (None where an operand is anything else: the caller's general way converts or refuses it.  16 tokens through 28 blocks'
-// caches, 29 calls that the host bounds: 313 us with checks and allocations in Python, see sc_cache, 140-151 here.)
+// caches, 29 calls that the host bounds: 313 us with checks and allocations in Python, see sc_cache, 140-157 here.)
 
 // A contiguous tensor of `type` on the current device; NULL: something else.  None is not one.
 const at::Tensor* local(PyObject* o, at::ScalarType type) {
