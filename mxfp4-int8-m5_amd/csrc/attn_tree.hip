@@ -245,7 +245,10 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
         // ---- in powers of two; masked
         float x[RT][8], inverse = 0.0f;
         if constexpr (EIGHT) {
-            const float vscale = scales == 0.0f && ln >= 8 ? 1.0f : scales;   // a row of zeros (scale 0) counts in the denominator alone
+            // A row of zeros (scale 0) counts in the denominator alone: it takes a scale below all that matter beside it, so that its score
+            // does not set the reference (as 1 it took the bits of rows of 1e-6), and no smaller, so that 2^31 such weights of up
+            // to 2^14, times 2^80, fit the denominator.
+            const float vscale = scales == 0.0f && ln >= 8 ? 0x1p-80f : scales;
             const float both = ln < 8 ? scales * a.scale : __builtin_amdgcn_logf(vscale);
             inverse = __builtin_amdgcn_rcpf(vscale);
             inverse = inverse == inverse ? inverse : 1.0f;   // (0 times NaN: the nodes that do not see the row)
