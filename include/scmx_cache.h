@@ -46,7 +46,7 @@ int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d
  * step's attention over an 8-bit cache.  With pos_dev, a position whose rows do not fit the cache gives zeros.
  * Over an 8-bit cache a row weighs by the product of its probability and its V row's scale, a half-precision number of which the
  * largest is 2^8 .. 2^14: products below 2^-22 of the largest lose bits, below 2^-39 they may vanish from the sum.  The denominator
- * is summed in float32 or more from the same products over the scales: a row whose product is below 2^-110 of another's may count as not
+ * is summed from the same products, in float32, over the scales: a row whose product is below 2^-110 of another's may count as not
  * seen.  V scales are positive and normal, or 0 for a row of zeros, which takes part as one with the scale 2^-80 would.  Over a
  * bf16 cache the probabilities are rounded to bf16, in the sum and in the denominator alike (2^-8 of sum p |v| at most).
  * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16 or 32 query rows; more than one needs

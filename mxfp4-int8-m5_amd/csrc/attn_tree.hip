@@ -88,7 +88,11 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
     // how far scores may pass the reference, and where it is put below the largest score (both in powers of two)
     constexpr float PASS = EIGHT ? 6.0f : 8.0f, BELOW = EIGHT ? 8.0f : 0.0f;
     __shared__ float s_o[WAVES][ROWS][D + 4];
-    __shared__ float2 s_ml[WAVES][ROWS];   // reference, denominator
+    // 8 bits: the denominators are sums of weights over scales, up to 2^14 / 2^-107 each, of any number of rows: tiles' sums in float32, the
+    // rest in float64 (30000 rows of 2^-98 overflow float32; the time is the same)
+    using Den = std::conditional_t<EIGHT, double, float>;
+    __shared__ float s_m[WAVES][ROWS];     // references
+    __shared__ Den s_l[WAVES][ROWS];       // denominators
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
     // blocks of the query rows of one range and KV head run on one XCD, behind one L2
@@ -203,14 +207,15 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
             for (int s = 0; s < SLICES; ++s) qf[rt][s] = *reinterpret_cast<const bf16x8*>(s_q + (16 * rt + ln) * QROW + q_at(s));
     }
     f32x4 o[RT][DPL], ones[RT];   // ones: sums of the rounded weights (bf16)
-    float m[RT], l[RT];
+    float m[RT];
+    Den l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
         for (int i = 0; i < DPL; ++i) o[rt][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         ones[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         m[rt] = NEG;
-        l[rt] = 0.0f;
+        l[rt] = 0;
     }
 
     // K of the next tile is requested when this one's scores stand, V when its product does: each has the other half of the
@@ -246,8 +251,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
         float x[RT][8], inverse = 0.0f;
         if constexpr (EIGHT) {
             // A row of zeros (scale 0) counts in the denominator alone: it takes a scale below all that matter beside it, so that its score
-            // does not set the reference (as 1 it took the bits of rows of 1e-6), and no smaller, so that 2^31 such weights of up
-            // to 2^14, times 2^80, fit the denominator.
+            // does not set the reference (as 1 it took the bits of rows of 1e-6), and no smaller, so that its weight is not below
+            // float32 beside large values.
             const float vscale = scales == 0.0f && ln >= 8 ? 0x1p-80f : scales;
             const float both = ln < 8 ? scales * a.scale : __builtin_amdgcn_logf(vscale);
             inverse = __builtin_amdgcn_rcpf(vscale);
@@ -319,12 +324,15 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
             }
         }
         if constexpr (EIGHT) {
+            float eight[RT] = {};   // (below 2^124)
             for_eight([&](auto e) __attribute__((always_inline)) {
                 constexpr int E = decltype(e)::value;
                 const float iv = row_lane<8 + E>(inverse);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) l[rt] = __builtin_fmaf(x[rt][E], iv, l[rt]);
+                for (int rt = 0; rt < RT; ++rt) eight[rt] = __builtin_fmaf(x[rt][E], iv, eight[rt]);
             }, std::make_integer_sequence<int, 8>{});
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) l[rt] += double(eight[rt]);
         }
         // ---- the tree's rows in bf16: a row that is not finite must not reach (0 times infinity) the queries that do not see it
         if (!EIGHT && tail) {
@@ -417,7 +425,6 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
     }
 
     // ---- the waves meet: their references first, so that what they leave in LDS only has to be added
-    float den[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if constexpr (EIGHT) {
@@ -426,27 +433,42 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
         } else {
             l[rt] = ones[rt][0];
         }
-        if (g == 0) s_ml[wave][16 * rt + ln] = float2{m[rt], l[rt]};
+        if (g == 0) {
+            s_m[wave][16 * rt + ln] = m[rt];
+            s_l[wave][16 * rt + ln] = l[rt];
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int r = 16 * rt + ln;
-        float2 ml[WAVES];
-        float mx = NEG;
+        float mw[WAVES], mx = NEG;
+        Den lw[WAVES], sum = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            ml[w] = s_ml[w][r];
-            mx = fmaxf(mx, ml[w].x);
+            mw[w] = s_m[w][r];
+            lw[w] = s_l[w][r];
+            mx = fmaxf(mx, mw[w]);
         }
-        den[rt] = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w)   // (l is 0 of a wave whose keys the query does not see)
-            if (ml[w].y != 0.0f) den[rt] = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[w].x - mx), ml[w].y, den[rt]);
-        float f = l[rt] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - mx);
-        if (whole) f *= den[rt] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den[rt]);   // (0: nothing was seen)
+            if (lw[w] != 0) {
+                if constexpr (EIGHT) sum = __builtin_fma(double(__builtin_amdgcn_exp2f(mw[w] - mx)), lw[w], sum);
+                else sum = __builtin_fmaf(__builtin_amdgcn_exp2f(mw[w] - mx), lw[w], sum);
+            }
+        float f = l[rt] == 0 ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - mx);
+        if (EIGHT && sum > 0x1p100) {   // rows of very small values: the sums in other units
+            sum *= 0x1p-64;
+            mx += 64.0f;
+#pragma unroll
+            for (int i = 0; i < DPL; ++i)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) o[rt][i][r4] *= 0x1p-64f;
+        }
+        const float den = float(sum);
+        if (whole) f *= den == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den);   // (0: nothing was seen)
         else if (wave == 0 && g == 0 && row0 + r < rows_all)
-            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, den[rt]};
+            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, den};
         if (row0 + r < rows_all) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)

@@ -62,6 +62,19 @@ def test_rows_of_zeros_count_in_the_denominator_alone(C, d, pos, splits, size, l
         check_relative(C.attn_tree(q, *c[:2], pos, bits(masks), *c[2:], splits=splits), q, c, masks, pos, d ** -0.5)
 
 
+@pytest.mark.parametrize("size", [2.0 ** -98, 2.0 ** -60, 1e-12, 2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("pos,splits", [(200, 1), (30000, 1), (30000, 8)])
+def test_values_of_any_size(C, size, pos, splits):
+    """The denominator holds as many rows of as small values as the append writes."""
+    T, hq, hk, d = 2, 4, 2, 128
+    rnd = gen(pos)
+    q = torch.ones(T, hq, d, device="cuda", dtype=torch.bfloat16).transpose(0, 1)
+    c = cache_of(rnd, hk, pos + T, d, size, 0, [])
+    for grow in (0.0, 12.0):   # scores that rise along the rows
+        c[2][:] += grow * float(np.log(2)) * torch.linspace(0, 1, pos + T, device="cuda") / (100 * d ** 0.5)
+        check_relative(C.attn_tree(q, *c[:2], pos, None, *c[2:], splits=splits), q, c, [1, 3], pos, d ** -0.5)
+
+
 def test_a_long_context_of_zeros(C):
     """All rows but one hold zeros, their scores rising: the one's share of them."""
     T, hq, hk, d, pos = 1, 2, 1, 64, 70000
