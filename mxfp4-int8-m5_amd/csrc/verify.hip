@@ -615,7 +615,7 @@ extern "C" int scmx_verify_drafts(const int64_t* tokens, const int32_t* parents,
         return SCMX_ERR_WORKSPACE;
     }
     const size_t cells = size_t(T) * chunks;
-    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels, greedy ? 1.0 : 92.33248261893657 / temperature,
+    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels, greedy ? 1.0 : 64.0 / M_LN2 / temperature,
                  uintptr_t(logits) % 16 == 0 && V % (logits_f32 ? 4 : 8) == 0, uintptr_t(draft) % 16 == 0 && V % 4 == 0,
                  static_cast<double*>(workspace), static_cast<double*>(workspace) + cells, nullptr};
     a.m = reinterpret_cast<float*>(a.s + cells * levels);
