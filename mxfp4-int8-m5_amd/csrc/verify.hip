@@ -5,7 +5,9 @@
 // follow S_{k+1} = sum max(a_k e - (b_k + 1) q, 0), a_{k+1} = a_k / S, b_{k+1} = (b_k + 1) / S.  None of it depends on which tokens
 // were drafted or taken, so one launch a level forms the sums of all nodes side by side, by chunks of the vocabulary, and the walk
 // itself is a single pass over the nodes with scalars.  The chunks' sums then say in which chunk the next token lies, and only
-// that chunk is looked at again.  Without a draft q is one-hot: the refused tokens' exponentials leave the sum.
+// that chunk is looked at again.  Without a draft q is one-hot: the refused tokens' exponentials leave the sum.  What remains is never
+// formed as a difference, which after refusals of nearly all probability would be rounding: the sums leave out the tokens of a
+// node's children, and the walk adds those that were not refused.
 // Everything is float64 (exponentials too): a sum of 150000 float32 probabilities is uncertain by more than the likelihood of most
 // tokens, and which token a random number names has to be the same for every order of summation.
 // Bound: float64 arithmetic and one reading of the logits (from the L2 again for each level); a few nodes, the launches.
@@ -33,7 +35,8 @@ struct VerifyArgs {
     int T, V, chunks, levels;
     double rate;       // 64 / (ln 2 temperature)
     bool logits_vec, draft_vec;
-    double* z;         // [T][chunks]: sums of a chunk relative to its largest logit (greedy: int32, where that is)
+    double* z;         // [T][chunks]: sums of a chunk relative to its largest logit, without a draft those of the tokens that no child
+                       // of the node holds (greedy: int32, where the largest is)
     double* s;         // [levels][T][chunks]: S_1 ...
     float* m;          // [T][chunks]: largest logits
 };
@@ -201,7 +204,10 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
     if (!GREEDY) copy_table(s_table);
     const size_t row = blockIdx.y;
     float x[2][8], m = -__builtin_inff();
-    const int v0 = blockIdx.x * VCHUNK + 8 * threadIdx.x;
+    const int v0 = blockIdx.x * VCHUNK + 8 * threadIdx.x, lane = threadIdx.x & 63;
+    const bool leaves = !GREEDY && !a.draft && lane < a.T;
+    const int parent = leaves ? a.parents[lane] : -1;
+    const int64_t held = leaves ? a.tokens[lane] - int64_t(blockIdx.x) * VCHUNK : -1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) logits8<F32>(a, row, v0 + t * 8 * VNT, x[t]);
 #pragma unroll
@@ -227,6 +233,16 @@ __global__ __launch_bounds__(VNT) void verify_stats_kernel(const VerifyArgs a) {
             reinterpret_cast<int32_t*>(a.z)[out] = at;
         }
         return;
+    }
+    uint64_t kids = __ballot(parent == int(blockIdx.y) && parent < lane && held >= 0 && held < VCHUNK);   // (the same in every wave)
+    while (kids) {
+        const int at = __builtin_amdgcn_readlane(int(held), __builtin_ctzll(kids));
+        kids &= kids - 1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (8 * int(threadIdx.x) + t * 8 * VNT + i == at) x[t][i] = __builtin_nanf("");   // weighs 0, whatever m is
     }
     double z = 0.0;
 #pragma unroll
@@ -321,22 +337,21 @@ template <bool F32, bool GREEDY>
 __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) {
     constexpr int WAVES = VWALK / 64, PER = VNODES / WAVES;
     __shared__ float s_m[VNODES];
-    __shared__ double s_z[VNODES], s_wave[WAVES], s_table[64], s_gone_e[VNODES], s_base, s_total;
+    __shared__ double s_z[VNODES], s_wave[WAVES], s_table[64], s_open_e[VNODES], s_base, s_total;
     __shared__ double s_w[GREEDY ? 1 : VNODES][64];   // the first 64 chunks' sums relative to the node's largest logit
     __shared__ double s_a[GREEDY ? 1 : VNODES][VLEVELS + 1], s_b[GREEDY ? 1 : VNODES][VLEVELS + 1];
     __shared__ int s_best[VNODES], s_level[GREEDY ? 1 : VNODES][VLEVELS + 1], s_last, s_lvl, s_gones, s_chunk, s_over[WAVES], s_some[WAVES];
-    __shared__ int64_t s_gone[VNODES];
+    __shared__ int s_gone[VNODES], s_open[VNODES], s_again[VNODES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (!GREEDY) copy_table(s_table);
-    // node `lane`: every wave knows the parents (it counts children), the first one the rest
+    // node `lane`: every wave knows the parents (it counts children) and tokens, the first one the rest
     const int parent = lane > 0 && lane < a.T ? a.parents[lane] : -1;
     const bool node = lane > 0 && lane < a.T && parent >= 0 && parent < lane;
-    int64_t token = -1;
+    const int64_t given = lane < a.T ? a.tokens[lane] : -1;
+    const bool known = node && given >= 0 && given < a.V;
+    const int token = known ? int(given) : -1 - lane;   // (one that no other node holds)
     float u = 0.0f, x = 0.0f, q = 0.0f;
-    bool known = false;
     if (wave == 0) {
-        if (node) token = a.tokens[lane];
-        known = node && token >= 0 && token < a.V;
         if (!GREEDY) {
             if (lane < a.T) u = a.uniforms[lane];
             if (known) x = logit<F32>(a.logits, size_t(parent) * a.V + token);
@@ -376,6 +391,12 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 if (lane == 0) s_best[row] = best;
             }
         } else {
+#pragma unroll
+            for (int r = 0; r < PER; ++r) {   // whether an earlier sibling holds the same token
+                const int c = wave + WAVES * r, pc = __builtin_amdgcn_readlane(parent, c), tc = __builtin_amdgcn_readlane(token, c);
+                const bool again = __ballot(lane < c && parent == pc && token == tc) != 0;
+                if (lane == 0) s_again[c] = again;
+            }
             __syncthreads();   // the table
 #pragma unroll
             for (int r = 0; r < PER; ++r) {
@@ -437,8 +458,11 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         const double e = known && !GREEDY ? weight(x, s_m[max(parent, 0)], a.rate, s_table) : 0.0, qd = known && a.draft ? double(q) : 1.0;
         const bool right = GREEDY && node && token == s_best[max(parent, 0)];
         int cur = 0, tried = 0;
-        uint64_t taken = 1, gone = 0;
-        double left = GREEDY ? 0.0 : s_z[0];
+        uint64_t taken = 1, gone = 0;   // gone: children of cur whose tokens were refused
+        const bool once = !GREEDY && !a.draft && known && !s_again[lane];
+        // what is left of cur's sum: the tokens that no child holds and, each once, those that are not gone
+        const auto rest = [&]() { return s_z[cur] + wave_sum64(once && parent == cur && !(gone >> lane & 1) ? e : 0.0); };
+        double left = GREEDY || a.draft ? 0.0 : rest();
         uint64_t kids = __ballot(node && parent == 0);
         const uint64_t yes = __ballot(right);
         while (kids) {   // children come after their parents
@@ -453,12 +477,14 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 take = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), c))) * qc < r;
                 ++tried;
             } else {
-                const int lo = __builtin_amdgcn_readlane(int(token), c), hi = __builtin_amdgcn_readlane(int(token >> 32), c);
-                const double ec = gone & __ballot(int(token) == lo && int(token >> 32) == hi) ? 0.0 : lane_of(e, c);
+                const double ec = gone >> c & 1 ? 0.0 : lane_of(e, c);
                 take = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), c))) * left < ec;
-                if (!take && ec > 0.0 && left - ec > 0.0) {
-                    left -= ec;
-                    gone |= 1ull << c;
+                if (!take && ec > 0.0) {
+                    const uint64_t before = gone;
+                    gone |= __ballot(parent == cur && token == __builtin_amdgcn_readlane(token, c));
+                    const double without = rest();
+                    if (without > 0.0) left = without;
+                    else gone = before;   // nothing would be left: it stays as it was
                 }
             }
             if (take) {
@@ -466,7 +492,7 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 taken |= 1ull << c;
                 gone = 0;
                 tried = 0;
-                left = GREEDY ? 0.0 : s_z[c];
+                if (!GREEDY && !a.draft) left = rest();
                 kids = __ballot(node && parent == c);
             }
         }
@@ -474,9 +500,11 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         const uint64_t below = (1ull << lane) - 1;
         if (taken >> lane & 1) a.path[__popcll(taken & below)] = lane;
         if (lane >= count && lane < a.T) a.path[lane] = -1;
-        if (gone >> lane & 1) {
-            s_gone[__popcll(gone & below)] = token;
-            s_gone_e[__popcll(gone & below)] = e;
+        const uint64_t open = __ballot(once && parent == cur && !(gone >> lane & 1));
+        if (gone >> lane & 1) s_gone[__popcll(gone & below)] = token;
+        if (open >> lane & 1) {
+            s_open[__popcll(open & below)] = token;
+            s_open_e[__popcll(open & below)] = e;
         }
         wave_sees();
         if (lane == 0) {
@@ -485,13 +513,13 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         }
         if (!GREEDY) {
             // ---- the chunk that the next token is in: lane i sums chunks i K .. (i + 1) K - 1
-            const int lvl = s_level[cur][tried], gones = int(__popcll(gone)), K = (a.chunks + 63) / 64;
+            const int lvl = s_level[cur][tried], gones = int(__popcll(gone)), opens = int(__popcll(open)), K = (a.chunks + 63) / 64;
             const auto part = [&](int c) {   // of the residual, in the units of the sums that it was taken from
                 if (c >= a.chunks) return 0.0;
                 if (lvl > 0) return a.s[(size_t(lvl - 1) * a.T + cur) * a.chunks + c];
                 double w = c < 64 ? s_w[cur][c] : a.z[size_t(cur) * a.chunks + c] * weight(a.m[size_t(cur) * a.chunks + c], s_m[cur], a.rate, s_table);
-                for (int i = 0; i < gones; ++i)
-                    if (s_gone[i] / VCHUNK == c) w = fmax(w - s_gone_e[i], 0.0);
+                for (int i = 0; i < opens; ++i)
+                    if (s_open[i] / VCHUNK == c) w += s_open_e[i];
                 return w;
             };
             double own = 0.0;
@@ -525,8 +553,8 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
     }
     if (GREEDY) return;
     __syncthreads();
-    // ---- that chunk again, four tokens a thread.  Its sum may be no more than the rounding of one from which all likely tokens were taken:
-    // then the first likely token of the chunks behind it, or the last of those before it.
+    // ---- that chunk again, four tokens a thread.  Against a draft its sum may be no more than rounding (of differences): then the first
+    // token of the chunks behind it that has any probability, or the last of those before it.
     const int cur = s_last, gones = s_gones, lvl = s_lvl, first = s_chunk;
     const double target = s_total, base = s_base;
     const float m = s_m[cur];

@@ -1,5 +1,5 @@
-"""Sampled verification at the borders of its decisions: random numbers a few 1e-13 to each side of one, at logits far apart,
-against the float64 walk (oracle/draft.py)."""
+"""Sampled verification at the borders of its decisions: random numbers a few 1e-13 to each side of one, at logits far apart, and what is
+left after refusals that took nearly all probability; against the float64 walk (oracle/draft.py)."""
 import numpy as np
 import pytest
 import torch
@@ -36,3 +36,44 @@ def test_random_numbers_beside_a_border_of_unlike_logits(D, temperature, drawn):
         assert (len(got[0]) == 2) == accept, (x, u)
         below += accept
     assert 0 < below < 24
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+def test_what_is_left_after_refusals_of_nearly_everything(D, chunked):   # noqa: F811
+    """Two refused tokens leave 2^-46 of the probability, half of it on a third: that one is decided by the rest's own sum, and so
+    is the token after it.  (A random number of 1 - 2^-24 refuses what leaves more than 2^-24.)"""
+    V = 9000
+    most = 0.99999994
+    for seed in range(16):
+        rng = np.random.default_rng(seed)
+        at = rng.choice(V, 400, replace=False) if chunked else rng.choice(4000, 400, replace=False)
+        logits = np.full((5, V), -np.inf, np.float32)
+        small = np.exp(0.5 * rng.normal(size=397))
+        row = np.concatenate([[0.0], [-22.5 * np.log(2)], [-45 * np.log(2)], np.log(small / small.sum()) - 45 * np.log(2)]).astype(np.float32)
+        logits[0, at] = row
+        logits[1:, 5] = 0.0
+        e = np.exp(row.astype(np.float64))
+        border = e[2] / e[2:].sum()
+        tokens, parents = [0, at[0], at[1], at[0], at[2]], [-1, 0, 0, 0, 0]   # (one of them a second time)
+        for side in (-1e-6, 1e-6):
+            u = [float(rng.random()), most, most, most, np.float32(border * (1 + side))]
+            want = O.verify(logits, tokens, parents, 1.0, u)
+            assert want[0] == ([0, 4] if side < 0 else [0])
+            assert run(D, logits, tokens, parents, torch.float32, 1.0, u) == want, (seed, side)
+
+
+@pytest.mark.parametrize("V", [40, 4096, 9000])
+def test_rows_without_a_finite_logit_and_drafted_tokens(D, V):   # noqa: F811
+    """Rows all -inf or NaN (every token counts alike) and rows with infinities, with children on some of their tokens."""
+    rng = np.random.default_rng(V)
+    for fill in (-np.inf, np.nan, 0.0):
+        for k in range(8):
+            logits = np.full((5, V), fill, np.float32)
+            if fill == 0.0:
+                logits[:, rng.choice(V, 7, replace=False)] = np.inf
+            kids = rng.choice(V, 4, replace=False) if fill != 0.0 else rng.choice(np.nonzero(np.isinf(logits[0]))[0], 4, replace=False)
+            u = rng.random(5).astype(np.float32)
+            if k % 2:
+                u[1:] = 0.99999994
+            tokens, parents = [0, *kids], [-1, 0, 0, 0, 0]
+            assert run(D, logits, tokens, parents, torch.float32, 0.7, u) == O.verify(logits, tokens, parents, 0.7, u)
