@@ -414,12 +414,26 @@ class DraftQwen3(DecodeQwen3):
     together, in one pass over the weights, and as many of them are accepted as the model's own probabilities allow, so that a step
     yields between one and T tokens.  tokens int64 [T]: token 0 is the sequence's newest one, not yet in the cache (a plain
     decode step's input), the others are drafts, whose places `tree` (sc_draft.DraftTree) says.  Where the drafts come from is the caller's.
-    graphs=True captures the step, verification and the move of the accepted rows included, once per number of nodes, cache and kind
-    of verification (temperature, with or without a draft), for as long as that cache is used: the tree's shape is an input of
-    the graph like its tokens, so every step may bring another one.  What is returned is fresh."""
+    graphs=True captures the step, verification and the move of the accepted rows included, once per number of nodes and kind of
+    verification: greedy, a temperature, or a temperature with a draft and the most children of a node.  Otherwise the tree's shape is
+    an input of the graph like its tokens, so every step may bring another one.  Kept are the graphs of the latest cache, and of the
+    TEMPERATURES latest temperatures; another cache or a fifth temperature drops the others' graphs and what they hold.  What is returned
+    is fresh."""
+
+    TEMPERATURES = 4
 
     def __init__(self, fused, graphs=False):
         super().__init__(fused, graphs=graphs)
+        self.temperatures = []   # with captured steps, the latest last
+
+    def _key(self, T, levels, temperature, cache):
+        """The key of a step's graph; drops the graphs of other caches, and of a temperature too many."""
+        if temperature != 0:
+            self.temperatures = [t for t in self.temperatures if t != temperature][1 - self.TEMPERATURES:] + [temperature]
+        for key, entry in list(self.graphs.items()):
+            if key[0] == "draft" and (entry[3] is not cache or key[3] not in (0.0, *self.temperatures)):
+                del self.graphs[key]
+        return "draft", T, levels, temperature
 
     def _linear(self, x, w, epi, res=None, nw=None):
         """A linear on a few rows x [T, K], RMSNorm with weight nw first.  One row takes the norm in the GEMV's prologue, several rows
@@ -472,7 +486,7 @@ class DraftQwen3(DecodeQwen3):
         self._check_tokens(tokens, tree)
         if temperature == 0:
             uniforms = draft = None
-        siblings = tree.siblings if draft is not None else None
+        siblings = None if draft is None else min(max(tree.siblings, 1), sc_draft.MAX_SIBLINGS)
         S.set_format(f.fmt)
         if self.graphs is None:
             out = self._draft_step(tokens, tree.packed, siblings, cache, off, temperature, uniforms, draft)
@@ -485,7 +499,7 @@ class DraftQwen3(DecodeQwen3):
             def fn(tokens, shape, uniforms=None, draft=None):
                 return self._draft_step(tokens, shape, siblings, cache, self.pos, temperature, uniforms, draft)
 
-            key = ("draft", tree.T, siblings, float(temperature))
+            key = self._key(tree.T, siblings, float(temperature), cache)
             out = tuple(t.clone() for t in self._replay(key, fn, [tokens, tree.packed, *(t for t, _ in given)], owner=cache))
         n = off + int(out[1])
         for c in cache:
