@@ -413,7 +413,8 @@ class DraftQwen3(DecodeQwen3):
     """A decode step for a tree of drafted tokens from a FusedQwen3 with epilogue="gemm": all T (1..64) go through the model
     together, in one pass over the weights, and as many of them are accepted as the model's own probabilities allow, so that a step
     yields between one and T tokens.  tokens int64 [T]: token 0 is the sequence's newest one, not yet in the cache (a plain
-    decode step's input), the others are drafts, whose places `tree` (sc_draft.DraftTree) says.  Where the drafts come from is the caller's.
+    decode step's input), the others are drafts, whose places `tree` (sc_draft.DraftTree) says; one outside the vocabulary (-1: no draft for
+    a place) is never taken.  Where the drafts come from is the caller's.
     graphs=True captures the step, verification and the move of the accepted rows included, once per number of nodes and kind of
     verification: greedy, a temperature, or a temperature with a draft and the most children of a node.  Otherwise the tree's shape is
     an input of the graph like its tokens, so every step may bring another one.  Kept are the graphs of the latest cache, and of the
@@ -458,7 +459,7 @@ class DraftQwen3(DecodeQwen3):
 
     def _hidden(self, tokens, T, depth, mask, cache, pos):
         f, a = self.f, self.args
-        h = f.embed.index_select(0, tokens)
+        h = f.embed.index_select(0, tokens.clamp(0, f.embed.shape[0] - 1))   # (a draft outside the vocabulary is never taken)
         for c, (nw, ws) in zip(cache, f.layers):
             k, v, ks, vs = C.tensors(c)
             y = self._linear(h, ws["qkv"], 1, nw=nw["input_layernorm"])

@@ -90,3 +90,26 @@ def test_captured_drafted_steps_over_a_long_cache(tiny, bits, n):
     m.hidden(ids_of(args, n, 4), cache)
     ref = m(tokens[line], cache)
     assert rel(out[1][line], ref) < 3e-2, rel(out[1][line], ref)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_places_without_a_draft(tiny, graphs, temperature):
+    """Tokens outside the vocabulary are never taken and change nothing for the nodes beside them."""
+    Q, args, state, packed = tiny
+    from mxfp4_int8_m5_amd.sc_draft import DraftTree
+    from oracle import draft as O
+    m = Q.FusedQwen3(args, state, packed)
+    tree, V = DraftTree([-1, 0, 0, 0, 1, 2, 2]), args.vocab_size
+    dec, u = Q.DraftQwen3(m, graphs=graphs), torch.rand(7, generator=torch.Generator().manual_seed(1)).cuda()
+    out = []
+    for none in ((-1, V, 2 ** 40, -2 ** 40), (3, 4, 5, 6)):
+        cache = m.make_cache(100, bits=8)
+        m.hidden(ids_of(args, 12, 6), cache)
+        tokens = torch.tensor([7, none[0], 9, none[1], 11, none[2], none[3]], device="cuda")
+        path, count, token, logits = dec.step(tokens, tree, cache, temperature, u)
+        out.append(logits)
+        want = O.verify(logits.float().cpu().numpy(), tokens.tolist(), tree.parent_list, temperature, u.cpu().numpy())
+        assert (path[:int(count)].tolist(), int(token)) == want
+        assert none[0] >= 0 or not set(path.tolist()) & {1, 3, 5, 6}
+    assert torch.equal(out[0][[0, 2]], out[1][[0, 2]])
