@@ -47,8 +47,8 @@ int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d
  * Over an 8-bit cache a row weighs by the product of its probability and its V row's scale, a half-precision number of which the
  * largest is 2^8 .. 2^14: products below 2^-22 of the largest lose bits, below 2^-39 they may vanish from the sum.  The denominator
  * is summed from the same products, in float32, over the scales: a row whose product is below 2^-110 of another's may count as not
- * seen.  V scales are positive and normal, or 0 for a row of zeros, which takes part as one with the scale 2^-80 would.  Over a
- * bf16 cache the probabilities are rounded to bf16, in the sum and in the denominator alike (2^-8 of sum p |v| at most).
+ * seen.  V scales are 2^-110 .. 2^122, as the append's are, or 0 for a row of zeros, which takes part as one with the scale 2^-80 would
+ * (others are not looked for: a negative or subnormal one gives NaN).  scale is finite, times log2 e too.  Over a bf16 cache the probabilities are rounded to bf16, in the sum and in the denominator alike (2^-8 of sum p |v| at most).
  * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16 or 32 query rows; more than one needs
  * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches.
  * scmx_attn_tree_splits: how many to take for n rows in all (the cache's, where the position is on the device); 1 for arguments that

@@ -630,8 +630,8 @@ extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void*
         set_error("attn_tree: %d rows from %lld on do not fit a cache of %d rows", T, (long long)pos0, cache_rows);
         return SCMX_ERR_ARG;
     }
-    if (!(scale >= -3.0e38f && scale <= 3.0e38f)) {
-        set_error("attn_tree: scale must be finite");
+    if (!(fabsf(scale * 1.4426950408889634f) <= 3.4028234e38f)) {   // (the kernel works in powers of two)
+        set_error("attn_tree: scale must be finite, times log2 e too");
         return SCMX_ERR_ARG;
     }
     if ((uintptr_t(q) | uintptr_t(kcache) | uintptr_t(vcache) | uintptr_t(out)) % 16) {
