@@ -2,16 +2,17 @@
 //
 // The tokens' query heads that share a KV head are the rows of one matrix product, so that a cache row is read once for all of
 // them: row r is token r / group, head r % group of the group.  A wave owns 16 or 32 rows and walks tiles of 32 keys with a running
-// reference (the softmax's maximum), sums in float32.  Both products are transposed,
+// reference (the softmax's maximum), sums in float32 (8 bits: denominators in float64).  Both products are transposed,
 //     S^T = K Q^T  (16x16x32 MFMA: rows = keys, columns = queries),   O^T = V^T P^T  (rows = head dimension, columns = queries),
 // so that a query is a lane column (lane % 16) in both, its statistics sit in the lanes that need them, and the S^T
 // accumulators, converted, are the second product's operand where they are: register 4t + r of lane group g = lane / 16 holds key
 // 16t + 4g + r of the tile, and V is read with the same key order.  The contraction over the head dimension may take any order
 // too, and takes the one in which a lane's 16-byte load of a K row is its operand.  A lane reads DPL = d / 16 consecutive values of eight V
 // rows and turns them in registers (byte permutes); MFMA i then yields head-dimension indexes DPL * row + i.  So nothing
-// is staged: no LDS, no barrier in the loop, every wave streams its own keys with the next tile's loads in flight.  Bound by reading the cache from
-// some ten thousand rows on (one token, 40000 rows of 8 x 128 in 8 bits: 4.7 TB/s), by latency and two launches below, and with many
-// tokens by a step's chain of products, exponentials and conversions (64 tokens of 32 heads: a wave's tile takes 1 us).
+// is staged: no LDS, no barrier in the loop, every wave streams its own keys with the next tile's loads in flight.  Bound by reading
+// the cache from some ten thousand rows on (one token, 40000 rows of 8 x 128 in 8 bits: 15.5 us, 5.4 TB/s, and 3.9 the join), by
+// latency and two launches below, and with many tokens by a step's chain of products, exponentials and conversions (64 tokens of 32
+// heads: a wave's tile takes 1 us).
 //
 // 8 bits: K codes become bf16 (exact; q stays as it is), the row's scale multiplies the score.  V codes become half precision
 // (exact), and the row's scale goes into the weight, w = p * scale, through the exponent: w = exp2(score + log2(scale) - reference).
@@ -37,8 +38,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int TKEYS = 32, TXCDS = 8, JNT = 256;
-// Waves of a workgroup.  Four, two workgroups a CU, whose starts and ends overlap; eight of one: 16 tokens, 3000 rows of 16:8 x 128, bf16
-// 12.4 -> 10.9 us, one token, 1000 rows, 8 bits 8.8 -> 7.6, 40000 rows 21.2 -> 20.8.
+// Waves of a workgroup.  Four, two workgroups a CU, whose starts and ends overlap, against eight of one (both launches, in a graph): 16
+// tokens, 3000 rows of 16:8 x 128, bf16 12.4 -> 10.9 us, one token, 1000 rows, 8 bits 8.8 -> 7.6, 40000 rows 21.2 -> 20.7.
 constexpr int TWAVES = 4, TNT = 64 * TWAVES;
 constexpr int TONE = 16;   // tiles up to which one range takes all (four a wave): a second launch costs a microsecond more than the steps it saves
 
@@ -603,8 +604,10 @@ extern "C" int scmx_attn_tree_splits(int T, int n, int hq, int hk, int d) {
     if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
     const int qrows = T * (hq / hk), rt = tree_blocks(qrows, d), tiles = tiles_of(n);
     if (tiles <= TONE) return 1;
-    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, which the join likes better (94 tiles:
-    // 24 ranges 11.3 us, 16 10.9).
+    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, whose join reads half as much.  That pays
+    // for 32 query rows of 128 (16 tokens of 16:8 x 128, 16 ranges / a tile a wave: 94 tiles 10.9 / 11.2 us, 128 tiles bf16 12.4 / 13.0,
+    // 65 tiles 10.7 / 10.5), and costs fewer or narrower rows 0.1 to 0.4 us (94 tiles, one token of 16:8 x 128 8.5 / 8.4, of 14:2 x 64
+    // 7.1 / 6.8), one token over bf16 rows of 256 up to 1.6 (128 tiles 15.2 / 13.6).
     const int64_t most = 256 / (int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)));
     const int even = (tiles + TWAVES - 1) / TWAVES, ranges = even > 16 && even <= 32 ? 16 : even < 64 ? even : 64;
     return most < 1 ? 1 : ranges < most ? ranges : int(most);

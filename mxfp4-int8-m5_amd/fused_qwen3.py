@@ -438,7 +438,7 @@ class DraftQwen3(DecodeQwen3):
 
     def _linear(self, x, w, epi, res=None, nw=None):
         """A linear on a few rows x [T, K], RMSNorm with weight nw first.  One row takes the norm in the GEMV's prologue, several rows
-        apart (each workgroup would norm them all): 28 blocks of 2048 x 6144, a captured step of 4 nodes 1.66 ms against 1.44, of 8 2.18
+        apart (each workgroup would norm them all): 28 blocks of 2048 x 6144, a captured step of 4 nodes 1.66 ms against 1.45, of 8 2.18
         against 1.64 (quantized with the norm 1.63, through the few-row GEMM 1.72)."""
         f = self.f
         if nw is not None and x.shape[0] > 1:
