@@ -2,8 +2,8 @@
  * (device pointers, the caller's stream, no allocation, no synchronisation, no state, SCMX_ERR_* and scmx_last_error()).
  * The reference has none of these: its decode step takes one token, its cache holds the model's type.
  *
- * A cache is a K and a V tensor (two, not one twice) [hk, cache_rows, d], either bf16 (kscale = vscale = NULL) or INT8 with one float scale per row
- * (kscale, vscale [hk, cache_rows]): value = code * scale.  8-bit rows take d + 4 bytes where bf16 rows take 2 d.
+ * A cache is a K and a V tensor (two, not one twice) [hk, cache_rows, d], either bf16 (kscale = vscale = NULL) or INT8 with one
+ * float scale per row (kscale, vscale [hk, cache_rows]): value = code * scale.  8-bit rows take d + 4 bytes where bf16 rows take 2 d.
  * A tree of drafted tokens has its T (1..64) nodes in rows pos .. pos + T - 1 behind the pos rows of the sequence, every node
  * after its parent, node 0 the sequence's newest token.  pos is *pos_dev when pos_dev != NULL (a device-resident position, so that a
  * captured graph can be replayed for every step), else pos0.  d is 64, 128 or 256.  Tensors are 16-byte aligned (scales, masks and
@@ -40,15 +40,16 @@ int scmx_cache_read(const int8_t* kcache, const int8_t* vcache, const float* ksc
 int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d, int cache_rows, const int32_t* path,
                     const int32_t* count, int T, const int64_t* pos_dev, int64_t pos0, void* stream);
 
-/* Attention of the T nodes of a tree: out bf16 [T, hq * d] = softmax(q . K^T * scale) V, q bf16 [T, hq, d], hq / hk up to 4096.  Every node sees
- * the rows below pos; row pos + j is seen by node i if bit j of mask[i] is set (mask NULL: j <= i, a chain).  A node that sees
- * nothing gets zeros; what a node does not see does not reach its result, infinities and NaN among it.  T = 1 is the decode
+/* Attention of the T nodes of a tree: out bf16 [T, hq * d] = softmax(q . K^T * scale) V, q bf16 [T, hq, d], hq / hk up to 4096.
+ * Every node sees the rows below pos; row pos + j is seen by node i if bit j of mask[i] is set (mask NULL: j <= i, a chain).  A node
+ * that sees nothing gets zeros; what a node does not see does not reach its result, infinities and NaN among it.  T = 1 is the decode
  * step's attention over an 8-bit cache.  With pos_dev, a position whose rows do not fit the cache gives zeros.
  * Over an 8-bit cache a row weighs by the product of its probability and its V row's scale, a half-precision number of which the
  * largest is 2^8 .. 2^14: products below 2^-22 of the largest lose bits, below 2^-39 they may vanish from the sum.  The denominator
  * is summed from the same products, in float32, over the scales: a row whose product is below 2^-110 of another's may count as not
  * seen.  V scales are 2^-110 .. 2^122, as the append's are, or 0 for a row of zeros, which takes part as one with the scale 2^-80 would
- * (others are not looked for: a negative or subnormal one gives NaN).  scale is finite, times log2 e too.  Over a bf16 cache the probabilities are rounded to bf16, in the sum and in the denominator alike (2^-8 of sum p |v| at most).
+ * (others are not looked for: a negative or subnormal one gives NaN).  Over a bf16 cache the probabilities are rounded to bf16, in the
+ * sum and in the denominator alike (2^-8 of sum p |v| at most).  scale is finite, times log2 e too.
  * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16 or 32 query rows; more than one needs
  * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches.
  * scmx_attn_tree_splits: how many to take for n rows in all (the cache's, where the position is on the device); 1 for arguments that

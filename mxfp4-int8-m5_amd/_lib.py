@@ -1,5 +1,5 @@
-"""Access to libscmx.so (the C ABI declared in include/scmx.h and scmx_cache.h): `native()` is what the wrappers call, tensors in, one native
-call per launch (csrc/torch_binding.cpp); `load()` the whole ABI through ctypes, for the queries and for foreign callers,
+"""Access to libscmx.so (the C ABI declared in include/scmx.h and scmx_cache.h): `native()` is what the wrappers call, tensors in, one
+native call per launch (csrc/torch_binding.cpp); `load()` the whole ABI through ctypes, for the queries and for foreign callers,
 with `call`, `ptr` and `stream` to check a status and to make arguments of tensors.
 There is no fallback: a missing or incomplete library raises, and so does every call that returns a negative status."""
 import ctypes as C

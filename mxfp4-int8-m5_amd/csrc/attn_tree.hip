@@ -41,7 +41,8 @@ constexpr int TKEYS = 32, TXCDS = 8, JNT = 256;
 // Waves of a workgroup.  Four, two workgroups a CU, whose starts and ends overlap, against eight of one (both launches, in a graph): 16
 // tokens, 3000 rows of 16:8 x 128, bf16 12.4 -> 10.9 us, one token, 1000 rows, 8 bits 8.8 -> 7.6, 40000 rows 21.2 -> 20.7.
 constexpr int TWAVES = 4, TNT = 64 * TWAVES;
-constexpr int TONE = 16;   // tiles up to which one range takes all (four a wave): a second launch costs a microsecond more than the steps it saves
+// Tiles up to which one range takes all (four a wave): a second launch costs a microsecond more than the steps it saves.
+constexpr int TONE = 16;
 
 struct TreeArgs {
     const uint16_t* q;
@@ -89,8 +90,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
     // how far scores may pass the reference, and where it is put below the largest score (both in powers of two)
     constexpr float PASS = EIGHT ? 6.0f : 8.0f, BELOW = EIGHT ? 8.0f : 0.0f;
     __shared__ float s_o[WAVES][ROWS][D + 4];
-    // 8 bits: the denominators are sums of weights over scales, up to 2^14 / 2^-107 each, of any number of rows: tiles' sums in float32, the
-    // rest in float64 (30000 rows of 2^-98 overflow float32; the time is the same)
+    // 8 bits: the denominators are sums of weights over scales, up to 2^14 / 2^-107 each, of any number of rows: tiles' sums in float32,
+    // the rest in float64 (30000 rows of 2^-98 overflow float32; the time is the same)
     using Den = std::conditional_t<EIGHT, double, float>;
     __shared__ float s_m[WAVES][ROWS];     // references
     __shared__ Den s_l[WAVES][ROWS];       // denominators
@@ -169,7 +170,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
     constexpr int QPIECES = ROWS * D / 8, QROW = D + 8;   // 16-byte pieces; LDS row in values
     constexpr int QPER = (QPIECES + NT - 1) / NT;         // a thread (the ones left over bring some again)
     __shared__ __attribute__((aligned(16))) uint16_t s_q[QLDS ? ROWS * QROW : 1];
-    const auto q_at = [&](int s) { return EIGHT ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };   // slice s of a lane, in K's order
+    // slice s of a lane, in K's order
+    const auto q_at = [&](int s) { return EIGHT ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
     bf16x8 qf[RT][SLICES];
     u32x4 qraw[QPER];
     if constexpr (QLDS) {
@@ -235,8 +237,9 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
                 bf16x8 kf;
                 if constexpr (EIGHT) {
                     const uint32_t w0 = kr[h][sl / 2][2 * (sl & 1)], w1 = kr[h][sl / 2][2 * (sl & 1) + 1];
-                    const u32x4 p = {perm(byte_f32<1>(w0), byte_f32<0>(w0), 0x07060302u), perm(byte_f32<3>(w0), byte_f32<2>(w0), 0x07060302u),
-                                     perm(byte_f32<1>(w1), byte_f32<0>(w1), 0x07060302u), perm(byte_f32<3>(w1), byte_f32<2>(w1), 0x07060302u)};
+                    const u32x4 p = {
+                        perm(byte_f32<1>(w0), byte_f32<0>(w0), 0x07060302u), perm(byte_f32<3>(w0), byte_f32<2>(w0), 0x07060302u),
+                        perm(byte_f32<1>(w1), byte_f32<0>(w1), 0x07060302u), perm(byte_f32<3>(w1), byte_f32<2>(w1), 0x07060302u)};
                     kf = __builtin_bit_cast(bf16x8, p);
                 } else {
                     kf = __builtin_bit_cast(bf16x8, kr[h][sl]);
@@ -355,8 +358,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint64_t b = __builtin_amdgcn_ballot_w64(odd[e] != 0);
-                    const uint32_t of = uint32_t((b & 0xFFFFu) != 0) | uint32_t((b >> 16 & 0xFFFFu) != 0) << 1 | uint32_t((b >> 32 & 0xFFFFu) != 0) << 2 |
-                                        uint32_t((b >> 48) != 0) << 3;
+                    const uint32_t of = uint32_t((b & 0xFFFFu) != 0) | uint32_t((b >> 16 & 0xFFFFu) != 0) << 1 |
+                                        uint32_t((b >> 32 & 0xFFFFu) != 0) << 2 | uint32_t((b >> 48) != 0) << 3;
                     bad |= of << (4 * e);
 #pragma unroll
                     for (int w = 0; w < VW; ++w) vr[e][w] = of >> g & 1 ? 0 : vr[e][w];
@@ -391,7 +394,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
             const u32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-                ones[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, pf[rt]), ones[rt], 0, 0, 0);
+                ones[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, pf[rt]),
+                                                                   ones[rt], 0, 0, 0);
         }
         uint32_t pairs[2][4];   // 8 bits: bytes 0, 1 and 2, 3 of a word of two rows, side by side
 #pragma unroll
@@ -407,17 +411,20 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
                         pairs[1][e] = perm(hi, lo, 0x07030602u);
                     }
                     const uint32_t two = perm(0x64646464u, pairs[i % 4 / 2][e], i % 2 ? 0x04030402u : 0x04010400u);
-                    w[e] = __builtin_bit_cast(uint32_t, half2_t(__builtin_bit_cast(half2_t, two) - half2_t{_Float16(1152.0f), _Float16(1152.0f)}));
+                    const half2_t biased = __builtin_bit_cast(half2_t, two);
+                    w[e] = __builtin_bit_cast(uint32_t, half2_t(biased - half2_t{_Float16(1152.0f), _Float16(1152.0f)}));
                 }
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, pf[rt]), o[rt][i], 0, 0, 0);
+                    o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, pf[rt]),
+                                                                      o[rt][i], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = perm(vr[2 * e + 1][i / 2], vr[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, pf[rt]), o[rt][i], 0, 0, 0);
+                    o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, pf[rt]),
+                                                                       o[rt][i], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -469,7 +476,8 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
         const float den = float(sum);
         if (whole) f *= den == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(den);   // (0: nothing was seen)
         else if (wave == 0 && g == 0 && row0 + r < rows_all)
-            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, den};
+            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D +
+                                       2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, den};
         if (row0 + r < rows_all) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
@@ -499,13 +507,14 @@ __global__ __launch_bounds__(TNT, D == 256 && !EIGHT ? 1 : 2) void attn_tree_ker
 // Joins the ranges of one row of [T, hq], a workgroup: D / 4 lanes a range, the ranges dealt to the rest.  Bound by one trip to memory:
 // all that a thread reads is requested at once.  RANGES: at most.
 template <int D, int RANGES>
-__global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
-                                                             int splits, const int64_t* pos_dev, int64_t pos0) {
+__global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq,
+                                                             int rows, int splits, const int64_t* pos_dev, int64_t pos0) {
     constexpr int PARTS = JNT / (D / 4), PER = (RANGES + PARTS - 1) / PARTS;
     __shared__ float s_num[PARTS][D];
     const int lane = threadIdx.x & 63, p = threadIdx.x / (D / 4), e = threadIdx.x % (D / 4) * 4;
     const float* num0 = part + size_t(blockIdx.x) * splits * D + e;
-    const float2 ml = reinterpret_cast<const float2*>(part + size_t(T) * hq * splits * D)[size_t(blockIdx.x) * splits + min(lane, splits - 1)];
+    const float2 ml =
+        reinterpret_cast<const float2*>(part + size_t(T) * hq * splits * D)[size_t(blockIdx.x) * splits + min(lane, splits - 1)];
     f32x4 v[PER];
 #pragma unroll
     for (int u = 0; u < PER; ++u) v[u] = *reinterpret_cast<const f32x4*>(num0 + size_t(min(p + u * PARTS, splits - 1)) * D);
@@ -542,8 +551,8 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_kernel(const float* __rest
 // The same for up to 8 ranges and a wave a row, four rows a workgroup: the parts of a row meet across lanes.  64 tokens of 32 heads, four
 // ranges of 6000 rows 22.9 -> 21.0 us with the attention; with 16 ranges a wave has too much in a row (one token, 4000 rows 8.5 -> 9.0).
 template <int D>
-__global__ __launch_bounds__(JNT) void attn_tree_join_rows_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq, int rows,
-                                                                  int splits, const int64_t* pos_dev, int64_t pos0) {
+__global__ __launch_bounds__(JNT) void attn_tree_join_rows_kernel(const float* __restrict__ part, uint16_t* __restrict__ out, int T, int hq,
+                                                                  int rows, int splits, const int64_t* pos_dev, int64_t pos0) {
     constexpr int LANES = D / 4, PARTS = 64 / LANES, PER = 8 / PARTS;
     const int lane = threadIdx.x & 63, p = lane / LANES, e = lane % LANES * 4;
     const unsigned all = unsigned(T) * hq, row = min(blockIdx.x * (JNT / 64) + threadIdx.x / 64, all - 1);   // (the last one again)
@@ -575,7 +584,9 @@ __global__ __launch_bounds__(JNT) void attn_tree_join_rows_kernel(const float* _
     for (int off = LANES; off < 64; off <<= 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) num[i] += __shfl_xor(num[i], off, WAVE);
-    if (p == 0) *reinterpret_cast<u32x2*>(out + size_t(row) * D + e) = u32x2{f32_to_bf16x2(num[0] * inv, num[1] * inv), f32_to_bf16x2(num[2] * inv, num[3] * inv)};
+    if (p == 0)
+        *reinterpret_cast<u32x2*>(out + size_t(row) * D + e) =
+            u32x2{f32_to_bf16x2(num[0] * inv, num[1] * inv), f32_to_bf16x2(num[2] * inv, num[3] * inv)};
 }
 
 template <int D, int RT>
@@ -584,9 +595,9 @@ static void launch_tree(const TreeArgs& a, hipStream_t st) {
     if (a.ks) attn_tree_kernel<D, RT, true><<<dim3(grid), dim3(TNT), 0, st>>>(a);
     else attn_tree_kernel<D, RT, false><<<dim3(grid), dim3(TNT), 0, st>>>(a);
     if (a.splits == 1) return;
-    const unsigned rows = unsigned(a.T) * a.hq;
+    const unsigned rows = unsigned(a.T) * a.hq, fours = (rows + JNT / 64 - 1) / (JNT / 64);
     if (a.splits <= 8)
-        attn_tree_join_rows_kernel<D><<<dim3((rows + JNT / 64 - 1) / (JNT / 64)), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
+        attn_tree_join_rows_kernel<D><<<dim3(fours), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
     else if (a.splits <= 16)
         attn_tree_join_kernel<D, 16><<<dim3(rows), dim3(JNT), 0, st>>>(a.part, a.out, a.T, a.hq, a.rows, a.splits, a.pos_dev, a.pos0);
     else
@@ -621,8 +632,8 @@ extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void*
         return SCMX_ERR_ARG;
     }
     if (T < 1 || T > 64 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || hq / hk > 4096 || cache_rows < T) {
-        set_error("attn_tree: need 1..64 nodes, hq %% hk == 0, up to 4096 query heads a KV head and a cache that holds the tree (T=%d hq=%d hk=%d rows=%d)", T, hq,
-                  hk, cache_rows);
+        set_error("attn_tree: need 1..64 nodes, hq %% hk == 0, up to 4096 query heads a KV head and a cache that holds the tree "
+                  "(T=%d hq=%d hk=%d rows=%d)", T, hq, hk, cache_rows);
         return SCMX_ERR_ARG;
     }
     if (d != 64 && d != 128 && d != 256) {
@@ -646,8 +657,9 @@ extern "C" int scmx_attn_tree(const uint16_t* q, const void* kcache, const void*
         return SCMX_ERR_ARG;
     }
     const int qrows = T * (hq / hk);
-    TreeArgs a{q, static_cast<const uint8_t*>(kcache), static_cast<const uint8_t*>(vcache), kscale, vscale, mask, pos_dev, pos0, out, workspace,
-               T, hq, hk, cache_rows, splits, 0, uint32_t(((uint64_t(1) << 32) + hq / hk - 1) / uint64_t(hq / hk)), scale * 1.4426950408889634f};
+    const uint32_t by_group = uint32_t(((uint64_t(1) << 32) + hq / hk - 1) / uint64_t(hq / hk));
+    TreeArgs a{q, static_cast<const uint8_t*>(kcache), static_cast<const uint8_t*>(vcache), kscale, vscale, mask, pos_dev, pos0, out,
+               workspace, T, hq, hk, cache_rows, splits, 0, by_group, scale * 1.4426950408889634f};
     const int rt = tree_blocks(qrows, d);
     a.blocks = (qrows + 16 * rt - 1) / (16 * rt);
     const hipStream_t st = (hipStream_t)stream;

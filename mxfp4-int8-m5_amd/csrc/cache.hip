@@ -98,7 +98,8 @@ __global__ __launch_bounds__(CNT) void cache_write_kernel(const WriteArgs a) {
         if constexpr (ACC) {
             const float xs = a.xscale[row];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = round_bf16(__fmul_rn(__fmul_rn(float(int32_t(raw.w[i / 4][i % 4])), xs), a.wscale[g * D + 8 * j + i]));
+            for (int i = 0; i < 8; ++i)
+                x[i] = round_bf16(__fmul_rn(__fmul_rn(float(int32_t(raw.w[i / 4][i % 4])), xs), a.wscale[g * D + 8 * j + i]));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -186,8 +187,8 @@ struct KeepArgs {
 // blockIdx.x: KV head, y: K or V, z: layer.  The rows are read whole before any is written (a row may be both); up to 64 rows of up
 // to 512 bytes.  Bound by latency: count, path, rows, stores.
 template <int ROWB>
-__global__ __launch_bounds__(CNT) void cache_keep_kernel(const KeepArgs a, bool eight, int rows, const int32_t* path, const int32_t* count, int T,
-                                                         const int64_t* pos_dev, int64_t pos0) {
+__global__ __launch_bounds__(CNT) void cache_keep_kernel(const KeepArgs a, bool eight, int rows, const int32_t* path, const int32_t* count,
+                                                         int T, const int64_t* pos_dev, int64_t pos0) {
     const int64_t pos = pos_dev ? pos_dev[0] : pos0;
     if (pos < 0 || pos > int64_t(rows) - T) return;
     const int kept = min(max(count[0], 0), T);
@@ -242,7 +243,8 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
                                 const uint16_t* kn, float eps, uint16_t* q, void* kcache, void* vcache, float* kscale, float* vscale, int L,
                                 int hq, int hk, int d, const float* inv_freq, const int32_t* depth, const int64_t* pos_dev, int64_t pos0,
                                 int cache_rows, void* stream) {
-    if ((L && ((!acc && !y) || !q)) || (acc && (!xscale || !wscale)) || !qn || !kn || !kcache || !vcache || !inv_freq || !kscale != !vscale) {
+    if ((L && ((!acc && !y) || !q)) || (acc && (!xscale || !wscale)) || !qn || !kn || !kcache || !vcache || !inv_freq ||
+        !kscale != !vscale) {
         set_error("cache_write: null pointer argument (an 8-bit cache has both scales, a bf16 one none)");
         return SCMX_ERR_ARG;
     }
@@ -256,7 +258,8 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
         return SCMX_ERR_ARG;
     }
     if (L == 0) return SCMX_OK;
-    const WriteArgs a{acc, xscale, wscale, y, qn, kn, eps, q, {kcache, vcache}, {kscale, vscale}, L, hq, hk, inv_freq, depth, pos_dev, pos0, cache_rows};
+    const WriteArgs a{acc, xscale, wscale, y, qn, kn, eps, q, {kcache, vcache}, {kscale, vscale}, L, hq, hk, inv_freq, depth, pos_dev, pos0,
+                      cache_rows};
     const int groups = CNT / (d / 8), turns = (hq + 2 * hk + groups - 1) / groups;
     // a few tokens are spread over the CUs; a prompt fills them with a workgroup a token, which then takes the angles once
     const dim3 grid(L, L >= 256 ? 1 : turns);
@@ -274,8 +277,8 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
     return check_launch("cache_write");
 }
 
-extern "C" int scmx_cache_read(const int8_t* kcache, const int8_t* vcache, const float* kscale, const float* vscale, uint16_t* k, uint16_t* v,
-                               int hk, int d, int cache_rows, int row0, int n, void* stream) {
+extern "C" int scmx_cache_read(const int8_t* kcache, const int8_t* vcache, const float* kscale, const float* vscale, uint16_t* k,
+                               uint16_t* v, int hk, int d, int cache_rows, int row0, int n, void* stream) {
     if (!kcache || !vcache || !kscale || !vscale || (n && (!k || !v))) {
         set_error("cache_read: null pointer argument");
         return SCMX_ERR_ARG;
@@ -325,8 +328,8 @@ extern "C" int scmx_cache_keep(const uint64_t* caches, int layers, int eight, in
         for (int l = 0; l < n; ++l)
             for (int i = 0; i < each; ++i) a.t[l][i] = reinterpret_cast<void*>(uintptr_t(caches[size_t(l0 + l) * each + i]));
         const auto go = [&](auto rowb) {
-            cache_keep_kernel<decltype(rowb)::value><<<dim3(hk, 2, n), dim3(CNT), 0, (hipStream_t)stream>>>(a, eight != 0, cache_rows, path, count,
-                                                                                                            T, pos_dev, pos0);
+            cache_keep_kernel<decltype(rowb)::value>
+                <<<dim3(hk, 2, n), dim3(CNT), 0, (hipStream_t)stream>>>(a, eight != 0, cache_rows, path, count, T, pos_dev, pos0);
         };
         switch (eight ? d : 2 * d) {
             case 64: go(std::integral_constant<int, 64>{}); break;

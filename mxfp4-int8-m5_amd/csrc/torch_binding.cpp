@@ -319,13 +319,15 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t* dev;
         int64_t pos;
         const int32_t* depth;
-        if (!ints_of(args, {4, 5, 6, 7}) || !PyFloat_Check(args[3]) || !cache_of(args[8], args[9], args[12], args[13], c) || !position_of(args[10], dev, pos))
+        if (!ints_of(args, {4, 5, 6, 7}) || !PyFloat_Check(args[3]) || !cache_of(args[8], args[9], args[12], args[13], c) ||
+            !position_of(args[10], dev, pos))
             Py_RETURN_NONE;
         const int64_t L = as_int(args[4]), hq = as_int(args[5]), hk = as_int(args[6]), d = as_int(args[7]);
-        const at::Tensor *y = local(args[0], at::ScalarType::BFloat16), *qn = local(args[1], at::ScalarType::BFloat16), *kn = local(args[2], at::ScalarType::BFloat16),
-                         *freq = local(args[11], at::ScalarType::Float);
-        if (!y || !qn || !kn || !freq || L < 0 || L > INT32_MAX || hq < 1 || hq > 65535 || hk != c.hk || d != c.d || y->dim() != 2 || y->size(0) < L ||
-            y->size(1) != (hq + 2 * hk) * d || qn->numel() != d || kn->numel() != d || freq->numel() != d / 2 || !optional_of(args[14], at::ScalarType::Int, L, depth))
+        const at::Tensor *y = local(args[0], at::ScalarType::BFloat16), *qn = local(args[1], at::ScalarType::BFloat16),
+                         *kn = local(args[2], at::ScalarType::BFloat16), *freq = local(args[11], at::ScalarType::Float);
+        if (!y || !qn || !kn || !freq || L < 0 || L > INT32_MAX || hq < 1 || hq > 65535 || hk != c.hk || d != c.d || y->dim() != 2 ||
+            y->size(0) < L || y->size(1) != (hq + 2 * hk) * d || qn->numel() != d || kn->numel() != d || freq->numel() != d / 2 ||
+            !optional_of(args[14], at::ScalarType::Int, L, depth))
             Py_RETURN_NONE;
         at::Tensor q;
         int rc;
@@ -333,8 +335,9 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const NoGil released;
             q = at::Tensor(at::detail::empty_strided_cuda({hq, L, d}, {d, hq * d, 1}, at::ScalarType::BFloat16, y->device()));
             const auto bf = [](const at::Tensor* t) { return static_cast<const uint16_t*>(t->data_ptr()); };
-            rc = scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), float(PyFloat_AS_DOUBLE(args[3])), static_cast<uint16_t*>(q.data_ptr()), c.k->data_ptr(),
-                                  c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), int(L), int(hq), int(hk), int(d), static_cast<const float*>(freq->data_ptr()), depth, dev, pos,
+            rc = scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), float(PyFloat_AS_DOUBLE(args[3])),
+                                  static_cast<uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs),
+                                  int(L), int(hq), int(hk), int(d), static_cast<const float*>(freq->data_ptr()), depth, dev, pos,
                                   int(c.rows), stream());
         }
         if (rc != SCMX_OK) return status("scmx_cache_write", rc);
@@ -355,12 +358,15 @@ PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
             (args[7] != Py_None && !PyFloat_Check(args[7])) || (args[8] != Py_None && !PyLong_CheckExact(args[8])))
             Py_RETURN_NONE;
         const at::Tensor& q = THPVariable_Unpack(args[0]);
-        if (!q.is_cuda() || q.get_device() != c10::hip::current_device() || q.scalar_type() != at::ScalarType::BFloat16 || q.dim() != 3) Py_RETURN_NONE;
-        const int64_t hq = q.size(0), T = q.size(1), d = q.size(2);   // the view of [T, hq, d] storage
-        if (T < 1 || T > 64 || hq < 1 || hq > 65535 || d != c.d || c.hk < 1 || hq % c.hk || c.rows < T || q.stride(2) != 1 || (hq > 1 && q.stride(0) != d) ||
-            (T > 1 && q.stride(1) != hq * d) || !optional_of(args[4], at::ScalarType::Long, T, mask) || pos < 0 || pos > INT32_MAX - 64)
+        if (!q.is_cuda() || q.get_device() != c10::hip::current_device() || q.scalar_type() != at::ScalarType::BFloat16 || q.dim() != 3)
             Py_RETURN_NONE;
-        const int splits = args[8] != Py_None ? convert<int>(args[8]) : scmx_attn_tree_splits(int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
+        const int64_t hq = q.size(0), T = q.size(1), d = q.size(2);   // the view of [T, hq, d] storage
+        if (T < 1 || T > 64 || hq < 1 || hq > 65535 || d != c.d || c.hk < 1 || hq % c.hk || c.rows < T || q.stride(2) != 1 ||
+            (hq > 1 && q.stride(0) != d) || (T > 1 && q.stride(1) != hq * d) ||
+            !optional_of(args[4], at::ScalarType::Long, T, mask) || pos < 0 || pos > INT32_MAX - 64)
+            Py_RETURN_NONE;
+        const int splits = args[8] != Py_None ? convert<int>(args[8])
+                                              : scmx_attn_tree_splits(int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
         if (splits < 1 || splits > 64) Py_RETURN_NONE;
         const float scale = args[7] == Py_None ? float(1.0 / std::sqrt(double(d))) : float(PyFloat_AS_DOUBLE(args[7]));
         at::Tensor out;
@@ -369,9 +375,9 @@ PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const NoGil released;
             out = fresh(q, at::ScalarType::BFloat16, {T, hq * d});
             const c10::DataPtr work = scratch(splits > 1 ? size_t(splits * T * hq * (d + 2)) * sizeof(float) : 0);
-            rc = scmx_attn_tree(static_cast<const uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), mask, dev, pos,
-                                static_cast<uint16_t*>(out.data_ptr()), int(T), int(hq), int(c.hk), int(d), int(c.rows), scale,
-                                splits > 1 ? static_cast<float*>(work.get()) : nullptr, splits, stream());
+            rc = scmx_attn_tree(static_cast<const uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs),
+                                mask, dev, pos, static_cast<uint16_t*>(out.data_ptr()), int(T), int(hq), int(c.hk), int(d),
+                                int(c.rows), scale, splits > 1 ? static_cast<float*>(work.get()) : nullptr, splits, stream());
         }
         if (rc != SCMX_OK) return status("scmx_attn_tree", rc);
         return THPVariable_Wrap(std::move(out));
@@ -394,8 +400,9 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const NoGil released;
             k = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
             v = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
-            rc = scmx_cache_read(static_cast<const int8_t*>(c.k->data_ptr()), static_cast<const int8_t*>(c.v->data_ptr()), c.scale(c.ks), c.scale(c.vs),
-                                 static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()), int(c.hk), int(c.d), int(c.rows), int(row0), int(rows), stream());
+            const auto codes = [](const at::Tensor* t) { return static_cast<const int8_t*>(t->data_ptr()); };
+            rc = scmx_cache_read(codes(c.k), codes(c.v), c.scale(c.ks), c.scale(c.vs), static_cast<uint16_t*>(k.data_ptr()),
+                                 static_cast<uint16_t*>(v.data_ptr()), int(c.hk), int(c.d), int(c.rows), int(row0), int(rows), stream());
         }
         if (rc != SCMX_OK) return status("scmx_cache_read", rc);
         PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
@@ -412,7 +419,8 @@ PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor *path = local(args[1], at::ScalarType::Int), *count = local(args[2], at::ScalarType::Int);
         const int64_t* dev;
         int64_t pos;
-        if (!PyList_CheckExact(args[0]) || !path || !count || count->numel() != 1 || path->numel() > 64 || !position_of(args[3], dev, pos)) Py_RETURN_NONE;
+        if (!PyList_CheckExact(args[0]) || !path || !count || count->numel() != 1 || path->numel() > 64 || !position_of(args[3], dev, pos))
+            Py_RETURN_NONE;
         const Py_ssize_t layers = PyList_GET_SIZE(args[0]);
         std::vector<uint64_t> pointers;
         pointers.reserve(size_t(layers) * 4);
@@ -421,7 +429,8 @@ PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
             PyObject* t = PyList_GET_ITEM(args[0], i);
             if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 4) Py_RETURN_NONE;
             c = CacheTensors();
-            if (!cache_of(PyTuple_GET_ITEM(t, 0), PyTuple_GET_ITEM(t, 1), PyTuple_GET_ITEM(t, 2), PyTuple_GET_ITEM(t, 3), c)) Py_RETURN_NONE;
+            if (!cache_of(PyTuple_GET_ITEM(t, 0), PyTuple_GET_ITEM(t, 1), PyTuple_GET_ITEM(t, 2), PyTuple_GET_ITEM(t, 3), c))
+                Py_RETURN_NONE;
             if (i == 0) first = c;
             else if (c.hk != first.hk || c.rows != first.rows || c.d != first.d || !c.ks != !first.ks) Py_RETURN_NONE;
             for (const at::Tensor* x : {c.k, c.v, c.ks, c.vs})
@@ -429,7 +438,8 @@ PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         if (layers < 1 || layers > 1024) Py_RETURN_NONE;
         const int rc = scmx_cache_keep(pointers.data(), int(layers), first.ks != nullptr, int(first.hk), int(first.d), int(first.rows),
-                                       static_cast<const int32_t*>(path->data_ptr()), static_cast<const int32_t*>(count->data_ptr()), int(path->numel()), dev, pos, stream());
+                                       static_cast<const int32_t*>(path->data_ptr()), static_cast<const int32_t*>(count->data_ptr()),
+                                       int(path->numel()), dev, pos, stream());
         if (rc != SCMX_OK) return status("scmx_cache_keep", rc);
         Py_RETURN_TRUE;
     } catch (...) {
@@ -443,8 +453,8 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != 7) fail(PyExc_TypeError, "verify_drafts takes 7 arguments");
         if (!THPVariable_Check(args[0]) || !PyFloat_Check(args[3]) || !PyLong_CheckExact(args[6])) Py_RETURN_NONE;
         const bool f32 = THPVariable_Unpack(args[0]).scalar_type() == at::ScalarType::Float;
-        const at::Tensor *logits = local(args[0], f32 ? at::ScalarType::Float : at::ScalarType::BFloat16), *tokens = local(args[1], at::ScalarType::Long),
-                         *parents = local(args[2], at::ScalarType::Int);
+        const at::Tensor *logits = local(args[0], f32 ? at::ScalarType::Float : at::ScalarType::BFloat16),
+                         *tokens = local(args[1], at::ScalarType::Long), *parents = local(args[2], at::ScalarType::Int);
         if (!logits || !tokens || !parents || logits->dim() != 2) Py_RETURN_NONE;
         const int64_t T = logits->size(0), V = logits->size(1), levels = as_int(args[6]);
         const float *u, *draft;
@@ -460,9 +470,10 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
             count = fresh(*logits, at::ScalarType::Int, {1});
             next = fresh(*logits, at::ScalarType::Long, {1});
             const c10::DataPtr work = scratch(need);
-            rc = scmx_verify_drafts(static_cast<const int64_t*>(tokens->data_ptr()), static_cast<const int32_t*>(parents->data_ptr()), logits->data_ptr(), f32, draft,
-                                    PyFloat_AS_DOUBLE(args[3]), u, static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()),
-                                    static_cast<int64_t*>(next.data_ptr()), int(T), int(V), int(levels), work.get(), need, stream());
+            rc = scmx_verify_drafts(static_cast<const int64_t*>(tokens->data_ptr()), static_cast<const int32_t*>(parents->data_ptr()),
+                                    logits->data_ptr(), f32, draft, PyFloat_AS_DOUBLE(args[3]), u, static_cast<int32_t*>(path.data_ptr()),
+                                    static_cast<int32_t*>(count.data_ptr()), static_cast<int64_t*>(next.data_ptr()), int(T),
+                                    int(V), int(levels), work.get(), need, stream());
         }
         if (rc != SCMX_OK) return status("scmx_verify_drafts", rc);
         PyObject *a = THPVariable_Wrap(std::move(path)), *b = THPVariable_Wrap(std::move(count)), *c = THPVariable_Wrap(std::move(next));

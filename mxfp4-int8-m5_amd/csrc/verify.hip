@@ -133,7 +133,8 @@ __device__ __forceinline__ double lane_of(double v, int lane) {
 template <int CTRL>
 __device__ __forceinline__ double row_op(double v) {   // v of the lane that CTRL names; 0 where it names none
     const long long b = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_update_dpp(0, int(b), CTRL, 0xF, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), CTRL, 0xF, 0xF, true);
+    const int lo = __builtin_amdgcn_update_dpp(0, int(b), CTRL, 0xF, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), CTRL, 0xF, 0xF, true);
     return __longlong_as_double((long long)(uint64_t(uint32_t(hi)) << 32 | uint32_t(lo)));
 }
 // Over the wave, in every lane: within rows of 16 lanes by row operations, the four rows as scalars (a butterfly through LDS has six
@@ -384,8 +385,10 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
                 const int row = wave + WAVES * r;
                 if (row >= a.T) break;
                 int best = lane < a.chunks && pm[r] == m[r] ? at[r] : a.V - 1;
-                for (int c = 64 + lane; c < a.chunks; c += 64)
-                    if (a.m[size_t(row) * a.chunks + c] == m[r]) best = min(best, reinterpret_cast<const int32_t*>(a.z)[size_t(row) * a.chunks + c]);
+                for (int c = 64 + lane; c < a.chunks; c += 64) {
+                    const size_t i = size_t(row) * a.chunks + c;
+                    if (a.m[i] == m[r]) best = min(best, reinterpret_cast<const int32_t*>(a.z)[i]);
+                }
 #pragma unroll
                 for (int off = 32; off >= 1; off >>= 1) best = min(best, __shfl_xor(best, off, WAVE));
                 if (lane == 0) s_best[row] = best;
@@ -420,7 +423,8 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         for (int row = wave; row < a.T; row += WAVES) {
             double more = 0.0;
 #pragma unroll 1
-            for (size_t i = size_t(row) * a.chunks + 64 + lane; i < size_t(row + 1) * a.chunks; i += 64) more += a.z[i] * weight(a.m[i], s_m[row], a.rate, s_table);
+            for (size_t i = size_t(row) * a.chunks + 64 + lane; i < size_t(row + 1) * a.chunks; i += 64)
+                more += a.z[i] * weight(a.m[i], s_m[row], a.rate, s_table);
             more = wave_sum64(more);
             if (lane == 0) s_z[row] += more;
         }
@@ -517,7 +521,8 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
             const auto part = [&](int c) {   // of the residual, in the units of the sums that it was taken from
                 if (c >= a.chunks) return 0.0;
                 if (lvl > 0) return a.s[(size_t(lvl - 1) * a.T + cur) * a.chunks + c];
-                double w = c < 64 ? s_w[cur][c] : a.z[size_t(cur) * a.chunks + c] * weight(a.m[size_t(cur) * a.chunks + c], s_m[cur], a.rate, s_table);
+                const size_t at = size_t(cur) * a.chunks + c;
+                double w = c < 64 ? s_w[cur][c] : a.z[at] * weight(a.m[at], s_m[cur], a.rate, s_table);
                 for (int i = 0; i < opens; ++i)
                     if (s_open[i] / VCHUNK == c) w += s_open_e[i];
                 return w;
@@ -526,9 +531,11 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
 #pragma unroll 1
             for (int k = 0; k < K; ++k) own += part(lane * K + k);
             const double upto = wave_scan64(own);
-            const double total = lane_of(upto, 63), target = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), 0))) * total;
+            const double total = lane_of(upto, 63);
+            const double target = double(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), 0))) * total;
             const uint64_t over = __ballot(own > 0.0 && upto > target), some = __ballot(own > 0.0);
-            const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;   // (no sum above it: the last that has any)
+            // (no sum above it: the last that has any)
+            const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
             if (lane == who) {
                 double run = upto - own, base = run;
                 int chunk = lane * K;
@@ -595,7 +602,9 @@ __global__ __launch_bounds__(VWALK) void verify_walk_kernel(const VerifyArgs a) 
         __syncthreads();
         const int o = lane < WAVES ? s_over[lane] : -1, h = lane < WAVES ? s_some[lane] : -1;
         const uint64_t any = __ballot(o >= 0), rest = __ballot(h >= 0);
-        token_at = any ? __builtin_amdgcn_readlane(o, __builtin_ctzll(any)) : rest ? __builtin_amdgcn_readlane(h, 63 - __builtin_clzll(rest)) : -1;
+        token_at = any    ? __builtin_amdgcn_readlane(o, __builtin_ctzll(any))
+                   : rest ? __builtin_amdgcn_readlane(h, 63 - __builtin_clzll(rest))
+                          : -1;
         chunk += step;
         if (chunk == a.chunks) {
             step = -1;
@@ -643,7 +652,8 @@ extern "C" int scmx_verify_drafts(const int64_t* tokens, const int32_t* parents,
         return SCMX_ERR_WORKSPACE;
     }
     const size_t cells = size_t(T) * chunks;
-    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels, greedy ? 1.0 : 64.0 / M_LN2 / temperature,
+    VerifyArgs a{tokens, parents, logits, greedy ? nullptr : draft, uniforms, path, count, next, T, V, chunks, levels,
+                 greedy ? 1.0 : 64.0 / M_LN2 / temperature,
                  uintptr_t(logits) % 16 == 0 && V % (logits_f32 ? 4 : 8) == 0, uintptr_t(draft) % 16 == 0 && V % 4 == 0,
                  static_cast<double*>(workspace), static_cast<double*>(workspace) + cells, nullptr};
     a.m = reinterpret_cast<float*>(a.s + cells * levels);

@@ -133,9 +133,9 @@ class FusedQwen3:
         an int64 device tensor for graph replay) and the KV-cache append, in one kernel: returns q [hq, L, d]."""
         a = self.args
         if isinstance(c, C.Q8Cache):
-            return C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads, a.num_key_value_heads,
-                                 a.head_dim, c.k, c.v, c.offset if pos is None else pos, self.inv_freq, c.kscale, c.vscale, acc=acc,
-                                 xscale=xs, wscale=ws)
+            return C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads,
+                                 a.num_key_value_heads, a.head_dim, c.k, c.v, c.offset if pos is None else pos, self.inv_freq, c.kscale,
+                                 c.vscale, acc=acc, xscale=xs, wscale=ws)
         return S.qkv_headnorm_rope(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads,
                                    a.num_key_value_heads, a.head_dim, c.k, c.v, c.offset if pos is None else pos,
                                    self.inv_freq, acc=acc, xscale=xs, wscale=ws, token_major=L > 1)
@@ -374,7 +374,8 @@ class DecodeQwen3:
             c = cache[i]
             q = self._pre(h, nw, ws["qkv"], c, self.pos)
             if not self.fuse_attn:
-                q = C.attn_tree(q, c.k, c.v, self.pos, None, c.kscale, c.vscale) if isinstance(c, C.Q8Cache) else S.attn_decode(q, c.k, c.v, self.pos)
+                eight = isinstance(c, C.Q8Cache)
+                q = C.attn_tree(q, c.k, c.v, self.pos, None, c.kscale, c.vscale) if eight else S.attn_decode(q, c.k, c.v, self.pos)
             h = self._post(q, h, nw, ws)
         return self._logits(h)
 
@@ -445,7 +446,8 @@ class DraftQwen3(DecodeQwen3):
             x, nw = S.rmsnorm(x, nw, f.eps), None
         if x.shape[0] > 8:
             return S.linear_w4a8(x, w.codes, w.bcodes, w.wscale, w.N, epi, res, f.fmt)
-        return G.gemv(x, w.codes, w.bcodes, None, w.wscale, w.N, epi, res=res, pro=1 if nw is None else 2, nw=nw, eps=f.eps, fmt=f.fmt).view(x.shape[0], -1)
+        out = G.gemv(x, w.codes, w.bcodes, None, w.wscale, w.N, epi, res=res, pro=1 if nw is None else 2, nw=nw, eps=f.eps, fmt=f.fmt)
+        return out.view(x.shape[0], -1)
 
     def hidden(self, tokens, tree, cache, pos):
         """Final normed hidden states [T, D] of the tree's nodes, whose keys and values go to the caches' rows pos .. pos + T - 1 (pos: int,
@@ -463,8 +465,8 @@ class DraftQwen3(DecodeQwen3):
         for c, (nw, ws) in zip(cache, f.layers):
             k, v, ks, vs = C.tensors(c)
             y = self._linear(h, ws["qkv"], 1, nw=nw["input_layernorm"])
-            q = C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, T, a.num_attention_heads, a.num_key_value_heads, a.head_dim,
-                              k, v, pos, f.inv_freq, ks, vs, depth)
+            q = C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, T, a.num_attention_heads,
+                              a.num_key_value_heads, a.head_dim, k, v, pos, f.inv_freq, ks, vs, depth)
             h = self._linear(C.attn_tree(q, k, v, pos, mask, ks, vs), ws["o"], 2, h)
             h = self._linear(self._linear(h, ws["gu"], 3, nw=nw["post_attention_layernorm"]), ws["down"], 2, h)
         return S.rmsnorm(h, f.norm, f.eps)

@@ -46,7 +46,8 @@ def _check(cond, what):
 
 def _check_cache(kcache, vcache, kscale, vscale):
     """(hk, rows, d) of a cache whose tensors belong together."""
-    _check(kcache.dim() == 3 and kcache.shape == vcache.shape and kcache.dtype == vcache.dtype, "kcache and vcache are [hk, rows, d] of one type")
+    _check(kcache.dim() == 3 and kcache.shape == vcache.shape and kcache.dtype == vcache.dtype,
+           "kcache and vcache are [hk, rows, d] of one type")
     _check((kscale is None) == (vscale is None), "an 8-bit cache has both scales, a bf16 one none")
     if kscale is None:
         _check(kcache.dtype == BF, "a cache without scales is bfloat16")
@@ -74,7 +75,8 @@ def cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, ksc
     if q is not None:   # the operands of every step; anything else is converted or refused below
         return q
     src = y if y is not None else acc
-    _check(src is not None and src.dim() == 2 and src.shape[0] >= L >= 0 and src.shape[1] == (hq + 2 * hk) * d, "y or acc is [>= L, (hq + 2 hk) d]")
+    _check(src is not None and src.dim() == 2 and src.shape[0] >= L >= 0 and src.shape[1] == (hq + 2 * hk) * d,
+           "y or acc is [>= L, (hq + 2 hk) d]")
     _check(src.dtype == (BF if y is not None else torch.int32), "y is bfloat16, acc int32")
     if y is None:
         _check(xscale is not None and wscale is not None and xscale.dtype == wscale.dtype == torch.float32 and xscale.numel() >= L
@@ -86,8 +88,8 @@ def cache_write(y, qn, kn, eps, L, hq, hk, d, kcache, vcache, pos, inv_freq, ksc
     dev_pos, at = _position(pos)
     _on_device(src, qn, kn, kcache, vcache, kscale, vscale, inv_freq, depth, dev_pos, *((xscale, wscale) if y is None else ()))
     q = _lib.native().empty_bf16(src, L, hq, d)
-    _lib.native().scmx_cache_write(None if y is not None else acc, xscale, wscale, y, qn, kn, float(eps), q, kcache, vcache, kscale, vscale, L, hq,
-                                   hk, d, inv_freq, depth, dev_pos, at, kcache.shape[1])
+    _lib.native().scmx_cache_write(None if y is not None else acc, xscale, wscale, y, qn, kn, float(eps), q, kcache, vcache, kscale,
+                                   vscale, L, hq, hk, d, inv_freq, depth, dev_pos, at, kcache.shape[1])
     return q.transpose(0, 1)
 
 
@@ -107,8 +109,8 @@ def cache_read(kcache, vcache, kscale, vscale, n, row0=0):
 
 def cache_keep(caches, path, count, pos):
     """Row pos + j of every cache takes what row pos + path[j] held, for j < count: the accepted line of a tree moved together, all
-    blocks in one launch (up to 32 of them).  caches: (kcache, vcache, kscale, vscale) a block, all of one shape and type; path int32 [T], count int32
-    [1] as verify_drafts returns them.  Rows from pos + count on keep what they hold."""
+    blocks in one launch (up to 32 of them).  caches: (kcache, vcache, kscale, vscale) a block, all of one shape and type; path int32 [T],
+    count int32 [1] as verify_drafts returns them.  Rows from pos + count on keep what they hold."""
     if _lib.native().cache_keep(caches, path, count, pos):
         return
     caches = [tuple(c) for c in caches]
@@ -124,8 +126,8 @@ def cache_keep(caches, path, count, pos):
     _check(all(t.is_contiguous() for t in flat), "scmx kernels take contiguous tensors")
     _on_device(path, count, dev_pos, *flat)
     pointers = array("Q", [t.data_ptr() for t in flat])
-    _lib.native().scmx_cache_keep(pointers.buffer_info()[0], len(caches), int(eight), shape[0], shape[2], shape[1], path, count, path.numel(), dev_pos,
-                                  at)
+    _lib.native().scmx_cache_keep(pointers.buffer_info()[0], len(caches), int(eight), shape[0], shape[2], shape[1], path, count,
+                                  path.numel(), dev_pos, at)
 
 
 def attn_tree_splits(T, n, hq, hk, d):

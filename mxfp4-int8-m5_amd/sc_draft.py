@@ -10,8 +10,8 @@ MAX_SIBLINGS = 16   # children of a node that are tried against a draft's probab
 
 class DraftTree:
     """The shape of a tree of drafted tokens: parents[i] < i, -1 for node 0, the sequence's newest token.  On the device: `parents` and
-    `depth` int32 [T], `mask` int64 [T] (a node sees itself and its line back to the root), views of `packed`.  `siblings`: the most children
-    of a node."""
+    `depth` int32 [T], `mask` int64 [T] (a node sees itself and its line back to the root), views of `packed`.  `siblings`: the most
+    children of a node."""
 
     def __init__(self, parents, device="cuda"):
         parents = [int(p) for p in parents]
@@ -42,13 +42,14 @@ def verify_drafts(logits, tokens, parents, temperature=0.0, uniforms=None, draft
     """Which drafted tokens the target accepts, and the token after them: logits bf16 or float32 [T, V] (the target's after each node),
     tokens int64 [T], parents int32 [T] -> (path int32 [T], count int32 [1], next int64 [1]), all on the device: the accepted nodes from
     node 0 on, -1 behind them, their number, the next token.
-    temperature 0: greedy.  Otherwise uniforms float32 [T] in [0, 1) decide (entry 0 draws the next token, entry c tries node c), in float64, such
-    that the tokens are distributed as softmax(logits / temperature) whatever the draft was.  draft float32 [T, V]: the distributions that
-    a node's children were drawn from, with siblings, the most children of a node (1..16; further ones are not tried).  Without it the drafts
-    are taken as given (a draft's likeliest tokens, tokens from the text)."""
+    temperature 0: greedy.  Otherwise uniforms float32 [T] in [0, 1) decide (entry 0 draws the next token, entry c tries node c), in
+    float64, such that the tokens are distributed as softmax(logits / temperature) whatever the draft was.  draft float32 [T, V]: the
+    distributions that a node's children were drawn from, with siblings, the most children of a node (1..16; further ones are not tried).
+    Without it the drafts are taken as given (a draft's likeliest tokens, tokens from the text)."""
     _check(logits.dim() == 2 and logits.dtype in (BF, torch.float32), "logits are bfloat16 or float32 [T, V]")
     T, V = logits.shape
-    _check(tokens.dtype == torch.int64 and parents.dtype == torch.int32 and tokens.numel() == parents.numel() == T, "tokens are int64 [T], parents int32 [T]")
+    _check(tokens.dtype == torch.int64 and parents.dtype == torch.int32 and tokens.numel() == parents.numel() == T,
+           "tokens are int64 [T], parents int32 [T]")
     temperature = float(temperature)
     levels = 0
     if temperature == 0:
@@ -67,6 +68,6 @@ def verify_drafts(logits, tokens, parents, temperature=0.0, uniforms=None, draft
     path, count, token = n.empty_i32(logits, T), n.empty_i32(logits, 1), n.empty_i64(logits, 1)
     need = n.scmx_verify_workspace(T, V, levels)
     work = n.empty_u8(logits, need)
-    n.scmx_verify_drafts(tokens, parents, logits, int(logits.dtype == torch.float32), draft, temperature, uniforms, path, count, token, T, V, levels, work,
-                         need)
+    n.scmx_verify_drafts(tokens, parents, logits, int(logits.dtype == torch.float32), draft, temperature, uniforms, path, count, token, T,
+                         V, levels, work, need)
     return path, count, token

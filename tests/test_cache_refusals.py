@@ -4,8 +4,8 @@ import torch
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="the calls that are accepted would be launched")
-@pytest.mark.parametrize("scale,refused", [(2.4e38, True), (-2.4e38, True), (3.0e38, True), (float("inf"), True), (float("nan"), True), (2.3e38, False), (-2.3e38, False),
-                                           (0.0, False)])
+@pytest.mark.parametrize("scale,refused", [(2.4e38, True), (-2.4e38, True), (3.0e38, True), (float("inf"), True), (float("nan"), True),
+                                           (2.3e38, False), (-2.3e38, False), (0.0, False)])
 def test_attention_scales(scale, refused):
     """The scale is taken in powers of two, so that it has to be finite times log2 e."""
     import mxfp4_int8_m5_amd as scmx

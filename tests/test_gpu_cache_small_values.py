@@ -17,9 +17,9 @@ def C():
 
 
 def check_relative(out, q, c, masks, pos, scale):
-    """As tests.test_gpu_cache.check_attention, without its term of the largest value: a weight (probability times scale) is a half-precision
-    number with the largest between 2^8 and 2^14, so that one of less than 2^-14 is off by up to 2^-25, which is 2^-33 of the largest;
-    a code is up to 127."""
+    """As tests.test_gpu_cache.check_attention, without its term of the largest value: a weight (probability times scale) is a
+    half-precision number with the largest between 2^8 and 2^14, so that one of less than 2^-14 is off by up to 2^-25, which is 2^-33 of
+    the largest; a code is up to 127."""
     hk, _, d = c[0].shape
     T, hq = q.shape[1], q.shape[0]
     k, v, qs, vs = values(c[0], c[2]), values(c[1], c[3]), f64(q), f64(c[3])

@@ -49,7 +49,7 @@ def test_what_is_left_after_refusals_of_nearly_everything(D, chunked):   # noqa:
         at = rng.choice(V, 400, replace=False) if chunked else rng.choice(4000, 400, replace=False)
         logits = np.full((5, V), -np.inf, np.float32)
         small = np.exp(0.5 * rng.normal(size=397))
-        row = np.concatenate([[0.0], [-22.5 * np.log(2)], [-45 * np.log(2)], np.log(small / small.sum()) - 45 * np.log(2)]).astype(np.float32)
+        row = np.concatenate([np.log(2) * np.array([0.0, -22.5, -45.0]), np.log(small / small.sum()) - 45 * np.log(2)]).astype(np.float32)
         logits[0, at] = row
         logits[1:, 5] = 0.0
         e = np.exp(row.astype(np.float64))
