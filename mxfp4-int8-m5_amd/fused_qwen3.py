@@ -16,6 +16,7 @@ the reference (e2e/decode.py:30-33): one graph launch replaces about ten kernel 
 Beyond the reference: caches in 8 bits (make_cache(bits=8)) in every path, and DraftQwen3, a decode step that decides several
 tokens at once, a tree of drafted ones verified against the model's own probabilities."""
 import json
+import operator
 import os
 from dataclasses import dataclass, fields
 
@@ -234,6 +235,10 @@ class FusedQwen3:
         return self.logits(self.hidden(ids, cache))
 
 
+def _same(a, b):
+    return len(a) == len(b) and all(map(operator.is_, a, b))
+
+
 class DecodeQwen3:
     """Batch-1 decode from a FusedQwen3 with epilogue="gemm": W4A8 GEMVs on the packed weights
     (e2e/decode.py:29-99).  fuse_prologue="act" (default): RMSNorm + INT8 as separate kernels, the per-token INT8 of
@@ -241,9 +246,10 @@ class DecodeQwen3:
     separate.  graphs=True captures the two fixed-shape halves of every layer in HIP graphs on first use;
     graphs="step" captures the whole step (all layers and the output head) as one graph per cache.  A graph holds raw
     pointers into the cache it was captured with, so the decoder keeps that cache object alive next to the graph and,
-    handed a different one, captures again IN PLACE of the old entries: at most one cache (the latest) and its graphs
-    are held, a fresh cache per prompt does not accumulate; `release(cache)` drops them before the next prompt.  Tensors returned by `step` are fresh in every mode (the graphs' static outputs are
-    cloned).  fuse_attn=True (default): q/k norm, rotary embedding, cache append and the attention in one kernel;
+    handed a different one (or the same with other layers or tensors in it), captures again IN PLACE of the old entries:
+    at most one cache (the latest) and its graphs are held, a fresh cache per prompt does not accumulate;
+    `release(cache)` drops them before the next prompt.  Tensors returned by `step` are fresh in every mode (the graphs'
+    static outputs are cloned).  fuse_attn=True (default): q/k norm, rotary embedding, cache append and the attention in one kernel;
     False: two kernels (same bits).  head="packed": the output projection quantized to the published SC-MXFP4 format
     (32-blocks, multipliers 1,2,4,8) whatever format the model's layers use."""
 
@@ -331,20 +337,28 @@ class DecodeQwen3:
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 out = fn(*static)
-            self.graphs[key] = (g, static, out, owner)
+            self.graphs[key] = (g, static, out, owner, self._memory(owner))
         return self.graphs[key]
 
+    @staticmethod
+    def _memory(owner):
+        """The tensors of a cache (a list of layers) or of one layer: what captured kernels point into.  (28 layers:
+        10 - 20 us of a drafted step, which waits for the host; a plain one's are hidden.)"""
+        layers = owner if isinstance(owner, (list, tuple)) else () if owner is None else (owner,)
+        return [getattr(c, name, None) for name in ("k", "v", "kscale", "vscale") for c in layers]
+
     def _lookup(self, key, owner):
-        """The entry stored under key if it was captured for this very owner object; an entry of another owner is
-        dropped (with its graph, static buffers and the reference that kept the old cache alive)."""
+        """The entry stored under key if it was captured for this very owner object, with the tensors it has now (a list
+        may have got other layers, a layer other tensors); any other is dropped (with its graph, static buffers and the
+        references that kept the old cache alive)."""
         entry = self.graphs.get(key)
-        if entry is not None and entry[3] is not owner:
+        if entry is not None and (entry[3] is not owner or len(entry) > 4 and not _same(entry[4], self._memory(owner))):
             del self.graphs[key]
             entry = None
         return entry
 
     def _replay(self, key, fn, inputs, owner=None):
-        g, static, out, _ = self._capture(key, fn, inputs, owner)
+        g, static, out = self._capture(key, fn, inputs, owner)[:3]
         for dst, src in zip(static, inputs):
             dst.copy_(src)
         g.replay()
@@ -430,12 +444,16 @@ class DraftQwen3(DecodeQwen3):
 
     def _key(self, T, levels, temperature, cache):
         """The key of a step's graph; drops the graphs of other caches, and of a temperature too many."""
+        slot = "draft", T, levels, temperature
+        entry = self.graphs.get(slot)
+        if entry is not None and entry[3] is cache and temperature in (0.0, *self.temperatures[-1:]):
+            return slot
         if temperature != 0:
             self.temperatures = [t for t in self.temperatures if t != temperature][1 - self.TEMPERATURES:] + [temperature]
         for key, entry in list(self.graphs.items()):
             if key[0] == "draft" and (entry[3] is not cache or key[3] not in (0.0, *self.temperatures)):
                 del self.graphs[key]
-        return "draft", T, levels, temperature
+        return slot
 
     def _linear(self, x, w, epi, res=None, nw=None):
         """A linear on a few rows x [T, K], RMSNorm with weight nw first.  One row takes the norm in the GEMV's prologue, several rows
