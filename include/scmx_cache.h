@@ -49,7 +49,8 @@ int scmx_cache_keep(const uint64_t* caches, int layers, int eight, int hk, int d
  * is summed from the same products, in float32, over the scales: a row whose product is below 2^-110 of another's may count as not
  * seen.  V scales are 2^-110 .. 2^122, as the append's are, or 0 for a row of zeros, which takes part as one with the scale 2^-80 would
  * (others are not looked for: a negative or subnormal one gives NaN).  Over a bf16 cache the probabilities are rounded to bf16, in the
- * sum and in the denominator alike (2^-8 of sum p |v| at most).  scale is finite, times log2 e too.
+ * sum and in the denominator alike (2^-8 of sum p |v| at most), and the sum, in float32, is up to 2^8 (pos + T) times the largest
+ * |v|: values up to 1e30 over a million rows.  scale is finite, times log2 e too.
  * splits (1..64): ranges the rows are cut into, a workgroup per range, KV head and 16 or 32 query rows; more than one needs
  * `workspace`, float [splits * T * hq * (d + 2)], 16-byte aligned, used between the call's two launches.
  * scmx_attn_tree_splits: how many to take for n rows in all (the cache's, where the position is on the device); 1 for arguments that
