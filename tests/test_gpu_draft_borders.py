@@ -77,3 +77,31 @@ def test_rows_without_a_finite_logit_and_drafted_tokens(D, V):   # noqa: F811
                 u[1:] = 0.99999994
             tokens, parents = [0, *kids], [-1, 0, 0, 0, 0]
             assert run(D, logits, tokens, parents, torch.float32, 0.7, u) == O.verify(logits, tokens, parents, 0.7, u)
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_random_numbers_beside_a_second_sibling_s_border(D, drawn):   # noqa: F811
+    """After a refusal: the residual's share of the second child, where it holds 1.1 times the draft's at least (a digit of cancellation)."""
+    V, temperature, rng, found = 24, 0.7, np.random.default_rng(3), 0
+    logits = (3 * rng.normal(size=(300000, V))).astype(np.float32)
+    q = np.maximum(rng.dirichlet(np.ones(V), 300000), 1e-9).astype(np.float32)
+    p = logits.astype(np.float64) / temperature
+    p = np.exp(p - p.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    if drawn:
+        r = np.maximum(p - q, 0)
+        r /= r.sum(1, keepdims=True)
+        border = r[:, 1] / q[:, 1]
+        fits = (q[:, 0] * 0.99 > p[:, 0]) & (p[:, 1] > 1.1 * q[:, 1]) & (border < 0.99)
+    else:
+        border = p[:, 1] / p[:, 1:].sum(1)
+        fits = (p[:, 0] < 0.99) & (border < 0.99)
+    u = border.astype(np.float32)
+    off = np.abs(u / np.maximum(border, 1e-300) - 1)
+    for i in np.nonzero(fits & (off > 3e-13) & (off < (1e-10 if drawn else 2e-11)))[0][:12]:
+        rows, us, qs = np.repeat(logits[i:i + 1], 3, 0), [0.3, 0.99999994, u[i]], np.repeat(q[i:i + 1], 3, 0) if drawn else None
+        got = run(D, rows, [0, 0, 1], [-1, 0, 0], torch.float32, temperature, us, qs, 2)
+        assert (got[0] == [0, 2]) == (u[i] < border[i])
+        assert got == O.verify(rows, [0, 0, 1], [-1, 0, 0], temperature, us, qs, 2)
+        found += 1
+    assert found >= 4
