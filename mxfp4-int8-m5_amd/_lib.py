@@ -1,4 +1,4 @@
-"""Access to libscmx.so (the C ABI declared in include/scmx.h and scmx_cache.h): `native()` is what the wrappers call, tensors in, one
+"""Access to libscmx.so (the C ABI declared in include/scmx.h, scmx_cache.h and scmx_mx.h): `native()` is what the wrappers call, tensors in, one
 native call per launch (csrc/torch_binding.cpp); `load()` the whole ABI through ctypes, for the queries and for foreign callers,
 with `call`, `ptr` and `stream` to check a status and to make arguments of tensors.
 There is no fallback: a missing or incomplete library raises, and so does every call that returns a negative status."""
@@ -82,6 +82,19 @@ CACHE_SIGNATURES = {
     "scmx_verify_workspace": (_Z, [_I, _I, _I]),
     "scmx_verify_drafts": (_I, [_P, _P, _P, _I, _P, C.c_double, _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P]),
 }
+# and of include/scmx_mx.h
+MX_SIGNATURES = {
+    "scmx_mx_quantize": (_I, [_P, _I, _L, _P, _F, _P, _P, _I, _I, _P]),
+    "scmx_mx_dequantize": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "scmx_mx_mm": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "scmx_mx_linear_workspace": (_Z, [_I, _I, _I]),
+    "scmx_mx_linear": (_I, [_P, _L, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
+    "scmx_cache4_write": (_I, [_P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _I, _P]),
+    "scmx_cache4_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "scmx_cache4_keep": (_I, [_P, _I, _I, _I, _I, _P, _P, _I, _P, _L, _P]),
+    "scmx_attn_tree4": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _I, _I, _I, _I, _F, _P, _I, _P]),
+    "scmx_attn_tree4_splits": (_I, [_I, _I, _I, _I, _I]),
+}
 
 _lib = None
 
@@ -94,7 +107,7 @@ def load():
             raise RuntimeError(f"{LIB_PATH} is missing: build it with `python {os.path.join(HERE, 'build.py')}` "
                                "(there is no CPU or PyTorch fallback for these kernels)")
         lib = C.CDLL(LIB_PATH)
-        for name, (res, args) in (SIGNATURES | CACHE_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | CACHE_SIGNATURES | MX_SIGNATURES).items():
             fn = getattr(lib, name)       # AttributeError if the library lacks a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = lib

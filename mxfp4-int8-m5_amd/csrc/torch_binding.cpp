@@ -1,5 +1,5 @@
 // Python binding of the C ABI for torch tensors: `_binding`, a module whose functions are the entry points of
-// include/scmx.h and scmx_cache.h that enqueue work (and six of their queries), under the same names and with the same arguments except the
+// include/scmx.h, scmx_cache.h and scmx_mx.h that enqueue work (and their queries of sizes), under the same names and with the same arguments except the
 // last.  A pointer argument takes a tensor (contiguous, on the GPU), None or an integer address; a format argument an object
 // whose buffer is the scmx_format; the stream is the caller's current one and is not passed.  A negative status raises.
 //
@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/scmx_cache.h"
+#include "../../include/scmx_mx.h"
 
 namespace {
 
@@ -255,18 +256,28 @@ const at::Tensor* local(PyObject* o, at::ScalarType type) {
 struct CacheTensors {
     const at::Tensor *k, *v, *ks = nullptr, *vs = nullptr;
     int64_t hk, rows, d;
+    bool four = false;
     float* scale(const at::Tensor* t) const { return t ? static_cast<float*>(t->data_ptr()) : nullptr; }
+    static uint8_t* bytes(const at::Tensor* t) { return static_cast<uint8_t*>(t->data_ptr()); }
 };
 bool cache_of(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, CacheTensors& c) {
     const bool eight = ks != Py_None;
-    const at::ScalarType type = eight ? at::ScalarType::Char : at::ScalarType::BFloat16;
+    c.four = eight && THPVariable_Check(ks) && THPVariable_Unpack(ks).scalar_type() == at::ScalarType::Byte;
+    const at::ScalarType type = c.four ? at::ScalarType::Byte : eight ? at::ScalarType::Char : at::ScalarType::BFloat16;
     c.k = local(k, type);
     c.v = local(v, type);
     if (!c.k || !c.v || c.k->dim() != 3 || c.k->sizes() != c.v->sizes() || eight != (vs != Py_None)) return false;
     c.hk = c.k->size(0);
     c.rows = c.k->size(1);
     c.d = c.k->size(2);
-    if (eight) {
+    if (c.four) {
+        c.ks = local(ks, at::ScalarType::Byte);
+        c.vs = local(vs, at::ScalarType::Byte);
+        if (!c.ks || !c.vs || c.d % 16) return false;
+        for (const at::Tensor* t : {c.ks, c.vs})
+            if (t->dim() != 3 || t->size(0) != c.hk || t->size(1) != c.rows || t->size(2) != c.d / 16) return false;
+        c.d *= 2;
+    } else if (eight) {
         c.ks = local(ks, at::ScalarType::Float);
         c.vs = local(vs, at::ScalarType::Float);
         if (!c.ks || !c.vs) return false;
@@ -335,12 +346,17 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const NoGil released;
             q = at::Tensor(at::detail::empty_strided_cuda({hq, L, d}, {d, hq * d, 1}, at::ScalarType::BFloat16, y->device()));
             const auto bf = [](const at::Tensor* t) { return static_cast<const uint16_t*>(t->data_ptr()); };
-            rc = scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), float(PyFloat_AS_DOUBLE(args[3])),
-                                  static_cast<uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs),
-                                  int(L), int(hq), int(hk), int(d), static_cast<const float*>(freq->data_ptr()), depth, dev, pos,
-                                  int(c.rows), stream());
+            const float eps = float(PyFloat_AS_DOUBLE(args[3]));
+            auto* out = static_cast<uint16_t*>(q.data_ptr());
+            const auto* f = static_cast<const float*>(freq->data_ptr());
+            rc = c.four ? scmx_cache4_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), eps, out, c.bytes(c.k), c.bytes(c.v),
+                                            c.bytes(c.ks), c.bytes(c.vs), int(L), int(hq), int(hk), int(d), f, depth, dev, pos,
+                                            int(c.rows), stream())
+                        : scmx_cache_write(nullptr, nullptr, nullptr, bf(y), bf(qn), bf(kn), eps, out, c.k->data_ptr(), c.v->data_ptr(),
+                                           c.scale(c.ks), c.scale(c.vs), int(L), int(hq), int(hk), int(d), f, depth, dev, pos,
+                                           int(c.rows), stream());
         }
-        if (rc != SCMX_OK) return status("scmx_cache_write", rc);
+        if (rc != SCMX_OK) return status(c.four ? "scmx_cache4_write" : "scmx_cache_write", rc);
         return THPVariable_Wrap(std::move(q));
     } catch (...) {
         return raised();
@@ -366,7 +382,8 @@ PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
             !optional_of(args[4], at::ScalarType::Long, T, mask) || pos < 0 || pos > INT32_MAX - 64)
             Py_RETURN_NONE;
         const int splits = args[8] != Py_None ? convert<int>(args[8])
-                                              : scmx_attn_tree_splits(int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
+                                              : (c.four ? scmx_attn_tree4_splits : scmx_attn_tree_splits)(
+                                                    int(T), dev ? int(c.rows) : int(pos + T), int(hq), int(c.hk), int(d));
         if (splits < 1 || splits > 64) Py_RETURN_NONE;
         const float scale = args[7] == Py_None ? float(1.0 / std::sqrt(double(d))) : float(PyFloat_AS_DOUBLE(args[7]));
         at::Tensor out;
@@ -375,11 +392,15 @@ PyObject* attn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const NoGil released;
             out = fresh(q, at::ScalarType::BFloat16, {T, hq * d});
             const c10::DataPtr work = scratch(splits > 1 ? size_t(splits * T * hq * (d + 2)) * sizeof(float) : 0);
-            rc = scmx_attn_tree(static_cast<const uint16_t*>(q.data_ptr()), c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs),
-                                mask, dev, pos, static_cast<uint16_t*>(out.data_ptr()), int(T), int(hq), int(c.hk), int(d),
-                                int(c.rows), scale, splits > 1 ? static_cast<float*>(work.get()) : nullptr, splits, stream());
+            const auto* from = static_cast<const uint16_t*>(q.data_ptr());
+            auto* to = static_cast<uint16_t*>(out.data_ptr());
+            float* parts = splits > 1 ? static_cast<float*>(work.get()) : nullptr;
+            rc = c.four ? scmx_attn_tree4(from, c.bytes(c.k), c.bytes(c.v), c.bytes(c.ks), c.bytes(c.vs), mask, dev, pos, to, int(T), int(hq),
+                                          int(c.hk), int(d), int(c.rows), scale, parts, splits, stream())
+                        : scmx_attn_tree(from, c.k->data_ptr(), c.v->data_ptr(), c.scale(c.ks), c.scale(c.vs), mask, dev, pos, to, int(T),
+                                         int(hq), int(c.hk), int(d), int(c.rows), scale, parts, splits, stream());
         }
-        if (rc != SCMX_OK) return status("scmx_attn_tree", rc);
+        if (rc != SCMX_OK) return status(c.four ? "scmx_attn_tree4" : "scmx_attn_tree", rc);
         return THPVariable_Wrap(std::move(out));
     } catch (...) {
         return raised();
@@ -401,10 +422,13 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
             k = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
             v = fresh(*c.k, at::ScalarType::BFloat16, {c.hk, rows, c.d});
             const auto codes = [](const at::Tensor* t) { return static_cast<const int8_t*>(t->data_ptr()); };
-            rc = scmx_cache_read(codes(c.k), codes(c.v), c.scale(c.ks), c.scale(c.vs), static_cast<uint16_t*>(k.data_ptr()),
-                                 static_cast<uint16_t*>(v.data_ptr()), int(c.hk), int(c.d), int(c.rows), int(row0), int(rows), stream());
+            auto *kp = static_cast<uint16_t*>(k.data_ptr()), *vp = static_cast<uint16_t*>(v.data_ptr());
+            rc = c.four ? scmx_cache4_read(c.bytes(c.k), c.bytes(c.v), c.bytes(c.ks), c.bytes(c.vs), kp, vp, int(c.hk), int(c.d), int(c.rows),
+                                           int(row0), int(rows), stream())
+                        : scmx_cache_read(codes(c.k), codes(c.v), c.scale(c.ks), c.scale(c.vs), kp, vp, int(c.hk), int(c.d), int(c.rows),
+                                          int(row0), int(rows), stream());
         }
-        if (rc != SCMX_OK) return status("scmx_cache_read", rc);
+        if (rc != SCMX_OK) return status(c.four ? "scmx_cache4_read" : "scmx_cache_read", rc);
         PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
         return Py_BuildValue("(NN)", pk, pv);
     } catch (...) {
@@ -432,15 +456,17 @@ PyObject* cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
             if (!cache_of(PyTuple_GET_ITEM(t, 0), PyTuple_GET_ITEM(t, 1), PyTuple_GET_ITEM(t, 2), PyTuple_GET_ITEM(t, 3), c))
                 Py_RETURN_NONE;
             if (i == 0) first = c;
-            else if (c.hk != first.hk || c.rows != first.rows || c.d != first.d || !c.ks != !first.ks) Py_RETURN_NONE;
+            else if (c.hk != first.hk || c.rows != first.rows || c.d != first.d || !c.ks != !first.ks || c.four != first.four) Py_RETURN_NONE;
             for (const at::Tensor* x : {c.k, c.v, c.ks, c.vs})
                 if (x) pointers.push_back(reinterpret_cast<uintptr_t>(x->data_ptr()));
         }
         if (layers < 1 || layers > 1024) Py_RETURN_NONE;
-        const int rc = scmx_cache_keep(pointers.data(), int(layers), first.ks != nullptr, int(first.hk), int(first.d), int(first.rows),
-                                       static_cast<const int32_t*>(path->data_ptr()), static_cast<const int32_t*>(count->data_ptr()),
-                                       int(path->numel()), dev, pos, stream());
-        if (rc != SCMX_OK) return status("scmx_cache_keep", rc);
+        const auto ints = [](const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); };
+        const int rc = first.four ? scmx_cache4_keep(pointers.data(), int(layers), int(first.hk), int(first.d), int(first.rows), ints(path),
+                                                     ints(count), int(path->numel()), dev, pos, stream())
+                                  : scmx_cache_keep(pointers.data(), int(layers), first.ks != nullptr, int(first.hk), int(first.d),
+                                                    int(first.rows), ints(path), ints(count), int(path->numel()), dev, pos, stream());
+        if (rc != SCMX_OK) return status(first.four ? "scmx_cache4_keep" : "scmx_cache_keep", rc);
         Py_RETURN_TRUE;
     } catch (...) {
         return raised();
@@ -483,6 +509,124 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
+// ---- microscaled 4-bit values: sc_mx's functions for the operands of every step, in one call as above ------------------------------
+
+// Rows [M, K] of `x` on the current device, K contiguous values each, `ld` apart.
+bool rows_of(const at::Tensor& x, int64_t& M, int64_t& K, int64_t& ld) {
+    if (!x.is_cuda() || x.get_device() != c10::hip::current_device() || x.dim() != 2) return false;
+    M = x.size(0);
+    K = x.size(1);
+    ld = M > 1 ? x.stride(0) : K;
+    return M <= INT32_MAX && K >= 32 && K % 32 == 0 && K <= INT32_MAX && x.stride(1) == 1 && ld >= K;
+}
+// None, or the weight bf16 [K] of a norm of up to 16384 values.
+bool norm_of(PyObject* o, PyObject* eps, int64_t K, const uint16_t*& nw, float& e) {
+    nw = nullptr;
+    e = 0.0f;
+    if (o == Py_None) return true;
+    const at::Tensor* t = local(o, at::ScalarType::BFloat16);
+    if (!t || t->numel() != K || K > 16384 || !PyFloat_Check(eps)) return false;
+    nw = static_cast<const uint16_t*>(t->data_ptr());
+    e = float(PyFloat_AS_DOUBLE(eps));
+    return true;
+}
+// codes uint8 [rows, K / 2] and scales uint8 [rows, K / 32].
+bool pair_of(PyObject* codes, PyObject* scales, const at::Tensor*& c, const at::Tensor*& s) {
+    c = local(codes, at::ScalarType::Byte);
+    s = local(scales, at::ScalarType::Byte);
+    return c && s && c->dim() == 2 && s->dim() == 2 && c->size(0) == s->size(0) && c->size(1) == 16 * s->size(1) && s->size(1) > 0 &&
+           c->size(0) <= INT32_MAX && c->size(1) <= INT32_MAX / 2;
+}
+uint8_t* bytes(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+// mx_quantize(x, nw, eps)
+PyObject* mx_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 3) fail(PyExc_TypeError, "mx_quantize takes 3 arguments");
+        int64_t M, K, ld;
+        const uint16_t* nw;
+        float eps;
+        if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
+        const at::Tensor& x = THPVariable_Unpack(args[0]);
+        const at::ScalarType t = x.scalar_type();
+        const int type = t == at::ScalarType::BFloat16 ? SCMX_MX_BF16 : t == at::ScalarType::Half ? SCMX_MX_F16 : t == at::ScalarType::Float ? SCMX_MX_F32 : -1;
+        if (type < 0 || !rows_of(x, M, K, ld) || !norm_of(args[1], args[2], K, nw, eps) || (nw && type != SCMX_MX_BF16)) Py_RETURN_NONE;
+        at::Tensor codes, scales;
+        int rc;
+        {
+            const NoGil released;
+            codes = fresh(x, at::ScalarType::Byte, {M, K / 2});
+            scales = fresh(x, at::ScalarType::Byte, {M, K / 32});
+            rc = scmx_mx_quantize(x.data_ptr(), type, ld, nw, eps, bytes(codes), bytes(scales), int(M), int(K), stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_mx_quantize", rc);
+        PyObject *a = THPVariable_Wrap(std::move(codes)), *b = THPVariable_Wrap(std::move(scales));
+        return Py_BuildValue("(NN)", a, b);
+    } catch (...) {
+        return raised();
+    }
+}
+
+// mx_dequantize(codes, scales, f32)
+PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 3) fail(PyExc_TypeError, "mx_dequantize takes 3 arguments");
+        const at::Tensor *codes, *scales;
+        if (!PyBool_Check(args[2]) || !pair_of(args[0], args[1], codes, scales)) Py_RETURN_NONE;
+        const bool f32 = args[2] == Py_True;
+        const int64_t M = codes->size(0), K = 2 * codes->size(1);
+        at::Tensor out;
+        int rc;
+        {
+            const NoGil released;
+            out = fresh(*codes, f32 ? at::ScalarType::Float : at::ScalarType::BFloat16, {M, K});
+            rc = scmx_mx_dequantize(bytes(*codes), bytes(*scales), out.data_ptr(), f32 ? SCMX_MX_F32 : SCMX_MX_BF16, int(M), int(K), stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_mx_dequantize", rc);
+        return THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        return raised();
+    }
+}
+
+// mx_linear(x, wcodes, wscales, epi, res, nw, eps)
+PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 7) fail(PyExc_TypeError, "mx_linear takes 7 arguments");
+        int64_t M, K, ld;
+        const uint16_t* nw;
+        float eps;
+        const at::Tensor *codes, *scales, *res = nullptr;
+        if (!THPVariable_Check(args[0]) || !PyLong_CheckExact(args[3])) Py_RETURN_NONE;
+        const at::Tensor& x = THPVariable_Unpack(args[0]);
+        const int64_t epi = as_int(args[3]);
+        if (x.scalar_type() != at::ScalarType::BFloat16 || !rows_of(x, M, K, ld) || !pair_of(args[1], args[2], codes, scales) ||
+            2 * codes->size(1) != K || !norm_of(args[5], args[6], K, nw, eps) || epi < 1 || epi > 3)
+            Py_RETURN_NONE;
+        const int64_t N = codes->size(0);
+        if (N < 1 || (epi == 3 && N % 4)) Py_RETURN_NONE;
+        if (epi == 2) {
+            res = local(args[4], at::ScalarType::BFloat16);
+            if (!res || res->dim() != 2 || res->size(0) != M || res->size(1) != N) Py_RETURN_NONE;
+        }
+        at::Tensor out;
+        int rc;
+        {
+            const NoGil released;
+            out = fresh(x, at::ScalarType::BFloat16, {M, epi == 3 ? N / 2 : N});
+            const size_t need = scmx_mx_linear_workspace(int(M), int(N), int(K));
+            const c10::DataPtr work = scratch(need);
+            rc = scmx_mx_linear(static_cast<const uint16_t*>(x.data_ptr()), ld, nw, eps, bytes(*codes), bytes(*scales),
+                                res ? static_cast<const uint16_t*>(res->data_ptr()) : nullptr, static_cast<uint16_t*>(out.data_ptr()), int(epi),
+                                int(M), int(N), int(K), work.get(), need, stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_mx_linear", rc);
+        return THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        return raised();
+    }
+}
+
 #define ENTRY(fn) \
     {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(((Call<&fn>::name = #fn), &Call<&fn>::call))), METH_FASTCALL, nullptr}
 #define QUERY(fn) {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Query<&fn>::call)), METH_FASTCALL, nullptr}
@@ -510,6 +654,9 @@ PyMODINIT_FUNC PyInit__binding() {
         ENTRY(scmx_cache_write), ENTRY(scmx_cache_read), ENTRY(scmx_cache_keep), ENTRY(scmx_attn_tree), ENTRY(scmx_verify_drafts),
         QUERY(scmx_verify_workspace), QUERY(scmx_attn_tree_splits),
         FUNCTION(cache_write), FUNCTION(cache_read), FUNCTION(cache_keep), FUNCTION(attn_tree), FUNCTION(verify_drafts),
+        ENTRY(scmx_mx_quantize), ENTRY(scmx_mx_dequantize), ENTRY(scmx_mx_mm), ENTRY(scmx_mx_linear), ENTRY(scmx_cache4_write),
+        ENTRY(scmx_cache4_read), ENTRY(scmx_cache4_keep), ENTRY(scmx_attn_tree4), QUERY(scmx_mx_linear_workspace), QUERY(scmx_attn_tree4_splits),
+        FUNCTION(mx_quantize), FUNCTION(mx_dequantize), FUNCTION(mx_linear),
         FUNCTION(gemv),
         EMPTY(bf16, BFloat16), EMPTY(i8, Char), EMPTY(u8, Byte), EMPTY(i32, Int), EMPTY(i64, Long), EMPTY(f32, Float),
         {nullptr, nullptr, 0, nullptr}};
