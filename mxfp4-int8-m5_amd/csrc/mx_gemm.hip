@@ -1,8 +1,8 @@
-// Products of MXFP4 operands (include/scmx_mx.h, scmx_mx_mm and scmx_mx_linear) on the scaled matrix instructions: v_mfma_scale_f32_32x32x64 and
-// 16x16x128, both operands E2M1 with an E8M0 byte for 32 values, sums in float32.  The weights are the row operand, so that a lane's
+// Products of MXFP4 operands (include/scmx_mx.h, scmx_mx_mm and scmx_mx_linear) on the scaled matrix instructions: v_mfma_scale_f32_16x16x128,
+// both operands E2M1 with an E8M0 byte for 32 values, sums in float32.  The weights are the row operand, so that a lane's
 // accumulators are groups of four consecutive columns n of one row m, two gates and their two ups among them.
 //
-// A lane's operand of either instruction is 16 bytes of codes, one block of 32 values, with the block's byte beside it.  Which blocks
+// A lane's operand is 16 bytes of codes, one block of 32 values, with the block's byte beside it.  Which blocks
 // of K meet in an instruction is free, as long as both operands take the same.
 #include <type_traits>
 
@@ -11,7 +11,6 @@
 namespace scmx {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct MxArgs {
     const uint8_t* x;
@@ -30,29 +29,40 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
 }
 
-// Columns n .. n + 3 of row m (n a multiple of 4, both inside or past the ends).
-__device__ __forceinline__ void store4(const MxArgs& a, int m, int n, const float* v) {
-    if (m >= a.M || n >= a.N) return;
-    if (a.epi == 3) {
-        *reinterpret_cast<uint32_t*>(a.out + (size_t(m) * a.N + n) / 2) = f32_to_bf16x2(silu_mul(v[0], v[2]), silu_mul(v[1], v[3]));
-        return;
-    }
-    const size_t at = size_t(m) * a.N + n;
-    if (a.N % 4 == 0) {
-        u32x2 r = {0, 0};
-        if (a.epi == 2) r = *reinterpret_cast<const u32x2*>(a.res + at);
-        *reinterpret_cast<u32x2*>(a.out + at) =
-            a.epi == 2 ? u32x2{f32_to_bf16x2(v[0] + bf16_lo(r[0]), v[1] + bf16_hi(r[0])), f32_to_bf16x2(v[2] + bf16_lo(r[1]), v[3] + bf16_hi(r[1]))}
-                       : u32x2{f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3])};
+// Columns n .. n + 3 of row m, those that are inside (n is a multiple of 4), one by one.
+template <int EPI>
+__device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
+    if (m >= a.M) return;
+    if constexpr (EPI == 3) {
+        if (n < a.N) *reinterpret_cast<uint32_t*>(a.out + (size_t(m) * a.N + n) / 2) = f32_to_bf16x2(silu_mul(v[0], v[2]), silu_mul(v[1], v[3]));
     } else {
+        const size_t at = size_t(m) * a.N + n;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (n + i < a.N) a.out[at + i] = f32_to_bf16(a.epi == 2 ? v[i] + bf16_to_f32(a.res[at + i]) : v[i]);
+            if (n + i < a.N) a.out[at + i] = f32_to_bf16(EPI == 2 ? v[i] + bf16_to_f32(a.res[at + i]) : v[i]);
     }
+}
+
+// Columns n .. n + 7 (SwiGLU: n + 15) of row m, all inside, in one store of eight values; a row starts at any even address (the hardware takes
+// vectors at them).
+template <int EPI>
+__device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float* v) {
+    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    const size_t at = EPI == 3 ? (size_t(m) * a.N + n) / 2 : size_t(m) * a.N + n;
+    u32x4 r = {0, 0, 0, 0}, w;
+    if constexpr (EPI == 2) r = *reinterpret_cast<const u32x4u*>(a.res + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (EPI == 1) w[i] = f32_to_bf16x2(v[2 * i], v[2 * i + 1]);
+        else if constexpr (EPI == 2) w[i] = f32_to_bf16x2(v[2 * i] + bf16_lo(r[i]), v[2 * i + 1] + bf16_hi(r[i]));
+        else w[i] = f32_to_bf16x2(silu_mul(v[4 * i], v[4 * i + 2]), silu_mul(v[4 * i + 1], v[4 * i + 3]));
+    }
+    *reinterpret_cast<u32x4u*>(a.out + at) = w;
 }
 
 // Few rows: a workgroup per 16 columns and 16 rows, its waves take the steps of 128 along K in turn, straight from memory.
 constexpr int RWAVES = 4;
+template <int EPI>
 __global__ __launch_bounds__(64 * RWAVES) void mx_rows_kernel(const MxArgs a) {
     __shared__ f32x4 s_acc[RWAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, g = lane >> 4;
@@ -81,116 +91,266 @@ __global__ __launch_bounds__(64 * RWAVES) void mx_rows_kernel(const MxArgs a) {
     for (int w = 1; w < RWAVES; ++w)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += s_acc[w][lane][i];
-    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-    store4(a, m0 + ln, n0 + 4 * g, v);
+    store4<EPI>(a, m0 + ln, n0 + 4 * g, acc);
 }
 
-// 16 bytes a lane past the registers: to lds + 16 * lane, zeros where `at` is behind the buffer's end.  (A function of its own: in a template
-// the host's pass would drop the kernel.)
-__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t from, uint8_t* lds, unsigned at) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)lds, 16, int(at), 0, 0, 0);
+// 16 bytes a lane past the registers: to LDS byte `lds` + 16 * lane, zeros where `at` is behind the buffer's end.  Written out because the
+// compiler, which cannot tell one stage's place from another's, would wait for all such loads before each read of LDS; who reads what
+// they bring waits for them itself.  (m0 is the place; a state between its setting and its use.)
+typedef uint32_t Buffer __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_lds16(Buffer from, unsigned lds, unsigned at) {
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "{m0}"(lds), "v"(at), "s"(from) : "memory");
+}
+__device__ __forceinline__ Buffer buffer_of(const uint8_t* p, unsigned bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    return Buffer{uint32_t(__builtin_amdgcn_readfirstlane(int(at))), uint32_t(__builtin_amdgcn_readfirstlane(int(at >> 32))) & 0xFFFFu,
+                  uint32_t(__builtin_amdgcn_readfirstlane(int(bytes))), 0x00020000u};
+}
+__device__ __forceinline__ unsigned lds_offset(const uint8_t* p) {
+    return unsigned(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
 }
 
-// Many rows: a workgroup of WM x WN waves per BM x BN tile.  A stage is 256 of K: BN + BM rows of 128 bytes of codes, loaded into LDS past the
-// registers, 16 bytes a lane; chunk c of row r sits at chunk c ^ (r % 8), so that eight rows' chunks lie in different banks.  Rows and
-// blocks behind the operands' ends are out of the buffers' bounds and come as zeros.  A lane of half h takes block 4 h + s in step s, so that
-// the bytes of its four steps are one word, straight from memory.
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 1) void mx_tile_kernel(const MxArgs a, int tiles_m, int tiles_n) {
-    constexpr int NW = WM * WN, ROWS = BM + BN, STAGE = ROWS * 128, LOADS = ROWS / 8 / NW;
-    constexpr int TI = BN / WN / 32, TJ = BM / WM / 32;   // a wave's blocks of 32 columns n, of 32 rows m
-    static_assert(ROWS % (8 * NW) == 0 && BN % (8 * NW) == 0, "a wave loads whole pieces of one operand");
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, h = lane >> 5;
-    const int wm = wave % WM, wn = wave / WM;
-    const int m0 = int(blockIdx.x) % tiles_m * BM, n0 = int(blockIdx.x) / tiles_m * BN;
-    const int nb = a.K / 32, steps = (nb + 7) / 8;
-    const auto resource = [&](const uint8_t* p, int first, int rows, int most) {
-        const int n = min(rows - first, most);
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p) + size_t(first) * nb * 16, 0, n * nb * 16, 0x00020000);
+// acc += w x in place, step S's bytes of sw and sx.  Written out because the compiler otherwise moves accumulators between registers all
+// through a loop that leaves it none.  What it would add by itself: two states between a vector instruction's write of an operand and
+// this (`settle`), and eighteen between this and a read of acc by anything else (`done`); loads of operands it waits for by itself.
+template <int S>
+__device__ __forceinline__ void multiply(f32x4& acc, u32x4 w, u32x4 x, int sw, int sx) {
+    if constexpr (S == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+}
+__device__ __forceinline__ void settle() { asm volatile("s_nop 1"); }
+__device__ __forceinline__ void done() { asm volatile("s_nop 15\n\ts_nop 3"); }
+
+// Many rows: workgroups of 2 x 2 waves take BM x BN tiles in turn.  A stage is 256 of K: BN + BM rows of 128 bytes of codes, loaded into LDS past
+// the registers, 16 bytes a lane; chunk c (a block of 32) of row r sits at chunk (c % 2 * 4 + c / 2) ^ (r / 2 % 8), so that a fragment's
+// lanes find theirs in different banks.  Rows and blocks behind the operands' ends are out of the buffers' bounds and come as zeros.  In
+// step s of a stage's two, lane group g takes block 2 g + s, so that its bytes lie side by side.  The bytes of four stages come together,
+// 32 a row.
+//
+// Two stages: half way through one, its second step's fragments are in registers and the next stage has arrived (one barrier says both);
+// its place is loaded with the stage after the next, of the next tile too, while the second step multiplies, and the next stage's first
+// fragments are read.  So a tile's results are written while the next one's operands are on their way.
+//
+// Row p of the weights' part of LDS is a column of the tile such that Q fragments' accumulators (four for SwiGLU, else two) are 4 Q
+// consecutive columns of a lane, and the four lane groups' stores 64 bytes of a row.
+template <int BM, int BN, int EPI, bool EVEN>
+__global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int tiles_m, int tiles_n) {
+    constexpr int NW = 4, ROWS = BM + BN, STAGE = ROWS * 128, LOADS = ROWS / 8 / NW, WLOADS = BN / 8 / NW;
+    constexpr int TI = BN / 2 / 16, TJ = BM / 2 / 16;   // a wave's blocks of 16 columns n, of 16 rows m
+    constexpr int SROWS = ROWS * 32, READS = TI + TJ, Q = EPI == 3 ? 4 : 2;
+    constexpr int STORES = TI / Q * TJ;                 // a wave's stores of a whole tile
+    static_assert((BM == 32 || BM % 64 == 0) && BM <= 256 && BN % 128 == 0 && BN <= 256, "a wave loads whole pieces of one operand and holds 64 columns' fragments");
+    static_assert(READS == LOADS && STORES < 64, "as many fragments a step as pieces a stage; a counter of six bits");
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE], s_scale[2 * SROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
+    const int wm = wave % 2, wn = wave / 2;
+    // In a round of all workgroups a run of tiles to each XCD (workgroups are dealt to them in turn), in strips of eight tile rows
+    const int all = tiles_m * tiles_n, grid = int(gridDim.x), b = int(blockIdx.x);
+    const int mine = grid % 8 == 0 ? b % 8 * (grid / 8) + b / 8 : b;
+    const auto tile_m = [&](int o) { const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip); return (8 * strip + (o - strip * 8 * tiles_n) % high) * BM; };
+    const auto tile_n = [&](int o) { const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip); return (o - strip * 8 * tiles_n) / high * BN; };
+    const int nb = a.K / 32, stages = (nb + 7) / 8;
+    // row p of LDS: which row of its operand's part of the tile
+    const auto source = [](int p) { return p < BN ? p / (16 * Q) * (16 * Q) + p % 16 / 4 * (4 * Q) + p / 16 % Q * 4 + p % 4 : p - BN; };
+    // offsets of blocks from nb on get the top bit, which no buffer reaches (K <= 2^23: a tile's rows take up to 2^30 bytes)
+    const auto behind = [&](int c) { return unsigned(nb - 1 - c) & 0x80000000u; };
+    const unsigned codes_at = lds_offset(smem), scales_at = lds_offset(s_scale), row_bytes = unsigned(nb) * 16u;
+    // pieces of eight rows, wave's wave + 4 i; the lane's 16 bytes in a row of each
+    const int r8 = lane / 8, slot = (lane % 8) ^ (4 * (wave & 1) + r8 / 2), chunk = slot % 4 * 2 + slot / 4;
+    const unsigned wlane = unsigned(source(8 * wave + r8)) * row_bytes + 16u * chunk, xlane = unsigned(8 * wave + r8) * row_bytes + 16u * chunk;
+    // of scales waves 0 and 1 bring the weights', 2 and 3 the rows', 32 rows a piece
+    const bool of_w = wave < 2;
+    const int odd = of_w || BM > 32 ? wave & 1 : 0;
+    const int p0 = 32 * odd + lane / 2, half = 16 * (lane % 2 ^ (p0 / 8 & 1)), row0 = of_w ? source(p0) : p0;
+    const unsigned scales_to = (of_w ? 0 : BN * 32) + odd * 1024, slane = unsigned(row0) * unsigned(nb) + half;
+    // what is loaded next: stage l of tile lo, its bytes to place lq % 2
+    int lo = mine, l = 0, lq = 0;
+    Buffer wbuf, xbuf, sbuf;
+    const auto buffers = [&]() __attribute__((always_inline)) {
+        const int m0 = tile_m(lo), n0 = tile_n(lo), first = of_w ? n0 : m0, rows = of_w ? min(a.N - n0, BN) : min(a.M - m0, BM);
+        wbuf = buffer_of(a.w + size_t(n0) * row_bytes, unsigned(min(a.N - n0, BN)) * row_bytes);
+        xbuf = buffer_of(a.x + size_t(m0) * row_bytes, unsigned(min(a.M - m0, BM)) * row_bytes);
+        sbuf = buffer_of((of_w ? a.ws : a.xs) + size_t(first) * nb, unsigned(rows) * unsigned(nb));
     };
-    const auto wbuf = resource(a.w, n0, a.N, BN), xbuf = resource(a.x, m0, a.M, BM);
-    const int r8 = lane / 8, chunk = (lane % 8) ^ r8;
-    const auto load = [&](int step, int to) __attribute__((always_inline)) {
-        const bool there = step * 8 + chunk < nb;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int piece = wave + NW * i, row = piece * 8;   // pieces of the weights first
-            const bool of_w = row < BN;
-            const unsigned at = there ? unsigned((of_w ? row : row - BN) + r8) * unsigned(nb * 16) + unsigned(step * 8 + chunk) * 16u : 0x7FFFFFF0u;
-            uint8_t* lds = smem + to * STAGE + piece * 1024;
-            if (of_w) load_lds16(wbuf, lds, at);
-            else load_lds16(xbuf, lds, at);
-        }
+    const auto load = [&](int place, int i) __attribute__((always_inline)) {   // piece i of LOADS
+        const unsigned to = codes_at + place * STAGE + wave * 1024 + i * 4096;
+        const unsigned k = unsigned(l) * 128u | behind(l * 8 + chunk);
+        // (row 32 i + .. of LDS is row 32 i + .. of the weights for Q = 2, row 64 (i / 2) + 8 (i % 2) + .. for Q = 4)
+        if (i < WLOADS) load_lds16(wbuf, to, wlane + k + unsigned(Q == 2 ? 32 * i : i / 2 * 64 + i % 2 * 8) * row_bytes);
+        else load_lds16(xbuf, to, xlane + k + unsigned(i - WLOADS) * 32u * row_bytes);
     };
-    // The bytes of blocks 8 step + 4 h ..+ 3 of the lane's rows; bytes of blocks behind the end count as 127.
-    const auto bytes = [&](const uint8_t* s, int row, int rows, int step) __attribute__((always_inline)) {
-        const int64_t at = int64_t(min(row, rows - 1)) * nb + 8 * step + 4 * h, last = int64_t(rows) * nb - 4;
-        const int64_t from = min(at, last);   // (the last word of the tensor holds its last bytes)
-        typedef uint32_t u32u __attribute__((aligned(1)));
-        uint32_t v = *reinterpret_cast<const u32u*>(s + from);
-        if (8 * step + 8 > nb) {
-            const int left = nb - 8 * step - 4 * h;
-            v = at - from >= 4 ? 0 : v >> (8 * (at - from));
-            if (left <= 0) v = 0x7F7F7F7Fu;
-            else if (left < 4) v = (v & ((1u << (8 * left)) - 1)) | (0x7F7F7F7Fu << (8 * left));
-        }
-        return int(v);
-    };
-    f32x16 acc[TI][TJ];
+    const auto load_scales = [&]() __attribute__((always_inline)) {   // the bytes of stages l .. l + 3
+        const int c = 4 * l * 2 + half;
 #pragma unroll
-    for (int i = 0; i < TI; ++i)
+        for (int part = 0; part < (BN > BM ? BN : BM) / 64; ++part) {
+            if (part >= (of_w ? BN / 64 : BM == 32 ? 1 : BM / 64)) continue;
+            const unsigned to = (lq & 1) * SROWS + scales_to + part * 2048;
+            if constexpr (EVEN) {
+                load_lds16(sbuf, scales_at + to, (slane + 8u * l + part * 64u * unsigned(nb)) | behind(c));
+            } else {   // rows of bytes at any alignment: through the registers
+                const int rows = of_w ? a.N : a.M, row = min((of_w ? tile_n(lo) : tile_m(lo)) + 64 * part + row0, rows - 1);
+                const uint8_t* s = of_w ? a.ws : a.xs;
+                const int64_t first = int64_t(row) * nb + c, last = int64_t(rows) * nb - 4;
+                u32x4 v;
 #pragma unroll
-        for (int j = 0; j < TJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    load(0, 0);
-    for (int step = 0; step < steps; ++step) {
-        int sw[TI], sx[TJ];
-#pragma unroll
-        for (int i = 0; i < TI; ++i) sw[i] = bytes(a.ws, n0 + (wn * TI + i) * 32 + l32, a.N, step);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) sx[j] = bytes(a.xs, m0 + (wm * TJ + j) * 32 + l32, a.M, step);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();   // this stage has arrived, the other one is free
-        if (step + 1 < steps) load(step + 1, (step + 1) & 1);
-        const uint8_t* st = smem + (step & 1) * STAGE;
-        const auto frag = [&](int row, int s) __attribute__((always_inline)) {
-            return operand(*reinterpret_cast<const u32x4*>(st + row * 128 + (((4 * h + s) ^ (row & 7)) * 16)));
-        };
-        const auto part = [&](auto ss) __attribute__((always_inline)) {
-            constexpr int S = decltype(ss)::value;
-            i32x8 wf[TI], xf[TJ];
-#pragma unroll
-            for (int i = 0; i < TI; ++i) wf[i] = frag((wn * TI + i) * 32 + l32, S);
-#pragma unroll
-            for (int j = 0; j < TJ; ++j) xf[j] = frag(BN + (wm * TJ + j) * 32 + l32, S);
-#pragma unroll
-            for (int i = 0; i < TI; ++i)
-#pragma unroll
-                for (int j = 0; j < TJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], xf[j], acc[i][j], FP4, FP4, S, sw[i], S, sx[j]);
-        };
-        part(std::integral_constant<int, 0>{});
-        part(std::integral_constant<int, 1>{});
-        part(std::integral_constant<int, 2>{});
-        part(std::integral_constant<int, 3>{});
-    }
-#pragma unroll
-    for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                store4(a, m0 + (wm * TJ + j) * 32 + l32, n0 + (wn * TI + i) * 32 + 8 * q + 4 * h, v);
+                for (int u = 0; u < 4; ++u) {   // (the last word of the tensor holds its last bytes)
+                    typedef uint32_t u32u __attribute__((aligned(1)));
+                    const int64_t want = first + 4 * u, from = min(want, last);
+                    const uint32_t w = *reinterpret_cast<const u32u*>(s + from);
+                    v[u] = want - from >= 4 ? 0 : w >> (8 * int(want - from));
+                }
+                *reinterpret_cast<u32x4*>(s_scale + to + 16 * lane) = v;
             }
+        }
+        ++lq;
+    };
+    const auto loaded = [&]() __attribute__((always_inline)) {   // on to the next stage
+        if (++l < stages) return;
+        l = 0;
+        lo += grid;
+        if (lo >= all) lo = all - 1;   // (behind the last tile: some tile, for nobody)
+        buffers();
+    };
+    f32x4 acc[TI][TJ];
+    u32x4 wf[2][TI], xf[2][TJ];   // the fragments of a stage's two steps
+    int sw[TI], sx[TJ], sw_next[TI], sx_next[TJ];   // the bytes of both, and of the next stage's
+    int place = 0, quad = 0;   // where in LDS the present stage and its bytes are
+    const auto read = [&](int from, int r, int s) __attribute__((always_inline)) {   // fragment r of READS of step s
+        const uint8_t* at = smem + from * STAGE + (((4 * s + g) ^ (ln / 2)) * 16) + ln * 128;
+        if (r == 0) wf[s][0] = *reinterpret_cast<const u32x4*>(at + wn * TI * 2048);
+        else if (r <= TJ) xf[s][r - 1] = *reinterpret_cast<const u32x4*>(at + BN * 128 + (wm * TJ + r - 1) * 2048);
+        else wf[s][r - TJ] = *reinterpret_cast<const u32x4*>(at + (wn * TI + r - TJ) * 2048);
+    };
+    const auto read_scale = [&](int stage, int from, int r) __attribute__((always_inline)) {
+        const uint8_t* at = s_scale + from * SROWS + ((stage % 4 * 8 + 2 * g) ^ (ln / 8 * 16)) + ln * 32;
+        if (r < TI) sw_next[r] = *reinterpret_cast<const uint16_t*>(at + (wn * TI + r) * 512);
+        else sx_next[r - TI] = *reinterpret_cast<const uint16_t*>(at + BN * 32 + (wm * TJ + r - TI) * 512);
+    };
+    // The instructions of a step, and before them one after the other the `items` of item(0 ..), done when three quarters of the step are:
+    // a wave issues in order, and loads in a row would hold up the multiplications.
+    const auto step = [&](auto ss, auto items, auto&& item) __attribute__((always_inline)) {
+        constexpr int S = decltype(ss)::value, L = decltype(items)::value, N = TI * TJ, SPREAD = N * 3 / 4;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int i = n * L / SPREAD; i < (n + 1) * L / SPREAD && i < L; ++i) item(i);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply<S>(acc[n / TJ][n % TJ], wf[S][n / TJ], xf[S][n % TJ], sw[n / TJ], sx[n % TJ]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const auto barrier = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    buffers();
+    load_scales();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(0, i);
+    loaded();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    barrier();
+    if (l % 4 == 0) load_scales();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(1, i);
+    loaded();
+#pragma unroll
+    for (int r = 0; r < READS; ++r) read(0, r, 0);
+#pragma unroll
+    for (int r = 0; r < READS; ++r) read_scale(0, 0, r);
+    bool stores = false;   // of a whole tile are on their way
+    for (int o = mine; o < all; o += grid) {
+        const int m0 = tile_m(o), n0 = tile_n(o);
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < stages; ++t) {
+            // bytes of blocks behind the end are another row's: their codes are zeros, a NaN they must not be
+            const int left = nb - 8 * t - 2 * g, keep = left >= 2 ? 0xFFFF : left == 1 ? 0xFF : 0;
+#pragma unroll
+            for (int i = 0; i < TI; ++i) sw[i] = sw_next[i] & keep;
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) sx[j] = sx_next[j] & keep;
+            settle();
+            __builtin_amdgcn_sched_barrier(0);
+            step(std::integral_constant<int, 0>{}, std::integral_constant<int, READS>{},
+                 [&](int i) __attribute__((always_inline)) { read(place, i, 1); });
+            // every wave has read this stage whole, and the next one is there: its loads are older than the last tile's stores
+            if (t == 0 && stores) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(STORES) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            barrier();
+            // the stage after it into this one's place; the next one's first fragments
+            const int next = t + 1 < stages ? t + 1 : 0;
+            if (next % 4 == 0) quad ^= 1;
+            step(std::integral_constant<int, 1>{}, std::integral_constant<int, LOADS + 1 + 2 * READS>{}, [&](int i) __attribute__((always_inline)) {
+                if (i < 2 * LOADS) {
+                    if (i % 2 == 0) load(place, i / 2);
+                    else read(place ^ 1, i / 2, 0);
+                } else if (i == 2 * LOADS) {
+                    if constexpr (EVEN)
+                        if (l % 4 == 0) load_scales();
+                } else {
+                    read_scale(next, quad, i - 2 * LOADS - 1);
+                }
+            });
+            if constexpr (!EVEN)
+                if (l % 4 == 0) load_scales();
+            loaded();
+            place ^= 1;
+        }
+        done();
+        __builtin_amdgcn_sched_barrier(0);
+        if (BM + BN == 512 || n0 + BN <= a.N || a.N % 16 == 0) {   // (the largest tile takes no other N: no registers for it)
+            stores = m0 + BM <= a.M && n0 + BN <= a.N;   // (as many as counted)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                int m = m0 + (wm * TJ + j) * 16 + ln;
+                asm volatile("" : "+v"(m));   // (registers for one row's results at a time)
+#pragma unroll
+                for (int i = 0; i < TI; i += Q) {
+                    float v[4 * Q];
+#pragma unroll
+                    for (int r = 0; r < 4 * Q; ++r) v[r] = acc[i + r / 4][j][r % 4];
+                    const int n = n0 + (wn * TI + i) * 16 + 4 * Q * g;
+                    if (m < a.M && n < a.N) store<EPI>(a, m, n, v);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {   // the last columns of a number that is no multiple of 16: one by one
+            stores = false;
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+#pragma unroll
+                for (int i = 0; i < TI; ++i) store4<EPI>(a, m0 + (wm * TJ + j) * 16 + ln, n0 + source((wn * TI + i) * 16 + 4 * g), acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (what was loaded for nobody: not into the next workgroup's LDS)
 }
 
-template <int BM, int BN, int WM, int WN>
+template <typename F>
+static void by_epilogue(int epi, F&& go) {
+    if (epi == 1) go(std::integral_constant<int, 1>{});
+    else if (epi == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 3>{});
+}
+template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
     const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-    mx_tile_kernel<BM, BN, WM, WN><<<dim3(unsigned(tm) * unsigned(tn)), dim3(64 * WM * WN), 0, st>>>(a, tm, tn);
+    const unsigned tiles = unsigned(tm) * unsigned(tn), most = unsigned(device_cus()) * (BM + BN <= 256 ? 2 : 1);   // (as LDS holds)
+    const dim3 grid(tiles < most ? tiles : most);
+    by_epilogue(a.epi, [&](auto epi) {
+        constexpr int EPI = decltype(epi)::value;
+        if (a.K % 128 == 0) mx_tile_kernel<BM, BN, EPI, true><<<grid, dim3(256), 0, st>>>(a, tm, tn);
+        else mx_tile_kernel<BM, BN, EPI, false><<<grid, dim3(256), 0, st>>>(a, tm, tn);
+    });
 }
 
 }  // namespace scmx
@@ -234,13 +394,17 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     const hipStream_t st = (hipStream_t)stream;
     const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 4;   // (an operand has not four bytes of scales)
     if ((M <= 16 || tiny) && (M + 15) / 16 <= 65535) {
-        mx_rows_kernel<<<dim3((N + 15) / 16, (M + 15) / 16), dim3(64 * RWAVES), 0, st>>>(a);
-    } else if (int64_t(M) * N >= int64_t(256) * 256 * 200) {
-        launch_tile<256, 256, 2, 2>(a, st);
+        by_epilogue(epi, [&](auto e) {
+            mx_rows_kernel<decltype(e)::value><<<dim3((N + 15) / 16, (M + 15) / 16), dim3(64 * RWAVES), 0, st>>>(a);
+        });
+    } else if (int64_t(M) * N >= int64_t(256) * 256 * 200 && N % 16 == 0 && K % 128 == 0) {
+        launch_tile<256, 256>(a, st);
+    } else if (int64_t(M) * N >= int64_t(128) * 256 * 200) {
+        launch_tile<128, 256>(a, st);
     } else if (int64_t(M) * N >= int64_t(128) * 128 * 128) {
-        launch_tile<128, 128, 2, 2>(a, st);
+        launch_tile<128, 128>(a, st);
     } else {
-        launch_tile<64, 64, 2, 2>(a, st);
+        launch_tile<32, 128>(a, st);
     }
     return check_launch("mx_mm");
 }
