@@ -42,37 +42,58 @@ __device__ __forceinline__ uint32_t mx_codes(const float* x, uint32_t byte) {
 // The same of eight bf16 values, packed.
 __device__ __forceinline__ uint32_t mx_codes_bf16(u32x4 x, uint32_t byte) {
     const float s = mx_scale(byte);
+    const uint32_t a = x[0], b = x[1], c = x[2], d = x[3];   // (a bit cast of a vector's element takes the first)
     uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x[0]), s, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x[1]), s, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x[2]), s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x[3]), s, 3);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, a), s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, b), s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, c), s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, d), s, 3);
     return byte == 255 ? 0 : w;
 }
 
-// Eight values in float64 (a norm's, a rotation's) to codes: through a float rounded to odd (cut off, the last bit set if anything was), so
-// that none lands on the border of two codes that was beside it.  Magnitudes are held to 2^-120 .. 2^128 on the way, and the byte to 10
-// and above, below which 2^-120 would count.  Returns the codes; byte: the block's.
+// Values in float64 (a norm's, a rotation's) go through a float rounded to odd (cut off, the last bit set if anything was), so that none lands
+// on the border of two codes that was beside it.  Magnitudes are held to 2^-120 .. 2^128 on the way, and the byte to 10 and above, below
+// which 2^-120 would count.
+__device__ __forceinline__ uint32_t high(double v) { return uint32_t(__builtin_bit_cast(uint64_t, v) >> 32); }
+__device__ __forceinline__ float odd_float(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t hi = uint32_t(b >> 32), lo = uint32_t(b);
+    const uint32_t m = min(max(hi & 0x7FFFFFFFu, uint32_t(1023 - 120) << 20), 0x47EFFFFFu);
+    const uint32_t cut = ((m << 3) | (lo >> 29)) + 0x40000000u;   // the exponent less 896, to float's
+    return __uint_as_float((hi & 0x80000000u) | cut | uint32_t((lo & 0x1FFFFFFFu) != 0));
+}
+// The byte for the largest magnitude's upper word: exponent fields, float64's less 1023, less 2, plus 127; at most 252 (2^125, of which 6 is
+// below 2^128).
+__device__ __forceinline__ uint32_t mx_byte_f64(uint32_t top) {
+    return top >= 0x7FF00000u ? 255 : min(max(top >> 20, 898u + 10u) - 898u, 252u);
+}
+// Eight values of a lane, of a block that four lanes hold, to a word of codes; byte: the block's.
 __device__ __forceinline__ uint32_t mx_codes_f64(const double* v, uint32_t& byte) {
-    uint32_t hi[8], lo[8], top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, v[i]);
-        hi[i] = uint32_t(b >> 32);
-        lo[i] = uint32_t(b);
-        top = max(top, hi[i] & 0x7FFFFFFFu);
-    }
-    top = quad_max(top);
-    // exponent fields: float64's less 1023, less 2, plus 127; at most 252 (2^125, of which 6 is below 2^128)
-    byte = top >= 0x7FF00000u ? 255 : min(max(top >> 20, 898u + 10u) - 898u, 252u);
+    uint32_t top = 0;
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t m = min(max(hi[i] & 0x7FFFFFFFu, uint32_t(1023 - 120) << 20), 0x47EFFFFFu);
-        const uint32_t cut = ((m << 3) | (lo[i] >> 29)) + 0x40000000u;   // the exponent less 896, to float's
-        x[i] = __uint_as_float((hi[i] & 0x80000000u) | cut | uint32_t((lo[i] & 0x1FFFFFFFu) != 0));
+        top = max(top, high(v[i]) & 0x7FFFFFFFu);
+        x[i] = odd_float(v[i]);
     }
+    byte = mx_byte_f64(quad_max(top));
     return mx_codes(x, byte);
+}
+// A whole block of a lane.
+__device__ __forceinline__ u32x4 mx_block_f64(const double* v, uint32_t& byte) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, high(v[i]) & 0x7FFFFFFFu);
+    byte = mx_byte_f64(top);
+    u32x4 c;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = odd_float(v[8 * w + i]);
+        c[w] = mx_codes(x, byte);
+    }
+    return c;
 }
 
 // Byte B of a word of codes as two bf16 values in a word.

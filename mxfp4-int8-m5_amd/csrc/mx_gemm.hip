@@ -24,6 +24,8 @@ struct MxArgs {
 
 __device__ __forceinline__ i32x8 operand(u32x4 c) { return i32x8{int(c[0]), int(c[1]), int(c[2]), int(c[3]), 0, 0, 0, 0}; }
 constexpr int FP4 = 4;   // of the instructions' format operands
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // (the hardware takes vectors at any even address)
+typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 
 __device__ __forceinline__ float silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
@@ -47,7 +49,6 @@ __device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
 // vectors at them).
 template <int EPI>
 __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float* v) {
-    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
     const size_t at = EPI == 3 ? (size_t(m) * a.N + n) / 2 : size_t(m) * a.N + n;
     u32x4 r = {0, 0, 0, 0}, w;
     if constexpr (EPI == 2) r = *reinterpret_cast<const u32x4u*>(a.res + at);
@@ -60,38 +61,111 @@ __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float
     *reinterpret_cast<u32x4u*>(a.out + at) = w;
 }
 
-// Few rows: a workgroup per 16 columns and 16 rows, its waves take the steps of 128 along K in turn, straight from memory.
-constexpr int RWAVES = 4;
-template <int EPI>
-__global__ __launch_bounds__(64 * RWAVES) void mx_rows_kernel(const MxArgs a) {
-    __shared__ f32x4 s_acc[RWAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, g = lane >> 4;
+// Few rows: a workgroup per 16 columns and 16 rows, its waves take the steps of 128 along K in turn, straight from memory, and meet in LDS.  Bound by
+// reading the weights where there are many, by two trips to memory and the launch where there are few.
+// FROM_CODES: the rows are codes.  FROM_ROWS: they are bf16, and a lane makes its operand, a block of 32, of 64 bytes: no lane needs another's
+// values.  FROM_NORM: the rows' sums of squares first, by all waves, then as mx_norm_quantize_kernel, in float64.
+constexpr int FROM_CODES = 0, FROM_ROWS = 1, FROM_NORM = 2;
+constexpr int NORM_ROWS = 16;
+
+struct FewArgs : MxArgs {
+    const uint16_t* rows;
+    int64_t ldx;
+    const uint16_t* nw;
+    float eps;
+};
+
+// The operand and byte of a lane's block of 32 bf16 values.
+__device__ __forceinline__ u32x4 block_codes(const u32x4 (&v)[4], uint32_t& byte) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[i / 4][i % 4] & 0x7FFF7FFFu));
+    byte = mx_byte(uint32_t(max(top[0], top[1])) << 16);
+    u32x4 c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = mx_codes_bf16(v[i], byte);
+    return c;
+}
+
+template <int WAVES, int FROM>
+__global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(const FewArgs a) {
+    __shared__ f32x4 s_acc[WAVES][64];
+    __shared__ double s_sum[FROM == FROM_NORM ? NORM_ROWS : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, nb = a.K / 32;
     const size_t wr = min(n0 + ln, a.N - 1), xr = min(m0 + ln, a.M - 1);
     const u32x4* wp = reinterpret_cast<const u32x4*>(a.w) + wr * nb;
-    const u32x4* xp = reinterpret_cast<const u32x4*>(a.x) + xr * nb;
-    const uint8_t *wsp = a.ws + wr * nb, *xsp = a.xs + xr * nb;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 4 * wave; c0 < nb; c0 += 4 * RWAVES) {
-        const int c = c0 + g;
-        u32x4 wc = {0, 0, 0, 0}, xc = {0, 0, 0, 0};
-        int sw = 127, sx = 127;
-        if (c < nb) {
-            wc = wp[c];
-            xc = xp[c];
-            sw = wsp[c];
-            sx = xsp[c];
+    const uint8_t* wsp = a.ws + wr * nb;
+    const bool live = m0 + ln < a.M;   // (the lanes of rows that are not there load none)
+    double inv = 0;
+    if constexpr (FROM == FROM_NORM) {
+        for (int r = wave; r < min(a.M - m0, 16); r += WAVES) {
+            const u32x4u* p = reinterpret_cast<const u32x4u*>(a.rows + (m0 + r) * a.ldx);
+            double ss = 0;
+            for (int i = lane; i < a.K / 8; i += 64) {
+                const u32x4 v = p[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ss = __builtin_fma(double(bf16_lo(v[e])), double(bf16_lo(v[e])), ss);
+                    ss = __builtin_fma(double(bf16_hi(v[e])), double(bf16_hi(v[e])), ss);
+                }
+            }
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, WAVE);
+            if (lane == 0) s_sum[r] = ss;
         }
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc), operand(xc), acc, FP4, FP4, 0, sw, 0, sx);
+        __syncthreads();
+        inv = 1.0 / sqrt(s_sum[live ? ln : 0] / double(a.K) + double(a.eps));
+    }
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int U = 4;   // steps whose loads are on their way together
+    for (int c0 = 4 * wave; c0 < nb; c0 += 4 * WAVES * U) {
+        u32x4 wc[U], xc[U], raw[U][4], gain[4];
+        uint32_t sw[U], sx[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + 4 * WAVES * u + g;
+            const bool there = c < nb;
+            wc[u] = there ? wp[c] : u32x4{0, 0, 0, 0};
+            sw[u] = there ? wsp[c] : 0;
+            if constexpr (FROM == FROM_CODES) {
+                xc[u] = there && live ? (reinterpret_cast<const u32x4*>(a.x) + xr * nb)[c] : u32x4{0, 0, 0, 0};
+                sx[u] = there && live ? (a.xs + xr * nb)[c] : 0;
+            } else {
+                const u32x4u* p = reinterpret_cast<const u32x4u*>(a.rows + int64_t(xr) * a.ldx + 32 * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[u][i] = there && live ? u32x4(p[i]) : u32x4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if constexpr (FROM == FROM_ROWS) xc[u] = block_codes(raw[u], sx[u]);
+            if constexpr (FROM == FROM_NORM) {
+                const int c = min(c0 + 4 * WAVES * u + g, nb - 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gain[i] = reinterpret_cast<const u32x4u*>(a.nw + 32 * c)[i];
+                double v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const uint32_t x2 = raw[u][i / 8][i / 2 % 4], g2 = gain[i / 8][i / 2 % 4];
+                    v[i] = double(i % 2 ? bf16_hi(x2) : bf16_lo(x2)) * inv * double(i % 2 ? bf16_hi(g2) : bf16_lo(g2));
+                }
+                xc[u] = mx_block_f64(v, sx[u]);
+            }
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc[u]), operand(xc[u]), acc, FP4, FP4, 0, int(sw[u]), 0, int(sx[u]));
+        }
     }
     s_acc[wave][lane] = acc;
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int w = 1; w < RWAVES; ++w)
+    for (int w = 1; w < WAVES; ++w)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += s_acc[w][lane][i];
-    store4<EPI>(a, m0 + ln, n0 + 4 * g, acc);
+    if (a.epi == 1) store4<1>(a, m0 + ln, n0 + 4 * g, acc);
+    else if (a.epi == 2) store4<2>(a, m0 + ln, n0 + 4 * g, acc);
+    else store4<3>(a, m0 + ln, n0 + 4 * g, acc);
 }
 
 // 16 bytes a lane past the registers: to LDS byte `lds` + 16 * lane, zeros where `at` is behind the buffer's end.  Written out because the
@@ -341,6 +415,16 @@ static void by_epilogue(int epi, F&& go) {
     else if (epi == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 3>{});
 }
+// Waves of a workgroup by how many there are: some 2000 keep enough of the weights on their way.
+template <int FROM>
+static void launch_few(const FewArgs& a, hipStream_t st) {
+    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
+    const int64_t groups = int64_t(grid.x) * grid.y;
+    const int steps = (a.K + 127) / 128;
+    if (groups >= 512 || steps < 8) mx_few_kernel<4, FROM><<<grid, dim3(256), 0, st>>>(a);
+    else if (FROM == FROM_NORM || groups >= 256 || steps < 16) mx_few_kernel<8, FROM><<<grid, dim3(512), 0, st>>>(a);
+    else if constexpr (FROM != FROM_NORM) mx_few_kernel<16, FROM><<<grid, dim3(1024), 0, st>>>(a);   // (a norm takes more registers)
+}
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
     const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
@@ -356,6 +440,8 @@ static void launch_tile(const MxArgs& a, hipStream_t st) {
 }  // namespace scmx
 
 using namespace scmx;
+
+constexpr int FEW = 16;   // rows up to which they are few
 
 static int check_mm(const char* who, const void* w, const void* ws, const void* res, const void* out, int epi, int M, int N, int K) {
     if (M < 0 || N < 1 || K < 32 || K % 32 || K > (1 << 23) || epi < 1 || epi > 3 || (epi == 3 && N % 4)) {
@@ -393,24 +479,28 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     const MxArgs a{xcodes, xscales, wcodes, wscales, res, out, epi, M, N, K};
     const hipStream_t st = (hipStream_t)stream;
     const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 4;   // (an operand has not four bytes of scales)
-    if ((M <= 16 || tiny) && (M + 15) / 16 <= 65535) {
-        by_epilogue(epi, [&](auto e) {
-            mx_rows_kernel<decltype(e)::value><<<dim3((N + 15) / 16, (M + 15) / 16), dim3(64 * RWAVES), 0, st>>>(a);
-        });
+    if ((M <= FEW || tiny) && (M + 15) / 16 <= 65535) {
+        FewArgs f{};
+        static_cast<MxArgs&>(f) = a;
+        launch_few<FROM_CODES>(f, st);
     } else if (int64_t(M) * N >= int64_t(256) * 256 * 200 && N % 16 == 0 && K % 128 == 0) {
         launch_tile<256, 256>(a, st);
-    } else if (int64_t(M) * N >= int64_t(128) * 256 * 200) {
-        launch_tile<128, 256>(a, st);
-    } else if (int64_t(M) * N >= int64_t(128) * 128 * 128) {
+    } else if (int64_t(M) * N >= int64_t(128) * 128 * 200) {
         launch_tile<128, 128>(a, st);
+    } else if (int64_t(M) * N >= int64_t(64) * 128 * 200) {
+        launch_tile<64, 128>(a, st);
     } else {
         launch_tile<32, 128>(a, st);
     }
     return check_launch("mx_mm");
 }
 
+// Whether a linear layer's rows are quantised in the product's own kernel: every workgroup of 16 columns does it for itself, which reads the
+// rows N / 16 times.
+static bool in_one(int M, int N, int K) { return M <= FEW && int64_t(M) * K * N <= (int64_t(1) << 28); }
+
 extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K) {
-    if (M < 1 || N < 1 || K < 32 || K % 32) return 0;
+    if (M < 1 || N < 1 || K < 32 || K % 32 || in_one(M, N, K)) return 0;
     return size_t(M) * (K / 2) + size_t(M) * (K / 32);
 }
 
@@ -419,9 +509,26 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
                               void* stream) {
     if (int rc = check_mm("mx_linear", wcodes, wscales, res, out, epi, M, N, K)) return rc;
     const size_t need = scmx_mx_linear_workspace(M, N, K);
-    if (workspace_bytes < need || (need && !workspace) || uintptr_t(workspace) % 16) {
+    if (workspace_bytes < need || (need && (!workspace || uintptr_t(workspace) % 16))) {
         set_error("mx_linear: needs a 16-byte aligned workspace of %zu bytes", need);
         return SCMX_ERR_WORKSPACE;
+    }
+    if (M && (!x || uintptr_t(x) % 2 || uintptr_t(nw) % 2 || (M > 1 && ldx < K) || (nw && K > 16384))) {
+        set_error("mx_linear: need bf16 rows at least K apart, of up to 16384 values with a norm (M=%d K=%d ldx=%lld)", M, K, (long long)ldx);
+        return SCMX_ERR_ARG;
+    }
+    if (M == 0) return SCMX_OK;
+    if (M == 1) ldx = K;
+    if (in_one(M, N, K)) {
+        FewArgs a{};
+        static_cast<MxArgs&>(a) = MxArgs{nullptr, nullptr, wcodes, wscales, res, out, epi, M, N, K};
+        a.rows = x;
+        a.ldx = ldx;
+        a.nw = nw;
+        a.eps = eps;
+        if (nw) launch_few<FROM_NORM>(a, (hipStream_t)stream);
+        else launch_few<FROM_ROWS>(a, (hipStream_t)stream);
+        return check_launch("mx_linear");
     }
     uint8_t *codes = static_cast<uint8_t*>(workspace), *scales = codes + size_t(M) * (K / 2);
     if (int rc = scmx_mx_quantize(x, SCMX_MX_BF16, ldx, nw, eps, codes, scales, M, K, stream)) return rc;
