@@ -37,9 +37,9 @@ int scmx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, i
 int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, const uint16_t* res,
                uint16_t* out, int epi, int M, int N, int K, void* stream);
 
-/* scmx_mx_quantize (bf16, with nw or without) and scmx_mx_mm in one call.  workspace: scmx_mx_linear_workspace(M, N, K) bytes (0: none), 16-byte
+/* scmx_mx_quantize (bf16, with nw or without) and scmx_mx_mm in one call.  workspace: scmx_mx_linear_workspace(M, N, K, nw != NULL) bytes (0: none), 16-byte
  * aligned; it holds the rows' codes and scales between the call's launches. */
-size_t scmx_mx_linear_workspace(int M, int N, int K);
+size_t scmx_mx_linear_workspace(int M, int N, int K, int norm);
 int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw, float eps, const uint8_t* wcodes, const uint8_t* wscales,
                    const uint16_t* res, uint16_t* out, int epi, int M, int N, int K, void* workspace, size_t workspace_bytes,
                    void* stream);

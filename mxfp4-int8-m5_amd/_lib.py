@@ -87,7 +87,7 @@ MX_SIGNATURES = {
     "scmx_mx_quantize": (_I, [_P, _I, _L, _P, _F, _P, _P, _I, _I, _P]),
     "scmx_mx_dequantize": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "scmx_mx_mm": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
-    "scmx_mx_linear_workspace": (_Z, [_I, _I, _I]),
+    "scmx_mx_linear_workspace": (_Z, [_I, _I, _I, _I]),
     "scmx_mx_linear": (_I, [_P, _L, _P, _F, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P]),
     "scmx_cache4_write": (_I, [_P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _L, _I, _P]),
     "scmx_cache4_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),

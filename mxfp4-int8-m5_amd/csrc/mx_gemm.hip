@@ -61,21 +61,18 @@ __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float
     *reinterpret_cast<u32x4u*>(a.out + at) = w;
 }
 
-// Few rows: a workgroup per 16 columns and 16 rows, its waves take the steps of 128 along K in turn, straight from memory, and meet in LDS.  Bound by
-// reading the weights where there are many, by two trips to memory and the launch where there are few.
-// FROM_CODES: the rows are codes.  FROM_ROWS: they are bf16, and a lane makes its operand, a block of 32, of 64 bytes: no lane needs another's
-// values.  FROM_NORM: the rows' sums of squares first, by all waves, then as mx_norm_quantize_kernel, in float64.
-constexpr int FROM_CODES = 0, FROM_ROWS = 1, FROM_NORM = 2;
-constexpr int NORM_ROWS = 16;
+// Few rows: a workgroup per 16 columns and 16 rows.  4096 of K at a time, the rows' codes come to LDS, as they are or made of bf16 rows (a thread
+// takes a block of 32, 64 bytes, and needs no other's values), and the waves take steps of 128 side by side, the weights straight from memory,
+// requested before the rows.  The waves meet in LDS.  Bound by reading the weights where there are many (16384 x 8192), by the launch
+// and a trip to memory where there are few.
+constexpr int FEW_BLOCKS = 128;   // of K at a time
 
 struct FewArgs : MxArgs {
-    const uint16_t* rows;
+    const uint16_t* rows;   // NULL: codes
     int64_t ldx;
-    const uint16_t* nw;
-    float eps;
 };
 
-// The operand and byte of a lane's block of 32 bf16 values.
+// The operand and byte of a block of 32 bf16 values.
 __device__ __forceinline__ u32x4 block_codes(const u32x4 (&v)[4], uint32_t& byte) {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     u16x2 top = {0, 0};
@@ -88,72 +85,51 @@ __device__ __forceinline__ u32x4 block_codes(const u32x4 (&v)[4], uint32_t& byte
     return c;
 }
 
-template <int WAVES, int FROM>
+template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(const FewArgs a) {
+    constexpr int U = FEW_BLOCKS / 4 / WAVES;   // steps of a wave, whose loads are on their way together
     __shared__ f32x4 s_acc[WAVES][64];
-    __shared__ double s_sum[FROM == FROM_NORM ? NORM_ROWS : 1];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, nb = a.K / 32;
-    const size_t wr = min(n0 + ln, a.N - 1), xr = min(m0 + ln, a.M - 1);
+    __shared__ u32x4 s_x[16][FEW_BLOCKS + 1];   // (rows' blocks in different banks)
+    __shared__ uint8_t s_xs[16][FEW_BLOCKS + 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, nb = a.K / 32, high = min(a.M - m0, 16), row = min(ln, high - 1);
+    const size_t wr = min(n0 + ln, a.N - 1);
     const u32x4* wp = reinterpret_cast<const u32x4*>(a.w) + wr * nb;
     const uint8_t* wsp = a.ws + wr * nb;
-    const bool live = m0 + ln < a.M;   // (the lanes of rows that are not there load none)
-    double inv = 0;
-    if constexpr (FROM == FROM_NORM) {
-        for (int r = wave; r < min(a.M - m0, 16); r += WAVES) {
-            const u32x4u* p = reinterpret_cast<const u32x4u*>(a.rows + (m0 + r) * a.ldx);
-            double ss = 0;
-            for (int i = lane; i < a.K / 8; i += 64) {
-                const u32x4 v = p[i];
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b0 = 0; b0 < nb; b0 += FEW_BLOCKS) {
+        const int blocks = min(nb - b0, FEW_BLOCKS), per = ((blocks + 3) / 4 + WAVES - 1) / WAVES, first = wave * per;
+        u32x4 wc[U];
+        uint32_t sw[U];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    ss = __builtin_fma(double(bf16_lo(v[e])), double(bf16_lo(v[e])), ss);
-                    ss = __builtin_fma(double(bf16_hi(v[e])), double(bf16_hi(v[e])), ss);
-                }
+        for (int u = 0; u < U; ++u) {
+            const int c = 4 * (first + u) + g;
+            const bool there = u < per && c < blocks;
+            wc[u] = there ? wp[b0 + c] : u32x4{0, 0, 0, 0};
+            sw[u] = there ? wsp[b0 + c] : 0;
+        }
+        if (b0) __syncthreads();   // (all have read the blocks before)
+        for (int i = tid; i < high * blocks; i += 64 * WAVES) {
+            const int r = unsigned(i) / unsigned(blocks), c = i - r * blocks;
+            if (a.rows) {
+                const u32x4u* p = reinterpret_cast<const u32x4u*>(a.rows + (m0 + r) * a.ldx + 32 * (b0 + c));
+                const u32x4 v[4] = {p[0], p[1], p[2], p[3]};
+                uint32_t byte;
+                s_x[r][c] = block_codes(v, byte);
+                s_xs[r][c] = uint8_t(byte);
+            } else {
+                const size_t at = size_t(m0 + r) * nb + b0 + c;
+                s_x[r][c] = reinterpret_cast<const u32x4*>(a.x)[at];
+                s_xs[r][c] = a.xs[at];
             }
-#pragma unroll
-            for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, WAVE);
-            if (lane == 0) s_sum[r] = ss;
         }
         __syncthreads();
-        inv = 1.0 / sqrt(s_sum[live ? ln : 0] / double(a.K) + double(a.eps));
-    }
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = 4;   // steps whose loads are on their way together
-    for (int c0 = 4 * wave; c0 < nb; c0 += 4 * WAVES * U) {
-        u32x4 wc[U], xc[U], raw[U][4], gain[4];
-        uint32_t sw[U], sx[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = c0 + 4 * WAVES * u + g;
-            const bool there = c < nb;
-            wc[u] = there ? wp[c] : u32x4{0, 0, 0, 0};
-            sw[u] = there ? wsp[c] : 0;
-            if constexpr (FROM == FROM_CODES) {
-                xc[u] = there && live ? (reinterpret_cast<const u32x4*>(a.x) + xr * nb)[c] : u32x4{0, 0, 0, 0};
-                sx[u] = there && live ? (a.xs + xr * nb)[c] : 0;
-            } else {
-                const u32x4u* p = reinterpret_cast<const u32x4u*>(a.rows + int64_t(xr) * a.ldx + 32 * c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[u][i] = there && live ? u32x4(p[i]) : u32x4{0, 0, 0, 0};
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if constexpr (FROM == FROM_ROWS) xc[u] = block_codes(raw[u], sx[u]);
-            if constexpr (FROM == FROM_NORM) {
-                const int c = min(c0 + 4 * WAVES * u + g, nb - 1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) gain[i] = reinterpret_cast<const u32x4u*>(a.nw + 32 * c)[i];
-                double v[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint32_t x2 = raw[u][i / 8][i / 2 % 4], g2 = gain[i / 8][i / 2 % 4];
-                    v[i] = double(i % 2 ? bf16_hi(x2) : bf16_lo(x2)) * inv * double(i % 2 ? bf16_hi(g2) : bf16_lo(g2));
-                }
-                xc[u] = mx_block_f64(v, sx[u]);
-            }
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc[u]), operand(xc[u]), acc, FP4, FP4, 0, int(sw[u]), 0, int(sx[u]));
+            if (u >= per) break;
+            const int c = min(4 * (first + u) + g, blocks - 1);   // (behind the end: a block that meets zeros, its byte with them)
+            const uint32_t sx = 4 * (first + u) + g < blocks ? s_xs[row][c] : 0;
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc[u]), operand(s_x[row][c]), acc, FP4, FP4, 0, int(sw[u]), 0, int(sx));
         }
     }
     s_acc[wave][lane] = acc;
@@ -415,15 +391,15 @@ static void by_epilogue(int epi, F&& go) {
     else if (epi == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 3>{});
 }
-// Waves of a workgroup by how many there are: some 2000 keep enough of the weights on their way.
-template <int FROM>
+template <int WAVES>
+static void few(const FewArgs& a, hipStream_t st) {
+    mx_few_kernel<WAVES><<<dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * WAVES), 0, st>>>(a);
+}
+// Waves of a workgroup: more where there are few of them and K is long.  us with 4 / 8 / 16: one row of 12288 x 2048 6.2 / 5.9 / 6.5, of 2048 x
+// 6144 6.5 / 6.1 / 5.7, of 4096 x 4096 5.0 / 5.1 / 4.9, sixteen of 12288 x 2048 9.1 / 8.9 / 9.2.
 static void launch_few(const FewArgs& a, hipStream_t st) {
-    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
-    const int64_t groups = int64_t(grid.x) * grid.y;
-    const int steps = (a.K + 127) / 128;
-    if (groups >= 512 || steps < 8) mx_few_kernel<4, FROM><<<grid, dim3(256), 0, st>>>(a);
-    else if (FROM == FROM_NORM || groups >= 256 || steps < 16) mx_few_kernel<8, FROM><<<grid, dim3(512), 0, st>>>(a);
-    else if constexpr (FROM != FROM_NORM) mx_few_kernel<16, FROM><<<grid, dim3(1024), 0, st>>>(a);   // (a norm takes more registers)
+    if (int64_t((a.N + 15) / 16) * ((a.M + 15) / 16) < 256 && a.K > 4096) few<16>(a, st);
+    else few<8>(a, st);
 }
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
@@ -464,6 +440,28 @@ static int check_mm(const char* who, const void* w, const void* ws, const void* 
     return SCMX_OK;
 }
 
+// The tile that takes the least time: a stage of 256 of K takes a tile so long by itself, and so long when every CU has one (a CU that holds
+// several takes them in turn or side by side alike), measured in us from 17 to 8192 rows, 512 to 12288 columns, K from 2048 to 8192.  us for 32x128
+// / 64x128 / 128x128 / 256x256, 100 rows of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944
+// 20.6 / 14.3 / 12.8 / 28.4, 3000 of 12288 x 2048 96 / 66 / 55 / 60, 6000 179 / 125 / 98 / 94.
+static int tile_of(int M, int N, int K) {
+    constexpr int BM[4] = {32, 64, 128, 256}, BN[4] = {128, 128, 128, 256};
+    constexpr double ALONE[4] = {0.35, 0.40, 0.51, 1.33}, FULL[4] = {0.33, 0.47, 0.63, 2.1};
+    const int cus = device_cus(), most = N % 16 || K % 128 ? 3 : 4;   // (the largest takes whole groups of columns and words of bytes)
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < most; ++i) {
+        const int64_t tiles = int64_t((M + BM[i] - 1) / BM[i]) * ((N + BN[i] - 1) / BN[i]);
+        const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
+        const double us = ALONE[i] > FULL[i] * load ? ALONE[i] : FULL[i] * load;
+        if (us < least) {
+            least = us;
+            best = i;
+        }
+    }
+    return best;
+}
+
 extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, const uint16_t* res,
                           uint16_t* out, int epi, int M, int N, int K, void* stream) {
     if (int rc = check_mm("mx_mm", wcodes, wscales, res, out, epi, M, N, K)) return rc;
@@ -482,15 +480,14 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     if ((M <= FEW || tiny) && (M + 15) / 16 <= 65535) {
         FewArgs f{};
         static_cast<MxArgs&>(f) = a;
-        launch_few<FROM_CODES>(f, st);
-    } else if (int64_t(M) * N >= int64_t(256) * 256 * 200 && N % 16 == 0 && K % 128 == 0) {
-        launch_tile<256, 256>(a, st);
-    } else if (int64_t(M) * N >= int64_t(128) * 128 * 200) {
-        launch_tile<128, 128>(a, st);
-    } else if (int64_t(M) * N >= int64_t(64) * 128 * 200) {
-        launch_tile<64, 128>(a, st);
+        launch_few(f, st);
     } else {
-        launch_tile<32, 128>(a, st);
+        switch (tile_of(M, N, K)) {
+            case 0: launch_tile<32, 128>(a, st); break;
+            case 1: launch_tile<64, 128>(a, st); break;
+            case 2: launch_tile<128, 128>(a, st); break;
+            default: launch_tile<256, 256>(a, st);
+        }
     }
     return check_launch("mx_mm");
 }
@@ -499,8 +496,8 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
 // rows N / 16 times.
 static bool in_one(int M, int N, int K) { return M <= FEW && int64_t(M) * K * N <= (int64_t(1) << 28); }
 
-extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K) {
-    if (M < 1 || N < 1 || K < 32 || K % 32 || in_one(M, N, K)) return 0;
+extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K, int norm) {
+    if (M < 1 || N < 1 || K < 32 || K % 32 || (!norm && in_one(M, N, K))) return 0;
     return size_t(M) * (K / 2) + size_t(M) * (K / 32);
 }
 
@@ -508,7 +505,7 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
                               const uint16_t* res, uint16_t* out, int epi, int M, int N, int K, void* workspace, size_t workspace_bytes,
                               void* stream) {
     if (int rc = check_mm("mx_linear", wcodes, wscales, res, out, epi, M, N, K)) return rc;
-    const size_t need = scmx_mx_linear_workspace(M, N, K);
+    const size_t need = scmx_mx_linear_workspace(M, N, K, nw != nullptr);
     if (workspace_bytes < need || (need && (!workspace || uintptr_t(workspace) % 16))) {
         set_error("mx_linear: needs a 16-byte aligned workspace of %zu bytes", need);
         return SCMX_ERR_WORKSPACE;
@@ -519,15 +516,12 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
     }
     if (M == 0) return SCMX_OK;
     if (M == 1) ldx = K;
-    if (in_one(M, N, K)) {
+    if (in_one(M, N, K) && !nw) {
         FewArgs a{};
         static_cast<MxArgs&>(a) = MxArgs{nullptr, nullptr, wcodes, wscales, res, out, epi, M, N, K};
         a.rows = x;
         a.ldx = ldx;
-        a.nw = nw;
-        a.eps = eps;
-        if (nw) launch_few<FROM_NORM>(a, (hipStream_t)stream);
-        else launch_few<FROM_ROWS>(a, (hipStream_t)stream);
+        launch_few(a, (hipStream_t)stream);
         return check_launch("mx_linear");
     }
     uint8_t *codes = static_cast<uint8_t*>(workspace), *scales = codes + size_t(M) * (K / 2);

@@ -614,7 +614,7 @@ PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         {
             const NoGil released;
             out = fresh(x, at::ScalarType::BFloat16, {M, epi == 3 ? N / 2 : N});
-            const size_t need = scmx_mx_linear_workspace(int(M), int(N), int(K));
+            const size_t need = scmx_mx_linear_workspace(int(M), int(N), int(K), nw != nullptr);
             const c10::DataPtr work = scratch(need);
             rc = scmx_mx_linear(static_cast<const uint16_t*>(x.data_ptr()), ld, nw, eps, bytes(*codes), bytes(*scales),
                                 res ? static_cast<const uint16_t*>(res->data_ptr()) : nullptr, static_cast<uint16_t*>(out.data_ptr()), int(epi),

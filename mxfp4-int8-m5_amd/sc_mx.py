@@ -87,7 +87,7 @@ def linear(x, wcodes, wscales, epi=1, res=None, nw=None, eps=0.0):
     _on_device(x, nw, wcodes, wscales, res)
     x, (M, K) = _rows(x), x.shape
     N, out = _check_product(M, K, wcodes, wscales, epi, res, x)
-    need = _lib.native().scmx_mx_linear_workspace(M, N, K)
+    need = _lib.native().scmx_mx_linear_workspace(M, N, K, int(nw is not None))
     _lib.native().scmx_mx_linear(x.data_ptr(), _ldx(x), nw, S._eps(eps) if nw is not None else 0.0, wcodes, wscales, res, out, epi, M, N, K,
                                  _lib.native().empty_u8(x, need) if need else None, need)
     return out
