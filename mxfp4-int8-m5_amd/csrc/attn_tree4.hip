@@ -155,18 +155,27 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
     int qs[RT][QN];
     uint64_t seen[RT];
     const int start = first + wave < last ? first + wave : last - 1;   // (a wave without a tile loads one and uses none)
+    constexpr int PARTS = D / 64;   // pieces of 64 dimensions, 16 a lane
+    u32x4 qraw[RT][PARTS][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int r = min(row0 + 16 * rt + ln, rows_all - 1), i = token(r);
         seen[rt] = (a.mask ? uint64_t(a.mask[i]) : ~0ull >> (63 - i)) & ~0ull >> (64 - a.T);
         const uint16_t* qp = a.q + out_row(r) * D + 16 * g;
-        constexpr int PARTS = D / 64;   // pieces of 64 dimensions, 16 a lane
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) qraw[rt][p][h] = *reinterpret_cast<const u32x4*>(qp + 64 * p + 8 * h);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(start);
+    load_v(start);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
         uint32_t hi[PARTS][4], lo[PARTS][4], byte[PARTS];
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            const u32x4 raw[2] = {*reinterpret_cast<const u32x4*>(qp + 64 * p), *reinterpret_cast<const u32x4*>(qp + 64 * p + 8)};
-            byte[p] = split_e4m3(raw, hi[p], lo[p]);
-        }
+        for (int p = 0; p < PARTS; ++p) byte[p] = split_e4m3(qraw[rt][p], hi[p], lo[p]);
         // a piece has two blocks, whose bytes lie in lane groups 0, 1 and 2, 3; group g needs that of block g
         const int from = 32 * (g % 2) + ln;
         if constexpr (D == 64) {
@@ -194,8 +203,6 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             }
         }
     }
-    load_k(start);
-    load_v(start);
     f32x4 o[RT][DPL], ones[RT];   // ones: sums of the rounded weights
     float m[RT];
 #pragma unroll
@@ -416,8 +423,12 @@ extern "C" int scmx_attn_tree4_splits(int T, int n, int hq, int hk, int d) {
     if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
     const int qrows = T * (hq / hk), rt = tree4_blocks(qrows, d), tiles = tiles_of(n);
     if (tiles <= TONE) return 1;
-    // a workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, whose join reads half as much
-    const int64_t most = 256 / (int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)));
+    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, whose join reads half as much.  Two workgroups a
+    // CU where a wave has eight tiles and more: one token of 16:8 x 128, 16 / 32 / 64 ranges, 3000 rows 7.6 / 8.0 / -, 10000 9.8 / 9.0 / 9.1, 40000
+    // 25.3 / 16.9 / 14.3 us; 64 tokens of 32:8 x 128, 6000 rows, 4 / 8 / 16 ranges 18.7 / 18.2 / 28.8.  Eight waves a workgroup: 40000 rows 14.4 with
+    // 32 ranges, 15.2 with 64, 16 tokens of 3000 rows 12.1 (four 10.8), one range of 300 rows 5.9 (6.1), of 500 6.9 (6.6).
+    const int64_t groups = int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)), one = 256 / groups;
+    const int64_t most = tiles >= 8 * TWAVES * one ? 512 / groups : one;
     const int even = (tiles + TWAVES - 1) / TWAVES, ranges = even > 16 && even <= 32 ? 16 : even < 64 ? even : 64;
     return most < 1 ? 1 : ranges < most ? ranges : int(most);
 }
