@@ -79,23 +79,6 @@ __device__ __forceinline__ uint32_t mx_codes_f64(const double* v, uint32_t& byte
     byte = mx_byte_f64(quad_max(top));
     return mx_codes(x, byte);
 }
-// A whole block of a lane.
-__device__ __forceinline__ u32x4 mx_block_f64(const double* v, uint32_t& byte) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, high(v[i]) & 0x7FFFFFFFu);
-    byte = mx_byte_f64(top);
-    u32x4 c;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = odd_float(v[8 * w + i]);
-        c[w] = mx_codes(x, byte);
-    }
-    return c;
-}
-
 // Byte B of a word of codes as two bf16 values in a word.
 template <int B>
 __device__ __forceinline__ uint32_t mx_bf16x2(uint32_t w, float scale) {

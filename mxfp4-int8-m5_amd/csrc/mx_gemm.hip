@@ -25,7 +25,6 @@ struct MxArgs {
 __device__ __forceinline__ i32x8 operand(u32x4 c) { return i32x8{int(c[0]), int(c[1]), int(c[2]), int(c[3]), 0, 0, 0, 0}; }
 constexpr int FP4 = 4;   // of the instructions' format operands
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // (the hardware takes vectors at any even address)
-typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
 
 __device__ __forceinline__ float silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
@@ -92,7 +91,9 @@ __global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(const FewArgs a) {
     __shared__ u32x4 s_x[16][FEW_BLOCKS + 1];   // (rows' blocks in different banks)
     __shared__ uint8_t s_xs[16][FEW_BLOCKS + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16, nb = a.K / 32, high = min(a.M - m0, 16), row = min(ln, high - 1);
+    const unsigned down = (blockIdx.z * gridDim.y + blockIdx.y) * 16;
+    if (down >= unsigned(a.M)) return;
+    const int n0 = blockIdx.x * 16, m0 = int(down), nb = a.K / 32, high = min(a.M - m0, 16), row = min(ln, high - 1);
     const size_t wr = min(n0 + ln, a.N - 1);
     const u32x4* wp = reinterpret_cast<const u32x4*>(a.w) + wr * nb;
     const uint8_t* wsp = a.ws + wr * nb;
@@ -393,23 +394,24 @@ static void by_epilogue(int epi, F&& go) {
 }
 template <int WAVES>
 static void few(const FewArgs& a, hipStream_t st) {
-    mx_few_kernel<WAVES><<<dim3((a.N + 15) / 16, (a.M + 15) / 16), dim3(64 * WAVES), 0, st>>>(a);
+    const unsigned down = (unsigned(a.M) + 15) / 16, z = (down + 65534) / 65535;
+    mx_few_kernel<WAVES><<<dim3((unsigned(a.N) + 15) / 16, (down + z - 1) / z, z), dim3(64 * WAVES), 0, st>>>(a);
 }
 // Waves of a workgroup: more where there are few of them and K is long.  us with 4 / 8 / 16: one row of 12288 x 2048 6.2 / 5.9 / 6.5, of 2048 x
 // 6144 6.5 / 6.1 / 5.7, of 4096 x 4096 5.0 / 5.1 / 4.9, sixteen of 12288 x 2048 9.1 / 8.9 / 9.2.
 static void launch_few(const FewArgs& a, hipStream_t st) {
-    if (int64_t((a.N + 15) / 16) * ((a.M + 15) / 16) < 256 && a.K > 4096) few<16>(a, st);
+    if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) < 256 && a.K > 4096) few<16>(a, st);
     else few<8>(a, st);
 }
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
-    const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+    const int tm = int((unsigned(a.M) + BM - 1) / BM), tn = int((unsigned(a.N) + BN - 1) / BN);
     const unsigned tiles = unsigned(tm) * unsigned(tn), most = unsigned(device_cus()) * (BM + BN <= 256 ? 2 : 1);   // (as LDS holds)
     const dim3 grid(tiles < most ? tiles : most);
     by_epilogue(a.epi, [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
-        if (a.K % 128 == 0) mx_tile_kernel<BM, BN, EPI, true><<<grid, dim3(256), 0, st>>>(a, tm, tn);
-        else mx_tile_kernel<BM, BN, EPI, false><<<grid, dim3(256), 0, st>>>(a, tm, tn);
+        if (BM + BN == 512 || a.K % 128 == 0) mx_tile_kernel<BM, BN, EPI, true><<<grid, dim3(256), 0, st>>>(a, tm, tn);
+        else if constexpr (BM + BN < 512) mx_tile_kernel<BM, BN, EPI, false><<<grid, dim3(256), 0, st>>>(a, tm, tn);
     });
 }
 
@@ -451,7 +453,7 @@ static int tile_of(int M, int N, int K) {
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < most; ++i) {
-        const int64_t tiles = int64_t((M + BM[i] - 1) / BM[i]) * ((N + BN[i] - 1) / BN[i]);
+        const int64_t tiles = (int64_t(M) + BM[i] - 1) / BM[i] * ((int64_t(N) + BN[i] - 1) / BN[i]);
         const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
         const double us = ALONE[i] > FULL[i] * load ? ALONE[i] : FULL[i] * load;
         if (us < least) {
@@ -477,7 +479,7 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     const MxArgs a{xcodes, xscales, wcodes, wscales, res, out, epi, M, N, K};
     const hipStream_t st = (hipStream_t)stream;
     const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 4;   // (an operand has not four bytes of scales)
-    if ((M <= FEW || tiny) && (M + 15) / 16 <= 65535) {
+    if (M <= FEW || tiny) {
         FewArgs f{};
         static_cast<MxArgs&>(f) = a;
         launch_few(f, st);
@@ -510,7 +512,7 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
         set_error("mx_linear: needs a 16-byte aligned workspace of %zu bytes", need);
         return SCMX_ERR_WORKSPACE;
     }
-    if (M && (!x || uintptr_t(x) % 2 || uintptr_t(nw) % 2 || (M > 1 && ldx < K) || (nw && K > 16384))) {
+    if (M && (!x || uintptr_t(x) % 2 || uintptr_t(nw) % 2 || (M > 1 && (ldx < K || ldx > INT64_MAX / 8 / M)) || (nw && K > 16384))) {
         set_error("mx_linear: need bf16 rows at least K apart, of up to 16384 values with a norm (M=%d K=%d ldx=%lld)", M, K, (long long)ldx);
         return SCMX_ERR_ARG;
     }

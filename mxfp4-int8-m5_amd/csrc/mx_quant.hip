@@ -41,6 +41,14 @@ __device__ __forceinline__ void floats(const Raw8<TYPE>& r, float* x) {
     }
 }
 
+// The bits of the largest magnitude of eight bf16 values (a NaN above all others).
+__device__ __forceinline__ uint32_t max_bf16(const Raw8<SCMX_MX_BF16>& r) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, max(r.w[0][i] & 0x7FFFu, r.w[0][i] >> 16 & 0x7FFFu));
+    return top;
+}
+
 // A wave per 2048 values of a row.
 template <int TYPE, bool ALIGNED>
 __global__ __launch_bounds__(QNT) void mx_quantize_kernel(const void* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
@@ -69,8 +77,11 @@ __global__ __launch_bounds__(QNT) void mx_quantize_kernel(const void* __restrict
     }
 }
 
-// RMSNorm first: WPR waves a row, NC pieces of 8 values a lane.  Sums and products in float64 (they cost as much as float32's here):
-// a product rounded to float32 lands on the other side of a border between codes once in a million values, a third of the block's largest value off.
+// RMSNorm first: WPR waves a row, NC pieces of 8 values a lane.  The codes are those of the float64 values: a product rounded to float32 lands on the
+// other side of a border between codes once in a million values, a third of the block's largest value off.  Sums are in float64; the values are
+// taken in float32, within 3 * 2^-24 of float64's, and if 1 - 2^-21 and 1 + 2^-21 times each of them take the same codes and byte, so does what lies
+// between.  If not, once in some thousand pieces, or where magnitudes could leave float32's range, the wave takes its piece in float64: all in float64
+// is bound by its instructions (8192 rows of 2048 16.8 us).
 template <int NC, int WPR, bool ALIGNED>
 __global__ __launch_bounds__(QNT) void mx_norm_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ nw,
                                                                float eps, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int M,
@@ -103,17 +114,34 @@ __global__ __launch_bounds__(QNT) void mx_norm_quantize_kernel(const uint16_t* _
         for (int w = 0; w < WPR; ++w) ss += s_sum[w];
     }
     const double inv = 1.0 / sqrt(ss / double(K) + double(eps));
+    const float inv32 = float(inv);
+    const bool plain = inv32 > 0x1p-120f && inv32 < 0x1p120f;   // (not for an infinity or a NaN in the row)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int k = (c * 64 * WPR + t) * 8;
-        float f[8], g[8];
+        float f[8], g[8], v[8], below[8], above[8], top = 0.0f;
+        const Raw8<SCMX_MX_BF16> gain = load8<SCMX_MX_BF16, ALIGNED>(nw, min(k, K - 8));
         floats<SCMX_MX_BF16>(r[c], f);
-        floats<SCMX_MX_BF16>(load8<SCMX_MX_BF16, ALIGNED>(nw, min(k, K - 8)), g);
-        double v[8];
+        floats<SCMX_MX_BF16>(gain, g);
+        constexpr float BELOW = 1.0f - 0x1p-21f, ABOVE = 1.0f + 0x1p-21f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = double(f[i]) * inv * double(g[i]);
-        uint32_t byte;
-        const uint32_t w = mx_codes_f64(v, byte);
+        for (int i = 0; i < 8; ++i) {
+            v[i] = f[i] * inv32 * g[i];
+            top = fmaxf(top, fabsf(v[i]));
+            below[i] = v[i] * BELOW;
+            above[i] = v[i] * ABOVE;
+        }
+        top = __uint_as_float(quad_max(__float_as_uint(top)));
+        uint32_t byte = mx_byte(__float_as_uint(top * ABOVE)), w = mx_codes(above, byte);
+        // gains up to 2^60 and blocks from 2^-58 on: a product with the inverse that float32 cannot hold is a zero there
+        const bool sure = plain && max_bf16(gain) <= 0x5D80u && byte >= 67 && byte <= 252 && byte == mx_byte(__float_as_uint(top * BELOW)) &&
+                          w == mx_codes(below, byte);
+        if (__any(!sure)) {
+            double d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = double(f[i]) * inv * double(g[i]);
+            w = mx_codes_f64(d, byte);
+        }
         if (k < K) {
             *reinterpret_cast<uint32_t*>(codes + size_t(row) * (K / 2) + k / 2) = w;
             if (lane % 4 == 0) scales[size_t(row) * (K / 32) + k / 32] = uint8_t(byte);
@@ -144,7 +172,7 @@ template <int NC, bool ALIGNED>
 static void launch_norm(const void* x, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M, int K, int wpr,
                         hipStream_t st) {
     const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<dim3((M + 3) / 4), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
+    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<dim3((unsigned(M) + 3) / 4), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
     else mx_norm_quantize_kernel<NC, 4, ALIGNED><<<dim3(M), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
 }
 

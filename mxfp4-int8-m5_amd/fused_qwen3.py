@@ -13,7 +13,7 @@ epilogue="row":  INT32 GEMM out, then the row kernels res_norm_quant / swiglu_qu
 The decode step's fixed-shape halves can be captured in HIP graphs (graphs=True), which is what mx.compile does for
 the reference (e2e/decode.py:30-33): one graph launch replaces about ten kernel launches per layer.
 
-Beyond the reference: caches in 8 bits (make_cache(bits=8)) in every path, and DraftQwen3, a decode step that decides several
+Beyond the reference: caches in 8 bits (make_cache(bits=8)) and in MXFP4 (bits="mxfp4") in every path, and DraftQwen3, a decode step that decides several
 tokens at once, a tree of drafted ones verified against the model's own probabilities."""
 import json
 import operator
@@ -123,17 +123,19 @@ class FusedQwen3:
         return sum(w.nbytes() for _, ws in self.layers for w in ws.values())
 
     def make_cache(self, max_len=4096, bits=16):
-        """A cache a block, in bf16 or (bits=8) in 8 bits with a scale a row: half the bytes to keep and to read."""
-        if bits not in (8, 16):
-            raise ValueError("a cache has 16 or 8 bits")
-        return [(KVCache if bits == 16 else C.Q8Cache)(self.args, max_len, self.device) for _ in self.layers]
+        """A cache a block, in bf16, (bits=8) in 8 bits with a scale a row, half the bytes to keep and to read, or (bits="mxfp4") in
+        4-bit values with a scale every 32, little more than a quarter.  (The 4-bit values are named by their format: a plain 4 is none.)"""
+        if bits not in (16, 8, "mxfp4"):
+            raise ValueError('a cache has 16 or 8 bits, or is in "mxfp4"')
+        kind = KVCache if bits == 16 else C.Q8Cache if bits == 8 else C.Q4Cache
+        return [kind(self.args, max_len, self.device) for _ in self.layers]
 
     # ---- pieces shared by prefill and decode --------------------------------------------------------------------
     def _qkv(self, c, L, nw, y=None, acc=None, xs=None, ws=None, pos=None):
         """Per-head RMSNorm of q and k, rotary embedding at positions pos..pos+L-1 (pos defaults to the cache offset;
         an int64 device tensor for graph replay) and the KV-cache append, in one kernel: returns q [hq, L, d]."""
         a = self.args
-        if isinstance(c, C.Q8Cache):
+        if isinstance(c, C.FEW_BITS):
             return C.cache_write(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], self.eps, L, a.num_attention_heads,
                                  a.num_key_value_heads, a.head_dim, c.k, c.v, c.offset if pos is None else pos, self.inv_freq, c.kscale,
                                  c.vscale, acc=acc, xscale=xs, wscale=ws)
@@ -147,8 +149,8 @@ class FusedQwen3:
         if off + L > c.k.shape[1]:
             raise ValueError("KV cache is full")
         c.offset = off + L
-        if isinstance(c, C.Q8Cache):
-            if L <= C.MAX_NODES:   # few tokens read the 8-bit rows as they are
+        if isinstance(c, C.FEW_BITS):
+            if L <= C.MAX_NODES:   # few tokens read the rows as they are
                 return C.attn_tree(q, c.k, c.v, off, None, c.kscale, c.vscale)
             k, v = C.cache_read(c.k, c.v, c.kscale, c.vscale, off + L)
         elif L == 1:
@@ -288,7 +290,7 @@ class DecodeQwen3:
             y = G.gemv(xq, w.codes, w.bcodes, xs, w.wscale, w.N, 1, fmt=f.fmt)
         if self.fuse_attn:   # the attention output, not q: the token's k and v are in the cache afterwards
             a = self.args
-            if isinstance(c, C.Q8Cache):
+            if isinstance(c, C.FEW_BITS):
                 return C.attn_tree(f._qkv(c, 1, nw, y=y[None], pos=pos), c.k, c.v, pos, None, c.kscale, c.vscale)
             return S.attn_decode_qkv(y, nw["self_attn.q_norm"], nw["self_attn.k_norm"], f.eps, a.num_attention_heads,
                                      a.num_key_value_heads, a.head_dim, c.k, c.v, pos, f.inv_freq)
@@ -388,8 +390,8 @@ class DecodeQwen3:
             c = cache[i]
             q = self._pre(h, nw, ws["qkv"], c, self.pos)
             if not self.fuse_attn:
-                eight = isinstance(c, C.Q8Cache)
-                q = C.attn_tree(q, c.k, c.v, self.pos, None, c.kscale, c.vscale) if eight else S.attn_decode(q, c.k, c.v, self.pos)
+                few = isinstance(c, C.FEW_BITS)
+                q = C.attn_tree(q, c.k, c.v, self.pos, None, c.kscale, c.vscale) if few else S.attn_decode(q, c.k, c.v, self.pos)
             h = self._post(q, h, nw, ws)
         return self._logits(h)
 

@@ -33,9 +33,13 @@ class Q4Cache:
 
     def __init__(self, args, max_len, device="cuda"):
         hk, d = args.num_key_value_heads, args.head_dim
+        _check(d in (64, 128, 256), "a 4-bit cache has heads of 64, 128 or 256")
         zeros = lambda n: torch.zeros((hk, max_len, n), dtype=torch.uint8, device=device)   # noqa: E731
         self.k, self.v, self.kscale, self.vscale = zeros(d // 2), zeros(d // 2), zeros(d // 32), zeros(d // 32)
         self.offset = 0
+
+
+FEW_BITS = Q8Cache, Q4Cache
 
 
 def tensors(cache):
