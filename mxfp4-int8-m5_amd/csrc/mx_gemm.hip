@@ -442,20 +442,23 @@ static int check_mm(const char* who, const void* w, const void* ws, const void* 
     return SCMX_OK;
 }
 
-// The tile that takes the least time: a stage of 256 of K takes a tile so long by itself, and so long when every CU has one (a CU that holds
-// several takes them in turn or side by side alike), measured in us from 17 to 8192 rows, 512 to 12288 columns, K from 2048 to 8192.  us for 32x128
-// / 64x128 / 128x128 / 256x256, 100 rows of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944
-// 20.6 / 14.3 / 12.8 / 28.4, 3000 of 12288 x 2048 96 / 66 / 55 / 60, 6000 179 / 125 / 98 / 94.
+// The tile that takes the least time, in us: alone on a CU a stage of 256 of K and a tile's beginning and end take so long, and so long for each
+// tile when every CU has some (a CU that holds several takes them in turn or side by side alike); measured from 17 to 8192 rows, 512 to 16384
+// columns, K from 256 to 8192, where the choice is half a per cent off the best on average.  us for 32x128 / 64x128 / 128x128 / 256x256: 100 rows
+// of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944 20.6 / 14.3 / 12.8 / 28.4, 6000 of 12288 x
+// 2048 180 / 124 / 92 / 89, of 2048 x 8192 114 / 70 / 74 / 56, 4000 of 16384 x 512 58 / 44 / 35 / 46.
 static int tile_of(int M, int N, int K) {
     constexpr int BM[4] = {32, 64, 128, 256}, BN[4] = {128, 128, 128, 256};
-    constexpr double ALONE[4] = {0.35, 0.40, 0.51, 1.33}, FULL[4] = {0.33, 0.47, 0.63, 2.1};
+    constexpr double ALONE[4] = {0.34, 0.35, 0.49, 1.1}, ALONE_ENDS[4] = {1.1, 1.4, 1.8, 5.2};
+    constexpr double FULL[4] = {0.25, 0.34, 0.5, 1.4}, FULL_ENDS[4] = {0.45, 0.82, 1.2, 7.5};
     const int cus = device_cus(), most = N % 16 || K % 128 ? 3 : 4;   // (the largest takes whole groups of columns and words of bytes)
+    const double stages = (K + 255) / 256;
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < most; ++i) {
         const int64_t tiles = (int64_t(M) + BM[i] - 1) / BM[i] * ((int64_t(N) + BN[i] - 1) / BN[i]);
         const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
-        const double us = ALONE[i] > FULL[i] * load ? ALONE[i] : FULL[i] * load;
+        const double alone = ALONE[i] * stages + ALONE_ENDS[i], full = (FULL[i] * stages + FULL_ENDS[i]) * load, us = alone > full ? alone : full;
         if (us < least) {
             least = us;
             best = i;
