@@ -30,15 +30,15 @@ __device__ __forceinline__ uint32_t mx_byte(uint32_t top) {
 }
 
 // Eight float values of a lane to a word of codes, for the byte of their block.
-__device__ __forceinline__ uint32_t mx_codes(const float* x, uint32_t byte) {
+__device__ __forceinline__ uint32_t mx_codes_finite(const float* x, uint32_t byte) {
     const float s = mx_scale(byte);
     uint32_t w = 0;
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-    return byte == 255 ? 0 : w;
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
 }
+__device__ __forceinline__ uint32_t mx_codes(const float* x, uint32_t byte) { return byte == 255 ? 0 : mx_codes_finite(x, byte); }
 // The same of eight bf16 values, packed.
 __device__ __forceinline__ uint32_t mx_codes_bf16(u32x4 x, uint32_t byte) {
     const float s = mx_scale(byte);

@@ -41,14 +41,6 @@ __device__ __forceinline__ void floats(const Raw8<TYPE>& r, float* x) {
     }
 }
 
-// The bits of the largest magnitude of eight bf16 values (a NaN above all others).
-__device__ __forceinline__ uint32_t max_bf16(const Raw8<SCMX_MX_BF16>& r) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(r.w[0][i] & 0x7FFFu, r.w[0][i] >> 16 & 0x7FFFu));
-    return top;
-}
-
 // A wave per 2048 values of a row.
 template <int TYPE, bool ALIGNED>
 __global__ __launch_bounds__(QNT) void mx_quantize_kernel(const void* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
@@ -77,13 +69,30 @@ __global__ __launch_bounds__(QNT) void mx_quantize_kernel(const void* __restrict
     }
 }
 
+// A sum over a wave's lanes, in each of them: row operations within sixteen lanes, then the four rows.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return v + __builtin_bit_cast(double, uint64_t(dpp<CTRL>(uint32_t(b >> 32))) << 32 | dpp<CTRL>(uint32_t(b)));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = dpp_add<ROW_MIRROR>(dpp_add<HALF_MIRROR>(dpp_add<QUAD_SWAP2>(dpp_add<QUAD_SWAP1>(v))));
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    double sum = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        sum += __builtin_bit_cast(double, uint64_t(uint32_t(__builtin_amdgcn_readlane(int(b >> 32), 16 * r))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(b), 16 * r)));
+    return sum;
+}
+
 // RMSNorm first: WPR waves a row, NC pieces of 8 values a lane.  The codes are those of the float64 values: a product rounded to float32 lands on the
-// other side of a border between codes once in a million values, a third of the block's largest value off.  Sums are in float64; the values are
-// taken in float32, within 3 * 2^-24 of float64's, and if 1 - 2^-21 and 1 + 2^-21 times each of them take the same codes and byte, so does what lies
-// between.  If not, once in some thousand pieces, or where magnitudes could leave float32's range, the wave takes its piece in float64: all in float64
-// is bound by its instructions (8192 rows of 2048 16.8 us).
+// other side of a border between codes once in a million values, a third of the block's largest value off.  The sum of squares is in float64.  A
+// value times its gain is exact in float32; times the inverse less and more 2^-21 of it, which is rounded to within 3 * 2^-24, float64's result
+// lies between the two, and if both take the same code and byte, so does it.  If not, once in some thousand pieces, or where a product leaves
+// float32's range, the wave takes its piece in float64.  8192 rows of 2048 take 11.4 us, 32768 33.5 (without the norm 6.5, 25.0: memory); all in float64 16.8, its
+// instructions.
 template <int NC, int WPR, bool ALIGNED>
-__global__ __launch_bounds__(QNT) void mx_norm_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ nw,
+__global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ nw,
                                                                float eps, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int M,
                                                                int K) {
     __shared__ double s_sum[QNT / 64];
@@ -104,38 +113,38 @@ __global__ __launch_bounds__(QNT) void mx_norm_quantize_kernel(const uint16_t* _
         for (int i = 0; i < 8; ++i) part = __builtin_fma(double(f[i]), double(f[i]), part);
         if ((c * 64 * WPR + t) * 8 < K) ss += part;
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, WAVE);
+    ss = wave_sum(ss);
     if constexpr (WPR > 1) {
         if (lane == 0) s_sum[wave] = ss;
         __syncthreads();
         ss = 0;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) ss += s_sum[w];
+        for (int w = 0; w < WPR; ++w) ss += s_sum[wave / WPR * WPR + w];
     }
     const double inv = 1.0 / sqrt(ss / double(K) + double(eps));
-    const float inv32 = float(inv);
-    const bool plain = inv32 > 0x1p-120f && inv32 < 0x1p120f;   // (not for an infinity or a NaN in the row)
+    const float inv32 = float(inv), less = inv32 * (1.0f - 0x1p-21f), more = inv32 * (1.0f + 0x1p-21f);
+    // (not for an infinity or a NaN in the row; a product with a gain that float32 cannot hold, below 2^-126, is then a zero of blocks from 2^-58 on)
+    const bool plain = inv32 > 0x1p-120f && inv32 < 0x1p60f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int k = (c * 64 * WPR + t) * 8;
-        float f[8], g[8], v[8], below[8], above[8], top = 0.0f;
-        const Raw8<SCMX_MX_BF16> gain = load8<SCMX_MX_BF16, ALIGNED>(nw, min(k, K - 8));
+        float f[8], g[8], below[8], above[8];
         floats<SCMX_MX_BF16>(r[c], f);
-        floats<SCMX_MX_BF16>(gain, g);
-        constexpr float BELOW = 1.0f - 0x1p-21f, ABOVE = 1.0f + 0x1p-21f;
+        floats<SCMX_MX_BF16>(load8<SCMX_MX_BF16, ALIGNED>(nw, min(k, K - 8)), g);
+        int32_t plus = INT32_MIN;
+        uint32_t minus = 0;   // as bits the largest of either sign, a NaN above all others
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[i] = f[i] * inv32 * g[i];
-            top = fmaxf(top, fabsf(v[i]));
-            below[i] = v[i] * BELOW;
-            above[i] = v[i] * ABOVE;
+            const float v = f[i] * g[i];
+            plus = max(plus, int32_t(__float_as_uint(v)));
+            minus = max(minus, __float_as_uint(v));
+            below[i] = v * less;
+            above[i] = v * more;
         }
-        top = __uint_as_float(quad_max(__float_as_uint(top)));
-        uint32_t byte = mx_byte(__float_as_uint(top * ABOVE)), w = mx_codes(above, byte);
-        // gains up to 2^60 and blocks from 2^-58 on: a product with the inverse that float32 cannot hold is a zero there
-        const bool sure = plain && max_bf16(gain) <= 0x5D80u && byte >= 67 && byte <= 252 && byte == mx_byte(__float_as_uint(top * BELOW)) &&
-                          w == mx_codes(below, byte);
+        const float top = __uint_as_float(quad_max(max(uint32_t(plus) & 0x7FFFFFFFu, minus & 0x7FFFFFFFu)));
+        const uint32_t e = __float_as_uint(top * more) >> 23;
+        uint32_t byte = e - 2, w = mx_codes_finite(above, byte);
+        const bool sure = plain && e - 69u <= 254u - 69u && e == __float_as_uint(top * less) >> 23 && w == mx_codes_finite(below, byte);
         if (__any(!sure)) {
             double d[8];
 #pragma unroll
@@ -208,8 +217,9 @@ extern "C" int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint
     const hipStream_t st = (hipStream_t)stream;
     const bool aligned = (uintptr_t(x) | uintptr_t(nw)) % 16 == 0 && (M == 1 || ldx * size % 16 == 0);
     if (nw) {
-        // a wave a row where the rows are many and short enough for its registers, else four
-        const int wpr = K <= 4096 && M >= 1024 ? 1 : 4, pieces = (K / 8 + 64 * wpr - 1) / (64 * wpr);
+        // a wave a row where the rows are many and short enough for its registers, else four: 1024 / 2048 / 8192 rows of 2048 3.8 / 4.5 / 11.4 us,
+        // with four waves 3.3 / 4.7 / 12.8, 4096 rows of 1024 4.0 and 6.8
+        const int wpr = K <= 2048 && M >= 2048 ? 1 : 4, pieces = (K / 8 + 64 * wpr - 1) / (64 * wpr);
         const auto go = [&](auto nc) {
             constexpr int NC = decltype(nc)::value;
             if (aligned) launch_norm<NC, true>(x, ldx, nw, eps, codes, scales, M, K, wpr, st);
