@@ -218,8 +218,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
     const int odd = of_w || BM > 32 ? wave & 1 : 0;
     const int p0 = 32 * odd + lane / 2, half = 16 * (lane % 2 ^ (p0 / 8 & 1)), row0 = of_w ? source(p0) : p0;
     const unsigned scales_to = (of_w ? 0 : BN * 32) + odd * 1024, slane = unsigned(row0) * unsigned(nb) + half;
-    // what is loaded next: stage l of tile lo, its bytes to place lq % 2
-    int lo = mine, l = 0, lq = 0;
+    // what is loaded next: stage l of tile lo; the bytes loaded last went to place lq % 2
+    int lo = mine, l = 0, lq = -1;
     Buffer wbuf, xbuf, sbuf;
     const auto buffers = [&]() __attribute__((always_inline)) {
         const int m0 = tile_m(lo), n0 = tile_n(lo), first = of_w ? n0 : m0, rows = of_w ? min(a.N - n0, BN) : min(a.M - m0, BM);
@@ -234,30 +234,46 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
         if (i < WLOADS) load_lds16(wbuf, to, wlane + k + unsigned(Q == 2 ? 32 * i : i / 2 * 64 + i % 2 * 8) * row_bytes);
         else load_lds16(xbuf, to, xlane + k + unsigned(i - WLOADS) * 32u * row_bytes);
     };
-    const auto load_scales = [&]() __attribute__((always_inline)) {   // the bytes of stages l .. l + 3
-        const int c = 4 * l * 2 + half;
+    // The bytes of stages l .. l + 3; rows of bytes at any alignment come through the registers, and to LDS by put_scales.
+    constexpr int PARTS = (BN > BM ? BN : BM) / 64;
+    u32x4 held[EVEN ? 1 : PARTS];
+    int over[EVEN ? 1 : PARTS];   // how far behind the tensor's last word they are
+    bool holds = false;
+    const auto parts = [&](auto&& go) __attribute__((always_inline)) {
 #pragma unroll
-        for (int part = 0; part < (BN > BM ? BN : BM) / 64; ++part) {
-            if (part >= (of_w ? BN / 64 : BM == 32 ? 1 : BM / 64)) continue;
-            const unsigned to = (lq & 1) * SROWS + scales_to + part * 2048;
+        for (int part = 0; part < PARTS; ++part)
+            if (part < (of_w ? BN / 64 : BM == 32 ? 1 : BM / 64)) go(part, (lq & 1) * SROWS + scales_to + part * 2048);
+    };
+    const auto load_scales = [&]() __attribute__((always_inline)) {
+        const int c = 4 * l * 2 + half;
+        ++lq;
+        parts([&](int part, unsigned to) __attribute__((always_inline)) {
             if constexpr (EVEN) {
                 load_lds16(sbuf, scales_at + to, (slane + 8u * l + part * 64u * unsigned(nb)) | behind(c));
-            } else {   // rows of bytes at any alignment: through the registers
+            } else {
                 const int rows = of_w ? a.N : a.M, row = min((of_w ? tile_n(lo) : tile_m(lo)) + 64 * part + row0, rows - 1);
-                const uint8_t* s = of_w ? a.ws : a.xs;
                 const int64_t first = int64_t(row) * nb + c, last = int64_t(rows) * nb - 4;
-                u32x4 v;
+                typedef uint32_t u32u __attribute__((aligned(1)));
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {   // (the last word of the tensor holds its last bytes)
-                    typedef uint32_t u32u __attribute__((aligned(1)));
-                    const int64_t want = first + 4 * u, from = min(want, last);
-                    const uint32_t w = *reinterpret_cast<const u32u*>(s + from);
-                    v[u] = want - from >= 4 ? 0 : w >> (8 * int(want - from));
-                }
-                *reinterpret_cast<u32x4*>(s_scale + to + 16 * lane) = v;
+                for (int u = 0; u < 4; ++u) held[part][u] = *reinterpret_cast<const u32u*>((of_w ? a.ws : a.xs) + min(first + 4 * u, last));
+                over[part] = int(max(first - last, int64_t(-16)));
             }
-        }
-        ++lq;
+        });
+        holds = !EVEN;
+    };
+    const auto put_scales = [&]() __attribute__((always_inline)) {
+        if (EVEN || !holds) return;
+        holds = false;
+        parts([&](int part, unsigned to) __attribute__((always_inline)) {
+            u32x4 v;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {   // (the last word of the tensor holds its last bytes)
+                const int past = max(over[part] + 4 * u, 0);
+                v[u] = past >= 4 ? 0 : held[part][u] >> (8 * past);
+            }
+            *reinterpret_cast<u32x4*>(s_scale + to + 16 * lane) = v;
+        });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     const auto loaded = [&]() __attribute__((always_inline)) {   // on to the next stage
         if (++l < stages) return;
@@ -304,6 +320,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) load(0, i);
     loaded();
+    put_scales();
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     barrier();
     if (l % 4 == 0) load_scales();
@@ -335,6 +352,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
             // every wave has read this stage whole, and the next one is there: its loads are older than the last tile's stores
             if (t == 0 && stores) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(STORES) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            put_scales();
             barrier();
             // the stage after it into this one's place; the next one's first fragments
             const int next = t + 1 < stages ? t + 1 : 0;
