@@ -24,7 +24,8 @@ struct MxArgs {
 
 __device__ __forceinline__ i32x8 operand(u32x4 c) { return i32x8{int(c[0]), int(c[1]), int(c[2]), int(c[3]), 0, 0, 0, 0}; }
 constexpr int FP4 = 4;   // of the instructions' format operands
-typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // (the hardware takes vectors at any even address)
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // (the hardware takes vectors at any address)
+typedef uint32_t u32x4b __attribute__((ext_vector_type(4), aligned(1)));
 
 __device__ __forceinline__ float silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
     // The bytes of stages l .. l + 3; rows of bytes at any alignment come through the registers, and to LDS by put_scales.
     constexpr int PARTS = (BN > BM ? BN : BM) / 64;
     u32x4 held[EVEN ? 1 : PARTS];
-    int over[EVEN ? 1 : PARTS];   // how far behind the tensor's last word they are
+    int over[EVEN ? 1 : PARTS];   // bytes that they are behind what is held
     bool holds = false;
     const auto parts = [&](auto&& go) __attribute__((always_inline)) {
 #pragma unroll
@@ -252,11 +253,9 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
                 load_lds16(sbuf, scales_at + to, (slane + 8u * l + part * 64u * unsigned(nb)) | behind(c));
             } else {
                 const int rows = of_w ? a.N : a.M, row = min((of_w ? tile_n(lo) : tile_m(lo)) + 64 * part + row0, rows - 1);
-                const int64_t first = int64_t(row) * nb + c, last = int64_t(rows) * nb - 4;
-                typedef uint32_t u32u __attribute__((aligned(1)));
-#pragma unroll
-                for (int u = 0; u < 4; ++u) held[part][u] = *reinterpret_cast<const u32u*>((of_w ? a.ws : a.xs) + min(first + 4 * u, last));
-                over[part] = int(max(first - last, int64_t(-16)));
+                const int64_t first = int64_t(row) * nb + c, at = min(first, int64_t(rows) * nb - 16);   // (the last 16 hold the last bytes)
+                held[part] = *reinterpret_cast<const u32x4b*>((of_w ? a.ws : a.xs) + at);
+                over[part] = int(min(first - at, int64_t(16)));
             }
         });
         holds = !EVEN;
@@ -265,11 +264,18 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
         if (EVEN || !holds) return;
         holds = false;
         parts([&](int part, unsigned to) __attribute__((always_inline)) {
-            u32x4 v;
+            u32x4 v = held[part];
+            if (__any(over[part])) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {   // (the last word of the tensor holds its last bytes)
-                const int past = max(over[part] + 4 * u, 0);
-                v[u] = past >= 4 ? 0 : held[part][u] >> (8 * past);
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t two[2] = {0, 0};   // the words that hold word u's bytes
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i == u + over[part] / 4) two[0] = held[part][i];
+                        if (i == u + over[part] / 4 + 1) two[1] = held[part][i];
+                    }
+                    v[u] = uint32_t((uint64_t(two[1]) << 32 | two[0]) >> (8 * (over[part] % 4)));
+                }
             }
             *reinterpret_cast<u32x4*>(s_scale + to + 16 * lane) = v;
         });
@@ -499,7 +505,7 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     if (M == 0) return SCMX_OK;
     const MxArgs a{xcodes, xscales, wcodes, wscales, res, out, epi, M, N, K};
     const hipStream_t st = (hipStream_t)stream;
-    const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 4;   // (an operand has not four bytes of scales)
+    const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 16;   // (an operand has not sixteen bytes of scales)
     if (M <= FEW || tiny) {
         FewArgs f{};
         static_cast<MxArgs&>(f) = a;
