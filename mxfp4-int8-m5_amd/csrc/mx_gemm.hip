@@ -61,11 +61,11 @@ __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float
     *reinterpret_cast<u32x4u*>(a.out + at) = w;
 }
 
-// Few rows: a workgroup per 16 columns and 16 rows.  4096 of K at a time, the rows' codes come to LDS, as they are or made of bf16 rows (a thread
-// takes a block of 32, 64 bytes, and needs no other's values), and the waves take steps of 128 side by side, the weights straight from memory,
-// requested before the rows.  The waves meet in LDS.  Bound by reading the weights where there are many (16384 x 8192), by the launch
-// and a trip to memory where there are few.
-constexpr int FEW_BLOCKS = 128;   // of K at a time
+// Few rows: a workgroup per 16 columns (8 where the workgroups would be too few: half of a fragment's columns are none then) and 16 rows.  BLOCKS
+// of K at a time, the rows' codes come to LDS, as they are or made of bf16 rows (a thread takes a block of 32, 64 bytes, and needs no other's
+// values), and the waves take steps of 128 side by side, the weights straight from memory, requested before the rows.  The waves meet in
+// LDS.  Bound by reading the weights where there are many (16384 x 8192 20.3 us, 3.5 TB/s), by the launch and a trip to memory where there are few.
+constexpr int FEW_WAVES = 8;
 
 struct FewArgs : MxArgs {
     const uint16_t* rows;   // NULL: codes
@@ -85,28 +85,28 @@ __device__ __forceinline__ u32x4 block_codes(const u32x4 (&v)[4], uint32_t& byte
     return c;
 }
 
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(const FewArgs a) {
-    constexpr int U = FEW_BLOCKS / 4 / WAVES;   // steps of a wave, whose loads are on their way together
+template <int COLS, int BLOCKS>
+__global__ __launch_bounds__(64 * FEW_WAVES) void mx_few_kernel(const FewArgs a) {
+    constexpr int WAVES = FEW_WAVES, U = BLOCKS / 4 / WAVES;   // steps of a wave, whose loads are on their way together
     __shared__ f32x4 s_acc[WAVES][64];
-    __shared__ u32x4 s_x[16][FEW_BLOCKS + 1];   // (rows' blocks in different banks)
-    __shared__ uint8_t s_xs[16][FEW_BLOCKS + 4];
+    __shared__ u32x4 s_x[16][BLOCKS + 1];   // (rows' blocks in different banks)
+    __shared__ uint8_t s_xs[16][BLOCKS + 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
     const unsigned down = (blockIdx.z * gridDim.y + blockIdx.y) * 16;
     if (down >= unsigned(a.M)) return;
-    const int n0 = blockIdx.x * 16, m0 = int(down), nb = a.K / 32, high = min(a.M - m0, 16), row = min(ln, high - 1);
+    const int n0 = blockIdx.x * COLS, m0 = int(down), nb = a.K / 32, high = min(a.M - m0, 16), row = min(ln, high - 1);
     const size_t wr = min(n0 + ln, a.N - 1);
     const u32x4* wp = reinterpret_cast<const u32x4*>(a.w) + wr * nb;
     const uint8_t* wsp = a.ws + wr * nb;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b0 = 0; b0 < nb; b0 += FEW_BLOCKS) {
-        const int blocks = min(nb - b0, FEW_BLOCKS), per = ((blocks + 3) / 4 + WAVES - 1) / WAVES, first = wave * per;
+    for (int b0 = 0; b0 < nb; b0 += BLOCKS) {
+        const int blocks = min(nb - b0, BLOCKS), per = ((blocks + 3) / 4 + WAVES - 1) / WAVES, first = wave * per;
         u32x4 wc[U];
         uint32_t sw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = 4 * (first + u) + g;
-            const bool there = u < per && c < blocks;
+            const bool there = u < per && c < blocks && ln < COLS;
             wc[u] = there ? wp[b0 + c] : u32x4{0, 0, 0, 0};
             sw[u] = there ? wsp[b0 + c] : 0;
         }
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(const FewArgs a) {
     }
     s_acc[wave][lane] = acc;
     __syncthreads();
-    if (wave) return;
+    if (wave || 4 * g >= COLS) return;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w)
 #pragma unroll
@@ -416,16 +416,18 @@ static void by_epilogue(int epi, F&& go) {
     else if (epi == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 3>{});
 }
-template <int WAVES>
+template <int COLS, int BLOCKS>
 static void few(const FewArgs& a, hipStream_t st) {
     const unsigned down = (unsigned(a.M) + 15) / 16, z = (down + 65534) / 65535;
-    mx_few_kernel<WAVES><<<dim3((unsigned(a.N) + 15) / 16, (down + z - 1) / z, z), dim3(64 * WAVES), 0, st>>>(a);
+    mx_few_kernel<COLS, BLOCKS><<<dim3((unsigned(a.N) + COLS - 1) / COLS, (down + z - 1) / z, z), dim3(64 * FEW_WAVES), 0, st>>>(a);
 }
-// Waves of a workgroup: more where there are few of them and K is long.  us with 4 / 8 / 16: one row of 12288 x 2048 6.2 / 5.9 / 6.5, of 2048 x
-// 6144 6.5 / 6.1 / 5.7, of 4096 x 4096 5.0 / 5.1 / 4.9, sixteen of 12288 x 2048 9.1 / 8.9 / 9.2.
+// us with 16 columns and 128 blocks / 16 and 256 / 8 and 256: one row of 12288 x 2048 5.8 / 7.9 / 9.1, of 16384 x 8192 22.0 / 20.3 / 23.0, of 4096 x
+// 4096 4.8 / 4.9 / 5.1, of 2048 x 6144 5.8 / 5.3 / 4.5, 16 rows of 12288 x 2048 8.8 / 9.5 / 13.5, of 2048 x 6144 9.3 / 8.6 / 7.5.  16 waves: between
+// these, but 4.6 for 4096 x 4096.
 static void launch_few(const FewArgs& a, hipStream_t st) {
-    if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) < 256 && a.K > 4096) few<16>(a, st);
-    else few<8>(a, st);
+    if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) < 256) few<8, 256>(a, st);
+    else if (a.K > 4096) few<16, 256>(a, st);
+    else few<16, 128>(a, st);
 }
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
