@@ -8,7 +8,7 @@
  * Values become codes by one rule everywhere: byte - 127 = floor(log2 of the block's largest magnitude) - 2, at least -127, each value
  * over 2^(byte - 127) rounded to the nearest E2M1, ties to the even code, what passes 6 held to 6; a block with a NaN or an infinity
  * takes the byte 255 (codes 0).
- * codes are 16-byte aligned. */
+ * codes are 16-byte aligned, scales at any address. */
 #ifndef SCMX_MX_H
 #define SCMX_MX_H
 
@@ -22,7 +22,7 @@ extern "C" {
 #define SCMX_MX_F16 1
 #define SCMX_MX_F32 2
 
-/* x [M, K] of `type`, row i at element i * ldx (ldx >= K, any alignment), to codes and scales.  With nw (bf16 [K]; x bf16, K <= 16384):
+/* x [M, K] of `type` (K <= 2^30), row i at element i * ldx (ldx >= K, any alignment), to codes and scales.  With nw (bf16 [K]; x bf16, K <= 16384):
  * of the rows' RMSNorm x / sqrt(mean(x^2) + eps) * nw, in float64, so that a value beside the border of two codes takes its own; there
  * byte is at least 10, and magnitudes from 2^128 on count as the largest below. */
 int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M,
@@ -31,7 +31,7 @@ int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, f
 /* The values of M rows of K as bf16 or float32 (type; 16-byte aligned): exact but where they pass that type's range. */
 int scmx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int type, int M, int K, void* stream);
 
-/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values (K <= 2^23), on the scaled matrix instructions, sums in float32, each result rounded
+/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values (K <= 2^23, M and N < 2^31 - 511; N <= 2^26 where M <= 16), on the scaled matrix instructions, sums in float32, each result rounded
  * once to bf16: epi 1: out [M, N]; 2: + res [M, N]; 3: silu(gate) * up of w rows in the order of the SwiGLU epilogue of scmx.h (two gates,
  * their two ups; N a multiple of 4), out [M, N / 2]. */
 int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, const uint16_t* res,

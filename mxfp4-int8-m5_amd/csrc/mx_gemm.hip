@@ -429,6 +429,9 @@ static void launch_few(const FewArgs& a, hipStream_t st) {
     else if (a.K > 4096) few<16, 256>(a, st);
     else few<16, 128>(a, st);
 }
+// Whether every row's bytes are whole words.
+static bool words(const MxArgs& a) { return a.K % 128 == 0 && (reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) % 4 == 0; }
+
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
     const int tm = int((unsigned(a.M) + BM - 1) / BM), tn = int((unsigned(a.N) + BN - 1) / BN);
@@ -436,7 +439,7 @@ static void launch_tile(const MxArgs& a, hipStream_t st) {
     const dim3 grid(tiles < most ? tiles : most);
     by_epilogue(a.epi, [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
-        if (BM + BN == 512 || a.K % 128 == 0) mx_tile_kernel<BM, BN, EPI, true><<<grid, dim3(256), 0, st>>>(a, tm, tn);
+        if (BM + BN == 512 || words(a)) mx_tile_kernel<BM, BN, EPI, true><<<grid, dim3(256), 0, st>>>(a, tm, tn);
         else if constexpr (BM + BN < 512) mx_tile_kernel<BM, BN, EPI, false><<<grid, dim3(256), 0, st>>>(a, tm, tn);
     });
 }
@@ -473,11 +476,11 @@ static int check_mm(const char* who, const void* w, const void* ws, const void* 
 // columns, K from 256 to 8192, where the choice is half a per cent off the best on average.  us for 32x128 / 64x128 / 128x128 / 256x256: 100 rows
 // of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944 20.6 / 14.3 / 12.8 / 28.4, 6000 of 12288 x
 // 2048 180 / 124 / 92 / 89, of 2048 x 8192 114 / 70 / 74 / 56, 4000 of 16384 x 512 58 / 44 / 35 / 46.
-static int tile_of(int M, int N, int K) {
+static int tile_of(int M, int N, int K, bool words) {
     constexpr int BM[4] = {32, 64, 128, 256}, BN[4] = {128, 128, 128, 256};
     constexpr double ALONE[4] = {0.34, 0.35, 0.49, 1.1}, ALONE_ENDS[4] = {1.1, 1.4, 1.8, 5.2};
     constexpr double FULL[4] = {0.25, 0.34, 0.5, 1.4}, FULL_ENDS[4] = {0.45, 0.82, 1.2, 7.5};
-    const int cus = device_cus(), most = N % 16 || K % 128 ? 3 : 4;   // (the largest takes whole groups of columns and words of bytes)
+    const int cus = device_cus(), most = N % 16 || !words ? 3 : 4;   // (the largest takes whole groups of columns and words of bytes)
     const double stages = (K + 255) / 256;
     int best = 0;
     double least = 1e30;
@@ -508,12 +511,17 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     const MxArgs a{xcodes, xscales, wcodes, wscales, res, out, epi, M, N, K};
     const hipStream_t st = (hipStream_t)stream;
     const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 16;   // (an operand has not sixteen bytes of scales)
+    const int most = 0x7FFFFE00;   // (a tile's rows and columns behind the last are numbers too)
+    if (M <= FEW || tiny ? N > 1 << 26 : M > most || N > most) {
+        set_error("mx_mm: too many rows or columns (M=%d N=%d)", M, N);
+        return SCMX_ERR_ARG;
+    }
     if (M <= FEW || tiny) {
         FewArgs f{};
         static_cast<MxArgs&>(f) = a;
         launch_few(f, st);
     } else {
-        switch (tile_of(M, N, K)) {
+        switch (tile_of(M, N, K, words(a))) {
             case 0: launch_tile<32, 128>(a, st); break;
             case 1: launch_tile<64, 128>(a, st); break;
             case 2: launch_tile<128, 128>(a, st); break;
@@ -523,9 +531,10 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     return check_launch("mx_mm");
 }
 
-// Whether a linear layer's rows are quantised in the product's own kernel: every workgroup of 16 columns does it for itself, which reads the
-// rows N / 16 times.
-static bool in_one(int M, int N, int K) { return M <= FEW && int64_t(M) * K * N <= (int64_t(1) << 28); }
+// Whether a linear layer's rows are quantised in the product's own kernel: every workgroup of its columns does it for itself, which costs a
+// launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6, 16 rows of 4096 x 4096 (2^28)
+// 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1 / 15.9, 4 rows of 32768 x 8192 40.4 / 38.1.
+static bool in_one(int M, int N, int K) { return M <= FEW && int64_t(M) * K * N <= (int64_t(1) << 29); }
 
 extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K, int norm) {
     if (M < 1 || N < 1 || K < 32 || K % 32 || (!norm && in_one(M, N, K))) return 0;
@@ -547,7 +556,7 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
     }
     if (M == 0) return SCMX_OK;
     if (M == 1) ldx = K;
-    if (in_one(M, N, K) && !nw) {
+    if (in_one(M, N, K) && !nw) {   // (N is at most 2^24 then)
         FewArgs a{};
         static_cast<MxArgs&>(a) = MxArgs{nullptr, nullptr, wcodes, wscales, res, out, epi, M, N, K};
         a.rows = x;

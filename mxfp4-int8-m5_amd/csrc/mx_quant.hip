@@ -10,6 +10,13 @@ namespace scmx {
 
 constexpr int QNT = 256, QPIECES = 4;   // pieces of 512 values that a wave takes of a row at once
 
+// Blocks in two dimensions: a launch's threads in one are below 2^32.
+static dim3 grid_of(uint64_t blocks) {
+    const uint64_t x = blocks < (1u << 22) ? blocks : 1u << 22;
+    return dim3(unsigned(x), unsigned((blocks + x - 1) / x));
+}
+__device__ __forceinline__ uint64_t block_index() { return uint64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 template <int TYPE>
 struct Raw8 {
     u32x4 w[TYPE == SCMX_MX_F32 ? 2 : 1];
@@ -46,9 +53,9 @@ template <int TYPE, bool ALIGNED>
 __global__ __launch_bounds__(QNT) void mx_quantize_kernel(const void* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
                                                           uint8_t* __restrict__ scales, int M, int K, int chunks) {
     const int lane = threadIdx.x & 63;
-    const uint64_t unit = uint64_t(blockIdx.x) * (QNT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = int(unit / uint32_t(chunks)), k0 = int(unit - uint64_t(row) * uint32_t(chunks)) * (512 * QPIECES) + 8 * lane;
-    if (row >= M) return;
+    const uint64_t unit = block_index() * (QNT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = unit / uint32_t(chunks);
+    if (at >= uint64_t(M)) return;
+    const int row = int(at), k0 = int(unit - at * uint32_t(chunks)) * (512 * QPIECES) + 8 * lane;
     Raw8<TYPE> r[QPIECES];
 #pragma unroll
     for (int p = 0; p < QPIECES; ++p)   // (behind the row's end: its last values again)
@@ -97,8 +104,9 @@ __global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(c
                                                                int K) {
     __shared__ double s_sum[QNT / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = wave % WPR * 64 + lane;
-    const int row = blockIdx.x * (QNT / 64 / WPR) + wave / WPR;
-    if (row >= M) return;   // (a row's waves together)
+    const uint64_t unit = block_index() * (QNT / 64 / WPR) + wave / WPR;
+    if (unit >= uint64_t(M)) return;   // (a row's waves together)
+    const int row = int(unit);
     Raw8<SCMX_MX_BF16> r[NC];
     const size_t at = size_t(int64_t(row) * ldx);
 #pragma unroll
@@ -162,7 +170,7 @@ __global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(c
 template <bool F32>
 __global__ __launch_bounds__(QNT) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             void* __restrict__ out, uint64_t words) {
-    const uint64_t i = uint64_t(blockIdx.x) * QNT + threadIdx.x;   // of eight values
+    const uint64_t i = block_index() * QNT + threadIdx.x;   // of eight values
     if (i >= words) return;
     const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i];
     const float s = mx_scale(scales[i / 4]);
@@ -181,8 +189,8 @@ template <int NC, bool ALIGNED>
 static void launch_norm(const void* x, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M, int K, int wpr,
                         hipStream_t st) {
     const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<dim3((unsigned(M) + 3) / 4), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
-    else mx_norm_quantize_kernel<NC, 4, ALIGNED><<<dim3(M), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
+    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<grid_of((uint64_t(M) + 3) / 4), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
+    else mx_norm_quantize_kernel<NC, 4, ALIGNED><<<grid_of(M), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
 }
 
 }  // namespace scmx
@@ -191,8 +199,8 @@ using namespace scmx;
 
 extern "C" int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M,
                                 int K, void* stream) {
-    if (M < 0 || K < 32 || K % 32 || (type != SCMX_MX_BF16 && type != SCMX_MX_F16 && type != SCMX_MX_F32)) {
-        set_error("mx_quantize: need rows of a multiple of 32 values in bf16, fp16 or float32 (M=%d K=%d type=%d)", M, K, type);
+    if (M < 0 || K < 32 || K % 32 || K > (1 << 30) || (type != SCMX_MX_BF16 && type != SCMX_MX_F16 && type != SCMX_MX_F32)) {
+        set_error("mx_quantize: need rows of a multiple of 32 values, up to 2^30, in bf16, fp16 or float32 (M=%d K=%d type=%d)", M, K, type);
         return SCMX_ERR_ARG;
     }
     if (M && (!x || !codes || !scales)) {
@@ -233,14 +241,14 @@ extern "C" int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint
     }
     const int chunks = (K + 512 * QPIECES - 1) / (512 * QPIECES);
     const uint64_t blocks = (uint64_t(M) * chunks + QNT / 64 - 1) / (QNT / 64);
-    if (blocks > 0x7FFFFFFFull) {
+    if (blocks > (uint64_t(1) << 37)) {
         set_error("mx_quantize: too many values (M=%d K=%d)", M, K);
         return SCMX_ERR_ARG;
     }
     const auto go = [&](auto t) {
         constexpr int TYPE = decltype(t)::value;
-        if (aligned) mx_quantize_kernel<TYPE, true><<<dim3(unsigned(blocks)), dim3(QNT), 0, st>>>(x, ldx, codes, scales, M, K, chunks);
-        else mx_quantize_kernel<TYPE, false><<<dim3(unsigned(blocks)), dim3(QNT), 0, st>>>(x, ldx, codes, scales, M, K, chunks);
+        if (aligned) mx_quantize_kernel<TYPE, true><<<grid_of(blocks), dim3(QNT), 0, st>>>(x, ldx, codes, scales, M, K, chunks);
+        else mx_quantize_kernel<TYPE, false><<<grid_of(blocks), dim3(QNT), 0, st>>>(x, ldx, codes, scales, M, K, chunks);
     };
     if (type == SCMX_MX_BF16) go(std::integral_constant<int, SCMX_MX_BF16>{});
     else if (type == SCMX_MX_F16) go(std::integral_constant<int, SCMX_MX_F16>{});
@@ -262,13 +270,13 @@ extern "C" int scmx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, v
         return SCMX_ERR_ARG;
     }
     const uint64_t words = uint64_t(M) * (K / 8), blocks = (words + QNT - 1) / QNT;
-    if (blocks > 0x7FFFFFFFull) {
+    if (blocks > (uint64_t(1) << 37)) {
         set_error("mx_dequantize: too many values (M=%d K=%d)", M, K);
         return SCMX_ERR_ARG;
     }
     if (M == 0) return SCMX_OK;
     const hipStream_t st = (hipStream_t)stream;
-    if (type == SCMX_MX_F32) mx_dequantize_kernel<true><<<dim3(unsigned(blocks)), dim3(QNT), 0, st>>>(codes, scales, out, words);
-    else mx_dequantize_kernel<false><<<dim3(unsigned(blocks)), dim3(QNT), 0, st>>>(codes, scales, out, words);
+    if (type == SCMX_MX_F32) mx_dequantize_kernel<true><<<grid_of(blocks), dim3(QNT), 0, st>>>(codes, scales, out, words);
+    else mx_dequantize_kernel<false><<<grid_of(blocks), dim3(QNT), 0, st>>>(codes, scales, out, words);
     return check_launch("mx_dequantize");
 }

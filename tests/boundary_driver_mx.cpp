@@ -61,6 +61,9 @@ int main() {
     expect_valid(quantize(p(0) + 2, SCMX_MX_F16, 2051, nullptr, 3, 2048), "quantize fp16 at odd places");
     expect_valid(quantize(p(0), SCMX_MX_BF16, 16384, u16(1), 1, 16384), "quantize a norm");
     expect_valid(quantize(p(0), SCMX_MX_F32, 32, nullptr, 2147483647, 32), "quantize, most rows");
+    expect_valid(quantize(p(0), SCMX_MX_BF16, 32, u16(1), 2147483647, 32), "quantize a norm, most rows");
+    expect_valid(quantize(p(0), SCMX_MX_F32, 1 << 30, nullptr, 1, 1 << 30), "quantize, longest rows");
+    expect(quantize(p(0), SCMX_MX_F32, (1 << 30) + 32, nullptr, 1, (1 << 30) + 32), SCMX_ERR_ARG, "quantize, rows too long");
     expect(quantize(nullptr, SCMX_MX_BF16, 32, nullptr, 0, 32), SCMX_OK, "quantize nothing");
     expect(quantize(nullptr, SCMX_MX_BF16, 32, nullptr, 1, 32), SCMX_ERR_ARG, "quantize without rows");
     expect(quantize(p(0), 3, 32, nullptr, 1, 32), SCMX_ERR_ARG, "quantize another type");
@@ -85,7 +88,9 @@ int main() {
         for (int K : {32, 96, 2048, 8192})
             for (int epi : {1, 2, 3}) expect_valid(mm(epi, M, 4096, K, u16(4)), "mm");
     expect_valid(mm(1, 2147483647, 3, 32), "mm, most rows");
-    expect_valid(mm(1, 5, 2147483647, 32), "mm, most columns");
+    expect_valid(mm(1, 5, 1 << 26, 32), "mm, most columns");
+    expect(mm(1, 5, (1 << 26) + 1, 32), SCMX_ERR_ARG, "mm, too many columns");
+    expect(mm(1, 2147483647, 15, 64), SCMX_ERR_ARG, "mm, too many rows");
     expect(mm(1, 0, 64, 64), SCMX_OK, "mm of nothing");
     expect(mm(0, 1, 64, 64), SCMX_ERR_ARG, "mm, epilogue 0");
     expect(mm(4, 1, 64, 64), SCMX_ERR_ARG, "mm, epilogue 4");

@@ -100,3 +100,39 @@ def test_norms_on_the_borders(X):   # noqa: F811
     for rows in (x, x[:7]):   # a wave a row, four waves a row
         for eps in (0.0, 2.0 ** -30, 2.0 ** -24, 2.0 ** -20, 2.0 ** -10):
             assert same(X.quantize(rows, w, eps), O.quantize(O.rmsnorm(f64(rows), f64(w), eps), 10, 252)), eps
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 600, 256), (40, 130, 512), (300, 1500, 384), (2040, 8192, 1152)])
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_scales_at_any_address(X, M, N, K, at):   # noqa: F811
+    """Bytes that start off a word, of rows of whole words: the results of aligned ones, which take other tiles and sums of another order."""
+    rnd = gen(M + at)
+    x, w = operands(X, rnd, M, N, K)
+    xq = X.quantize(x)
+
+    def moved(t):
+        out = torch.empty(t.numel() + at, dtype=torch.uint8, device="cuda")[at:].view(t.shape)
+        return out.copy_(t)
+
+    rows = np.arange(0, M, max(1, M // 40))
+    pick = torch.from_numpy(rows).cuda()
+    xv, wv = O.values(*host(xq[0][pick], xq[1][pick])), O.values(*host(*w))
+    for s, ws in ((moved(xq[1]), w[1]), (xq[1], moved(w[1])), (moved(xq[1]), moved(w[1]))):
+        check_product(X.mm(xq[0], s, w[0], ws)[pick], xv, wv, 1, None)
+        assert np.array_equal(f64(X.dequantize(w[0], ws)), O.values(*host(*w)))
+    check_product(X.linear(x, w[0], moved(w[1]))[pick], xv, wv, 1, None)
+
+
+def test_rows_beyond_a_launchs_threads(X):   # noqa: F811
+    """2^25 rows of one block: more threads than a launch has in one dimension; there and back."""
+    M = (1 << 25) + 3
+    x = torch.arange(M * 32, device="cuda", dtype=torch.int32).remainder(251).sub(125).to(BF).view(M, 32)
+    codes, scales = X.quantize(x)
+    few = torch.cat([torch.arange(0, M, 1000003, device="cuda"), torch.arange(M - 20, M, device="cuda")])
+    assert same((codes[few], scales[few]), O.quantize(f64(x[few])))
+    back = X.dequantize(codes, scales)
+    assert np.array_equal(f64(back[few]), O.values(*host(codes[few], scales[few])))
+    del back
+    gain = torch.ones(32, device="cuda", dtype=BF)
+    codes, scales = X.quantize(x, gain, 1e-6)
+    assert same((codes[few], scales[few]), O.quantize(O.rmsnorm(f64(x[few]), np.ones(32), 1e-6), 10, 252))
