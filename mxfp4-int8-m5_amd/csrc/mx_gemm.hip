@@ -31,7 +31,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)) * u;
 }
 
-// Columns n .. n + 3 of row m, those that are inside (n is a multiple of 4), one by one.
+// Columns n .. n + 3 of row m, those that are inside (n is a multiple of 4); one by one where rows are no multiple of 4.
 template <int EPI>
 __device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
     if (m >= a.M) return;
@@ -39,6 +39,14 @@ __device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
         if (n < a.N) *reinterpret_cast<uint32_t*>(a.out + (size_t(m) * a.N + n) / 2) = f32_to_bf16x2(silu_mul(v[0], v[2]), silu_mul(v[1], v[3]));
     } else {
         const size_t at = size_t(m) * a.N + n;
+        if (a.N % 4 == 0) {
+            if (n >= a.N) return;
+            u32x2 r = {0, 0};
+            if constexpr (EPI == 2) r = *reinterpret_cast<const u32x2*>(a.res + at);
+            *reinterpret_cast<u32x2*>(a.out + at) = EPI == 2 ? u32x2{f32_to_bf16x2(v[0] + bf16_lo(r[0]), v[1] + bf16_hi(r[0])), f32_to_bf16x2(v[2] + bf16_lo(r[1]), v[3] + bf16_hi(r[1]))}
+                                                             : u32x2{f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3])};
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (n + i < a.N) a.out[at + i] = f32_to_bf16(EPI == 2 ? v[i] + bf16_to_f32(a.res[at + i]) : v[i]);
@@ -476,14 +484,17 @@ static int check_mm(const char* who, const void* w, const void* ws, const void* 
 // columns, K from 256 to 8192, where the choice is half a per cent off the best on average.  us for 32x128 / 64x128 / 128x128 / 256x256: 100 rows
 // of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944 20.6 / 14.3 / 12.8 / 28.4, 6000 of 12288 x
 // 2048 180 / 124 / 92 / 89, of 2048 x 8192 114 / 70 / 74 / 56, 4000 of 16384 x 512 58 / 44 / 35 / 46.
+// Some rows go to the kernel of few, 16 at a time, where its workgroups are few too (us with tiles / with it: 17 rows of 2048 x 2048 5.9 / 3.5, of 4096 x
+// 4096 8.6 / 6.7, of 12288 x 2048 6.1 / 9.0, 64 rows of 2048 x 2048 6.1 / 4.5, of 2048 x 8192 14.2 / 11.9, of 4096 x 4096 8.8 / 12.2, 333 of 512 x 2048 6.0 / 5.7).
+constexpr int NO_TILE = 4;
 static int tile_of(int M, int N, int K, bool words) {
     constexpr int BM[4] = {32, 64, 128, 256}, BN[4] = {128, 128, 128, 256};
     constexpr double ALONE[4] = {0.34, 0.35, 0.49, 1.1}, ALONE_ENDS[4] = {1.1, 1.4, 1.8, 5.2};
     constexpr double FULL[4] = {0.25, 0.34, 0.5, 1.4}, FULL_ENDS[4] = {0.45, 0.82, 1.2, 7.5};
     const int cus = device_cus(), most = N % 16 || !words ? 3 : 4;   // (the largest takes whole groups of columns and words of bytes)
-    const double stages = (K + 255) / 256;
-    int best = 0;
-    double least = 1e30;
+    const double stages = (K + 255) / 256, groups = double((int64_t(M) + 15) / 16) * double((int64_t(N) + 15) / 16) / cus;
+    int best = NO_TILE;
+    double least = (groups < 1 ? 1 : groups) * (0.135 * stages + 0.33);
     for (int i = 0; i < most; ++i) {
         const int64_t tiles = (int64_t(M) + BM[i] - 1) / BM[i] * ((int64_t(N) + BN[i] - 1) / BN[i]);
         const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
@@ -511,21 +522,20 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     const MxArgs a{xcodes, xscales, wcodes, wscales, res, out, epi, M, N, K};
     const hipStream_t st = (hipStream_t)stream;
     const bool tiny = int64_t(K / 32) * (M < N ? M : N) < 16;   // (an operand has not sixteen bytes of scales)
-    const int most = 0x7FFFFE00;   // (a tile's rows and columns behind the last are numbers too)
-    if (M <= FEW || tiny ? N > 1 << 26 : M > most || N > most) {
+    const int tile = M <= FEW || tiny ? NO_TILE : tile_of(M, N, K, words(a)), most = 0x7FFFFE00;
+    if (tile == NO_TILE ? N > 1 << 26 : M > most || N > most) {   // (a tile's rows and columns behind the last are numbers too)
         set_error("mx_mm: too many rows or columns (M=%d N=%d)", M, N);
         return SCMX_ERR_ARG;
     }
-    if (M <= FEW || tiny) {
-        FewArgs f{};
-        static_cast<MxArgs&>(f) = a;
-        launch_few(f, st);
-    } else {
-        switch (tile_of(M, N, K, words(a))) {
-            case 0: launch_tile<32, 128>(a, st); break;
-            case 1: launch_tile<64, 128>(a, st); break;
-            case 2: launch_tile<128, 128>(a, st); break;
-            default: launch_tile<256, 256>(a, st);
+    switch (tile) {
+        case 0: launch_tile<32, 128>(a, st); break;
+        case 1: launch_tile<64, 128>(a, st); break;
+        case 2: launch_tile<128, 128>(a, st); break;
+        case 3: launch_tile<256, 256>(a, st); break;
+        default: {
+            FewArgs f{};
+            static_cast<MxArgs&>(f) = a;
+            launch_few(f, st);
         }
     }
     return check_launch("mx_mm");
