@@ -31,7 +31,7 @@ int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, f
 /* The values of M rows of K as bf16 or float32 (type; 16-byte aligned): exact but where they pass that type's range. */
 int scmx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int type, int M, int K, void* stream);
 
-/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values (K <= 2^23, M and N < 2^31 - 511; N <= 2^26 where M <= 16), on the scaled matrix instructions, sums in float32, each result rounded
+/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values (K <= 2^23, M and N < 2^31 - 511; N <= 2^26 where M <= 16 or M times K is below 512), on the scaled matrix instructions, sums in float32, each result rounded
  * once to bf16: epi 1: out [M, N]; 2: + res [M, N]; 3: silu(gate) * up of w rows in the order of the SwiGLU epilogue of scmx.h (two gates,
  * their two ups; N a multiple of 4), out [M, N / 2]. */
 int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, const uint16_t* res,

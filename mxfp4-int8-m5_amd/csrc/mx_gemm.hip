@@ -541,10 +541,13 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     return check_launch("mx_mm");
 }
 
-// Whether a linear layer's rows are quantised in the product's own kernel: every workgroup of its columns does it for itself, which costs a
-// launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6, 16 rows of 4096 x 4096 (2^28)
-// 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1 / 15.9, 4 rows of 32768 x 8192 40.4 / 38.1.
-static bool in_one(int M, int N, int K) { return M <= FEW && int64_t(M) * K * N <= (int64_t(1) << 29); }
+// Whether a linear layer's rows are quantised in the product's own kernel, that of few: every workgroup of its columns does it for itself, which
+// costs a launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6, 16 rows of 4096 x 4096
+// (2^28) 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1 / 15.9, 64 rows of 2048 x 2048
+// (2^28) 6.3 / 7.4, 32 of 2048 x 8192 (2^29) 10.5 / 11.7, of 4096 x 4096 10.2 / 9.9, 64 of 2048 x 8192 (2^30) 18.3 / 15.5.
+static bool in_one(int M, int N, int K) {
+    return int64_t(M) * N <= (int64_t(1) << 29) / K && (M <= FEW || tile_of(M, N, K, true) == NO_TILE);
+}
 
 extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K, int norm) {
     if (M < 1 || N < 1 || K < 32 || K % 32 || (!norm && in_one(M, N, K))) return 0;

@@ -115,7 +115,7 @@ int main() {
     expect(linear(1, 2, 4096, 2048, INT64_MAX, nullptr, 0, nullptr, u16(0)), SCMX_ERR_ARG, "linear of rows too far apart");
     expect(linear(1, 2, 4096, 32768, 32768, u16(1), size_t(1) << 30, p(6), u16(0)), SCMX_ERR_ARG, "linear, a norm of too many values");
     if (scmx_mx_linear_workspace(0, 1, 32, 1) || scmx_mx_linear_workspace(1, 0, 32, 1) || scmx_mx_linear_workspace(1, 1, 33, 1) || scmx_mx_linear_workspace(1, 4096, 2048, 0) ||
-        scmx_mx_linear_workspace(1, 4096, 2048, 1) != 1024 + 64 || scmx_mx_linear_workspace(333, 64, 96, 0) != 333 * 51)
+        scmx_mx_linear_workspace(1, 4096, 2048, 1) != 1024 + 64 || scmx_mx_linear_workspace(333, 64, 96, 1) != 333 * 51 || scmx_mx_linear_workspace(2147483647, 2147483647, 1 << 23, 0) == 0)
         ++failures;
 
     const auto write = [&](const uint16_t* y, uint8_t* ks, uint8_t* vs, int L, int hq, int hk, int d, int64_t pos, int rows, const int64_t* dev = nullptr) {
