@@ -589,6 +589,33 @@ PyObject* mx_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
 }
 
+// mx_mm(xcodes, xscales, wcodes, wscales, epi, res)
+PyObject* mx_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    try {
+        if (n != 6) fail(PyExc_TypeError, "mx_mm takes 6 arguments");
+        const at::Tensor *xc, *xs, *wc, *ws, *res = nullptr;
+        if (!PyLong_CheckExact(args[4]) || !pair_of(args[0], args[1], xc, xs) || !pair_of(args[2], args[3], wc, ws) || xc->size(1) != wc->size(1)) Py_RETURN_NONE;
+        const int64_t epi = as_int(args[4]), M = xc->size(0), N = wc->size(0), K = 2 * xc->size(1);
+        if (epi < 1 || epi > 3 || N < 1 || (epi == 3 && N % 4)) Py_RETURN_NONE;
+        if (epi == 2) {
+            res = local(args[5], at::ScalarType::BFloat16);
+            if (!res || res->dim() != 2 || res->size(0) != M || res->size(1) != N) Py_RETURN_NONE;
+        }
+        at::Tensor out;
+        int rc;
+        {
+            const NoGil released;
+            out = fresh(*xc, at::ScalarType::BFloat16, {M, epi == 3 ? N / 2 : N});
+            rc = scmx_mx_mm(bytes(*xc), bytes(*xs), bytes(*wc), bytes(*ws), res ? static_cast<const uint16_t*>(res->data_ptr()) : nullptr,
+                            static_cast<uint16_t*>(out.data_ptr()), int(epi), int(M), int(N), int(K), stream());
+        }
+        if (rc != SCMX_OK) return status("scmx_mx_mm", rc);
+        return THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        return raised();
+    }
+}
+
 // mx_linear(x, wcodes, wscales, epi, res, nw, eps)
 PyObject* mx_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
     try {
@@ -656,7 +683,7 @@ PyMODINIT_FUNC PyInit__binding() {
         FUNCTION(cache_write), FUNCTION(cache_read), FUNCTION(cache_keep), FUNCTION(attn_tree), FUNCTION(verify_drafts),
         ENTRY(scmx_mx_quantize), ENTRY(scmx_mx_dequantize), ENTRY(scmx_mx_mm), ENTRY(scmx_mx_linear), ENTRY(scmx_cache4_write),
         ENTRY(scmx_cache4_read), ENTRY(scmx_cache4_keep), ENTRY(scmx_attn_tree4), QUERY(scmx_mx_linear_workspace), QUERY(scmx_attn_tree4_splits),
-        FUNCTION(mx_quantize), FUNCTION(mx_dequantize), FUNCTION(mx_linear),
+        FUNCTION(mx_quantize), FUNCTION(mx_dequantize), FUNCTION(mx_mm), FUNCTION(mx_linear),
         FUNCTION(gemv),
         EMPTY(bf16, BFloat16), EMPTY(i8, Char), EMPTY(u8, Byte), EMPTY(i32, Int), EMPTY(i64, Long), EMPTY(f32, Float),
         {nullptr, nullptr, 0, nullptr}};

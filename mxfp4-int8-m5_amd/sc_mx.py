@@ -69,6 +69,9 @@ def _check_product(M, K, wcodes, wscales, epi, res, like):
 def mm(xcodes, xscales, wcodes, wscales, epi=1, res=None):
     """x w^T of MXFP4 rows x [M, K] and weights w [N, K], sums in float32 -> bfloat16: epi 1 [M, N], 2 + res [M, N], 3 SwiGLU of w rows in
     the order of sc_kernels.interleave_gate_up [M, N / 2]."""
+    out = _lib.native().mx_mm(xcodes, xscales, wcodes, wscales, epi, res)
+    if out is not None:
+        return out
     M, K = _check_pair(xcodes, xscales, "rows")
     _on_device(xcodes, xscales, wcodes, wscales, res if epi == 2 else None)
     N, out = _check_product(M, K, wcodes, wscales, epi, res, xcodes)
