@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        } else {   // the last columns of a number that is no multiple of 16: one by one
+        } else {   // the last columns of a number that is no multiple of 16: a fragment's four at a time
             stores = false;
 #pragma unroll
             for (int j = 0; j < TJ; ++j) {
@@ -429,11 +429,11 @@ static void few(const FewArgs& a, hipStream_t st) {
     const unsigned down = (unsigned(a.M) + 15) / 16, z = (down + 65534) / 65535;
     mx_few_kernel<COLS, BLOCKS><<<dim3((unsigned(a.N) + COLS - 1) / COLS, (down + z - 1) / z, z), dim3(64 * FEW_WAVES), 0, st>>>(a);
 }
-// us with 16 columns and 128 blocks / 16 and 256 / 8 and 256: one row of 12288 x 2048 5.8 / 7.9 / 9.1, of 16384 x 8192 22.0 / 20.3 / 23.0, of 4096 x
-// 4096 4.8 / 4.9 / 5.1, of 2048 x 6144 5.8 / 5.3 / 4.5, 16 rows of 12288 x 2048 8.8 / 9.5 / 13.5, of 2048 x 6144 9.3 / 8.6 / 7.5.  16 waves: between
-// these, but 4.6 for 4096 x 4096.
+// Eight columns where that leaves no CU two workgroups.  us with 16 columns and 128 blocks / 16 and 256 / 8 and 256: one row of 12288 x 2048 4.9 / 6.9 /
+// 7.7, of 16384 x 8192 20.1 / 17.9 / 20.0, of 4096 x 4096 4.1 / 4.2 / 4.5, of 2944 x 6752 4.3 / 4.2 / 4.9, of 2048 x 8192 6.1 / 5.9 / 4.5, 16 rows of 12288 x
+// 2048 5.6 / 7.7 / 9.0, of 2048 x 8192 7.8 / 7.8 / 6.7.  16 waves: between these; 64 blocks: no better.
 static void launch_few(const FewArgs& a, hipStream_t st) {
-    if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) < 256) few<8, 256>(a, st);
+    if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) <= device_cus() / 2) few<8, 256>(a, st);
     else if (a.K > 4096) few<16, 256>(a, st);
     else few<16, 128>(a, st);
 }
@@ -498,7 +498,8 @@ static int tile_of(int M, int N, int K, bool words) {
     for (int i = 0; i < most; ++i) {
         const int64_t tiles = (int64_t(M) + BM[i] - 1) / BM[i] * ((int64_t(N) + BN[i] - 1) / BN[i]);
         const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
-        const double alone = ALONE[i] * stages + ALONE_ENDS[i], full = (FULL[i] * stages + FULL_ENDS[i]) * load, us = alone > full ? alone : full;
+        const double alone = (ALONE[i] + (words ? 0 : 0.13)) * stages + ALONE_ENDS[i], full = ((FULL[i] + (words ? 0 : 0.08)) * stages + FULL_ENDS[i]) * load;
+        const double us = alone > full ? alone : full;
         if (us < least) {
             least = us;
             best = i;
@@ -545,8 +546,8 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
 // costs a launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6, 16 rows of 4096 x 4096
 // (2^28) 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1 / 15.9, 64 rows of 2048 x 2048
 // (2^28) 6.3 / 7.4, 32 of 2048 x 8192 (2^29) 10.5 / 11.7, of 4096 x 4096 10.2 / 9.9, 64 of 2048 x 8192 (2^30) 18.3 / 15.5.
-static bool in_one(int M, int N, int K) {
-    return int64_t(M) * N <= (int64_t(1) << 29) / K && (M <= FEW || tile_of(M, N, K, true) == NO_TILE);
+static bool in_one(int M, int N, int K) {   // (bytes off a word only turn more to that kernel)
+    return int64_t(M) * N <= (int64_t(1) << 29) / K && (M <= FEW || tile_of(M, N, K, K % 128 == 0) == NO_TILE);
 }
 
 extern "C" size_t scmx_mx_linear_workspace(int M, int N, int K, int norm) {
