@@ -64,7 +64,8 @@ int scmx_cache4_keep(const uint64_t* caches, int layers, int hk, int d, int cach
 
 /* scmx_attn_tree over such a cache.  q . K^T is taken to float32: q as two E4M3 parts a block of 32, whose sum differs from q by at most
  * 2^-23 of the block's largest value, times K as it is held.  The probabilities are held in 16 bits, as two bf16 parts, in the sum
- * and in the denominator alike (2^-15 of sum p |v| at most).  A row's NaN reaches the nodes that see it and no other.  Scale bytes of rows that are read are at most 252, as
+ * and in the denominator alike (2^-15 of sum p |v| at most).  Values of any size: sums of 6 * 2^125 over 2^31 rows stay in float32; where a
+ * query meets p |v| from 2^90 on, probabilities below 2^-80 of its largest may count as none.  A row's NaN reaches the nodes that see it and no other.  Scale bytes of rows that are read are at most 252, as
  * the append's are, or 255. */
 int scmx_attn_tree4_splits(int T, int n, int hq, int hk, int d);
 int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const uint8_t* vcache, const uint8_t* kscale, const uint8_t* vscale,

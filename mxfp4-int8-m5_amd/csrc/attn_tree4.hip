@@ -13,7 +13,7 @@
 // O^T = V^T P^T in bf16: a lane reads DPL = d / 16 consecutive codes of eight V rows, the conversion applies the row's block scale (exact
 // in bf16), byte permutes pair the rows.  The weights are two bf16 parts, what rounds to bf16 and what is left, 16 bits in all, and each product
 // is two: in one part (2^-8) the weights' rounding was as large as the result's, and larger where values cancel.  One token over 300 / 40000 rows
-// of 16:8 x 128 6.3 / 13.1 us, 64 tokens over 6000 of 32:8 x 128 20.8 (in one part 6.0 / 12.7 / 18.7).
+// of 16:8 x 128 6.3 / 13.1 us, 64 tokens over 6000 of 32:8 x 128 20.6 (in one part 6.0 / 12.6 / 18.6).
 #include <math.h>
 
 #include <type_traits>
@@ -205,10 +205,15 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             }
         }
     }
+    // Sums of weights up to 2^8 times values up to 6 * 2^125 pass float32.  Of fewer than 2^room rows they do not while a weight times a value's
+    // scale is below 2^(122 - room); a query that meets more has its reference 2^(10 + room) higher (lift), until its scores pass even that.
+    // (Not before: weights below 2^(room - 116) are lost then, which count where no other row's product is large.)
+    const int room = 32 - __builtin_clz(unsigned(n));
     f32x4 o[RT][DPL], ones[RT];   // ones: sums of the rounded weights
-    float m[RT];
+    float m[RT], lift[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+        lift[rt] = 0.0f;
 #pragma unroll
         for (int i = 0; i < DPL; ++i) o[rt][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         ones[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -260,7 +265,7 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             top[rt] = x[rt][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[rt] = fmaxf(top[rt], x[rt][e]);
-            any |= top[rt] > m[rt] + PASS;
+            any |= top[rt] > m[rt] + (PASS - lift[rt]);
         }
         if (__builtin_amdgcn_ballot_w64(any)) {
 #pragma unroll
@@ -268,7 +273,9 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
                 float t0 = fmaxf(top[rt], __shfl_xor(top[rt], 16, WAVE));
                 t0 = fmaxf(t0, __shfl_xor(t0, 32, WAVE));
                 // (each query by its own scores alone: no other query's change what it gets)
-                const float mn = t0 > m[rt] + PASS ? t0 : m[rt];
+                const bool passes = t0 > m[rt] + (PASS - lift[rt]);
+                if (t0 >= m[rt]) lift[rt] = 0.0f;   // (what was large is small now)
+                const float mn = passes ? t0 + lift[rt] : m[rt];
                 const float alpha = mn == NEG ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
                 m[rt] = mn;
 #pragma unroll
@@ -280,17 +287,11 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             }
         }
         // ---- weights
-        u32x4 pf[RT], pl[RT];   // to bf16, and what that leaves off
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const float shift = m[rt] == NEG ? 0.0f : m[rt];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[rt][e] = __builtin_amdgcn_exp2f(x[rt][e] - shift);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                pf[rt][e] = f32_to_bf16x2(x[rt][2 * e], x[rt][2 * e + 1]);
-                pl[rt][e] = f32_to_bf16x2(x[rt][2 * e] - bf16_lo(pf[rt][e]), x[rt][2 * e + 1] - bf16_hi(pf[rt][e]));
-            }
         }
         // ---- scales of the lane's eight keys: its block's byte of each row
         float sv[8];
@@ -303,6 +304,51 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             }
             sv[E] = mx_scale(w >> (8 * (ln * DPL / 32 % 4)) & 0xFFu);
         }, std::make_integer_sequence<int, 8>{});
+        // ---- large values, from 2^65 on: the two upper bits of a byte
+        uint32_t large = vs[0] & vs[0] << 1;
+        if constexpr (D == 256) large |= vs[1] & vs[1] << 1;
+        if (__builtin_amdgcn_ballot_w64((large & 0x80808080u) != 0)) {
+            uint32_t top = 0;   // the largest byte of the row that the lane holds (a NaN's is none)
+#pragma unroll
+            for (int i = 0; i < 4 * VW; ++i) {
+                const uint32_t byte = vs[i / 4] >> (8 * (i % 4)) & 0xFFu;
+                top = byte == 255 ? top : max(top, byte);
+            }
+            float most[8];   // the largest scale of the lane's keys
+            for_each([&](auto ec) __attribute__((always_inline)) {
+                constexpr int E = decltype(ec)::value;
+                most[E] = mx_scale(dpp<ROW_SHARE + E>(top));
+            }, std::make_integer_sequence<int, 8>{});
+            const float least = mx_scale(uint32_t(127 + 122 - room));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                bool meets = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) meets |= x[rt][e] * most[e] >= least;
+                const uint64_t b = __builtin_amdgcn_ballot_w64(meets && lift[rt] == 0.0f);
+                const uint64_t column = b | b >> 32;   // of the query's four lanes any
+                if (!((column | column >> 16) >> ln & 1)) continue;
+                lift[rt] = float(10 + room);
+                const float higher = m[rt] + lift[rt], down = __builtin_amdgcn_exp2f(m[rt] - higher);   // (m is finite: it has weights)
+                m[rt] = higher;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[rt][e] *= down;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) ones[rt][r] *= down;
+#pragma unroll
+                for (int i = 0; i < DPL; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[rt][i][r] *= down;
+            }
+        }
+        u32x4 pf[RT], pl[RT];   // the weights to bf16, and what that leaves off
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pf[rt][e] = f32_to_bf16x2(x[rt][2 * e], x[rt][2 * e + 1]);
+                pl[rt][e] = f32_to_bf16x2(x[rt][2 * e] - bf16_lo(pf[rt][e]), x[rt][2 * e + 1] - bf16_hi(pf[rt][e]));
+            }
         // ---- the tree's rows: a NaN must not reach (0 times NaN) the queries that do not see its row
         if (tail) {
             uint32_t bad = 0;
