@@ -53,11 +53,20 @@ __device__ __forceinline__ double half_away(double v) {   // of the lane half a 
     return __shfl_xor(v, 16, WAVE);
 }
 
+// Whether f lies in the middle of two bf16 numbers: only there does a float64's rounding to float decide the next one's.
+__device__ __forceinline__ bool tie(float f) { return (__float_as_uint(f) & 0xFFFFu) == 0x8000u; }
+// f, the float of v, and where that is such a middle and v is not its neighbour on v's side.
+__device__ __forceinline__ float beside(float f, double v) {
+    const double back = f;
+    const uint32_t b = __float_as_uint(f);
+    return !tie(f) || back == v ? f : __uint_as_float(fabs(back) > fabs(v) ? b - 1 : b + 1);
+}
+
 // One token per blockIdx.x.  A head of D values is held by D / 8 lanes, eight consecutive values each; four lanes hold a block of 32.  Per
 // head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
 // in float64 throughout: a float32 rounding before a code's lands on the other side of a border once in a million values, and a third of
-// the block's largest value off.  The angle in turns is off by 2^-53 of their number.
+// the block's largest value off (before a query's to bf16: once in a hundred thousand, by its last bit).  The angle in turns is off by 2^-53 of their number.
 template <int D, bool ACC>
 __global__ __launch_bounds__(CNT) void cache4_write_kernel(const Write4Args a) {
     constexpr int LPH = D / 8, GROUPS = CNT / LPH;
@@ -128,8 +137,19 @@ __global__ __launch_bounds__(CNT) void cache4_write_kernel(const Write4Args a) {
             }
             if (g < a.hq) {
                 u32x4 o;
+                float f[8];
+                bool ties = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = f32_to_bf16x2(float(v[2 * i]), float(v[2 * i + 1]));
+                for (int i = 0; i < 8; ++i) {
+                    f[i] = float(v[i]);
+                    ties |= tie(f[i]);
+                }
+                if (ties) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = beside(f[i], v[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = f32_to_bf16x2(f[2 * i], f[2 * i + 1]);
                 *reinterpret_cast<u32x4*>(a.q + (size_t(row) * a.hq + g) * D + 8 * j) = o;
                 continue;
             }
