@@ -10,6 +10,7 @@
 namespace scmx {
 
 constexpr int CNT = 256;
+constexpr unsigned WIDE = 1u << 22;   // workgroups of a launch in x at most (its threads in one dimension are below 2^32), the others in z
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct Write4Args {
@@ -62,7 +63,7 @@ __device__ __forceinline__ float beside(float f, double v) {
     return !tie(f) || back == v ? f : __uint_as_float(fabs(back) > fabs(v) ? b - 1 : b + 1);
 }
 
-// One token per blockIdx.x.  A head of D values is held by D / 8 lanes, eight consecutive values each; four lanes hold a block of 32.  Per
+// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each; four lanes hold a block of 32.  Per
 // head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
 // in float64 throughout: a float32 rounding before a code's lands on the other side of a border once in a million values, and a third of
@@ -71,7 +72,9 @@ template <int D, bool ACC>
 __global__ __launch_bounds__(CNT) void cache4_write_kernel(const Write4Args a) {
     constexpr int LPH = D / 8, GROUPS = CNT / LPH;
     __shared__ double s_sin[D / 2], s_cos[D / 2];
-    const int row = blockIdx.x, grp = threadIdx.x / LPH, j = threadIdx.x % LPH;
+    const unsigned token = blockIdx.z * gridDim.x + blockIdx.x;
+    if (token >= unsigned(a.L)) return;
+    const int row = int(token), grp = threadIdx.x / LPH, j = threadIdx.x % LPH;
     const int heads = a.hq + 2 * a.hk, stride = gridDim.y * GROUPS;
     const int64_t pos = a.pos_dev ? a.pos_dev[0] : a.pos0;
     const bool fits = pos >= 0 && pos <= int64_t(a.rows) - a.L;
@@ -162,14 +165,15 @@ __global__ __launch_bounds__(CNT) void cache4_write_kernel(const Write4Args a) {
     }
 }
 
-// 32 codes a lane, a block; blockIdx.y: KV head, blockIdx.z: K or V.
+// Eight values a lane, a word of codes; blockIdx.y: KV head, blockIdx.z % 2: K or V.
 __global__ __launch_bounds__(CNT) void cache4_read_kernel(const uint8_t* kc, const uint8_t* vc, const uint8_t* ks, const uint8_t* vs,
                                                           uint16_t* k, uint16_t* v, int d, int rows, int row0, int n) {
     const size_t first = size_t(blockIdx.y) * rows + row0;
-    const uint8_t* codes = (blockIdx.z ? vc : kc) + first * (d / 2);
-    const uint8_t* scales = (blockIdx.z ? vs : ks) + first * (d / 32);
-    uint16_t* out = (blockIdx.z ? v : k) + size_t(blockIdx.y) * n * d;
-    const size_t i = size_t(blockIdx.x) * CNT + threadIdx.x;   // of eight values
+    const bool is_v = blockIdx.z % 2;
+    const uint8_t* codes = (is_v ? vc : kc) + first * (d / 2);
+    const uint8_t* scales = (is_v ? vs : ks) + first * (d / 32);
+    uint16_t* out = (is_v ? v : k) + size_t(blockIdx.y) * n * d;
+    const size_t i = (size_t(blockIdx.z / 2) * gridDim.x + blockIdx.x) * CNT + threadIdx.x;   // of eight values
     if (i >= size_t(n) * (d / 8)) return;
     const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i];
     const float s = mx_scale(scales[i / 4]);
@@ -260,7 +264,8 @@ extern "C" int scmx_cache4_write(const int32_t* acc, const float* xscale, const 
                        cache_rows};
     const int groups = CNT / (d / 8), turns = (hq + 2 * hk + groups - 1) / groups;
     // a few tokens are spread over the CUs; a prompt fills them with a workgroup a token, which then takes the angles once
-    const dim3 grid(L, L >= 256 ? 1 : turns);
+    const unsigned x = std::min(unsigned(L), WIDE);
+    const dim3 grid(x, L >= 256 ? 1 : turns, (unsigned(L) + x - 1) / x);
     const hipStream_t st = (hipStream_t)stream;
     const auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
@@ -285,7 +290,8 @@ extern "C" int scmx_cache4_read(const uint8_t* kcache, const uint8_t* vcache, co
         return SCMX_ERR_ARG;
     }
     if (n == 0) return SCMX_OK;
-    const dim3 grid(unsigned((size_t(n) * (d / 8) + CNT - 1) / CNT), hk, 2);
+    const unsigned blocks = unsigned((size_t(n) * (d / 8) + CNT - 1) / CNT), x = std::min(blocks, WIDE);
+    const dim3 grid(x, hk, 2 * ((blocks + x - 1) / x));
     cache4_read_kernel<<<grid, dim3(CNT), 0, (hipStream_t)stream>>>(kcache, vcache, kscale, vscale, k, v, d, cache_rows, row0, n);
     return check_launch("cache4_read");
 }
