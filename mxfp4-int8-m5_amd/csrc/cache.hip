@@ -11,6 +11,7 @@
 namespace scmx {
 
 constexpr int CNT = 256;
+constexpr unsigned WIDE = 1u << 22;   // workgroups of a launch in x at most (its threads in one dimension are below 2^32), the others in z
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct WriteArgs {
@@ -54,7 +55,7 @@ __device__ __forceinline__ float partner(float v) {   // of the lane half a head
     return __shfl_xor(v, 16, WAVE);
 }
 
-// One token per blockIdx.x.  A head of D values is held by D / 8 lanes, eight consecutive values each: 16-byte loads, 16-byte
+// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each: 16-byte loads, 16-byte
 // (bf16) or 8-byte (codes) stores, the norm's sum and the row's maximum over the lanes of the group, and the partner of a
 // rotation half a group away at the same place.  Per head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
@@ -67,7 +68,9 @@ template <int D, bool EIGHT, bool ACC>
 __global__ __launch_bounds__(CNT) void cache_write_kernel(const WriteArgs a) {
     constexpr int LPH = D / 8, GROUPS = CNT / LPH;
     __shared__ float s_sin[D / 2], s_cos[D / 2];
-    const int row = blockIdx.x, grp = threadIdx.x / LPH, j = threadIdx.x % LPH;
+    const unsigned token = blockIdx.z * gridDim.x + blockIdx.x;
+    if (token >= unsigned(a.L)) return;
+    const int row = int(token), grp = threadIdx.x / LPH, j = threadIdx.x % LPH;
     const int heads = a.hq + 2 * a.hk, stride = gridDim.y * GROUPS;
     const int64_t pos = a.pos_dev ? a.pos_dev[0] : a.pos0;
     const bool fits = pos >= 0 && pos <= int64_t(a.rows) - a.L;
@@ -262,7 +265,8 @@ extern "C" int scmx_cache_write(const int32_t* acc, const float* xscale, const f
                       cache_rows};
     const int groups = CNT / (d / 8), turns = (hq + 2 * hk + groups - 1) / groups;
     // a few tokens are spread over the CUs; a prompt fills them with a workgroup a token, which then takes the angles once
-    const dim3 grid(L, L >= 256 ? 1 : turns);
+    const unsigned x = L < int(WIDE) ? unsigned(L) : WIDE;
+    const dim3 grid(x, L >= 256 ? 1 : turns, (unsigned(L) + x - 1) / x);
     const hipStream_t st = (hipStream_t)stream;
     const auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
