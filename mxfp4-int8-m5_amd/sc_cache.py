@@ -161,8 +161,9 @@ def cache_keep(caches, path, count, pos):
 
 
 def attn_tree_splits(T, n, hq, hk, d, bits=16):
-    """Ranges that n rows are cut into for T nodes."""
-    return (_lib.native().scmx_attn_tree4_splits if bits == 4 else _lib.native().scmx_attn_tree_splits)(T, n, hq, hk, d)
+    """Ranges that n rows are cut into for T nodes; bits as FusedQwen3.make_cache names them: 16, 8 or "mxfp4" (or 4)."""
+    _check(bits in (16, 8, 4, "mxfp4"), 'a cache has 16 or 8 bits, or is in "mxfp4"')
+    return (_lib.native().scmx_attn_tree4_splits if bits in (4, "mxfp4") else _lib.native().scmx_attn_tree_splits)(T, n, hq, hk, d)
 
 
 def attn_tree(q, kcache, vcache, pos, mask=None, kscale=None, vscale=None, scale=None, splits=None):
