@@ -22,23 +22,25 @@ extern "C" {
 #define SCMX_MX_F16 1
 #define SCMX_MX_F32 2
 
-/* x [M, K] of `type` (K <= 2^30), row i at element i * ldx (ldx >= K, any alignment), to codes and scales.  With nw (bf16 [K]; x bf16, K <= 16384):
- * of the rows' RMSNorm x / sqrt(mean(x^2) + eps) * nw, in float64, so that a value beside the border of two codes takes its own; there
- * byte is at least 10, and magnitudes from 2^128 on count as the largest below. */
+/* x [M, K] of `type` (K <= 2^30), row i at element i * ldx (ldx >= K, any alignment), to codes and scales.  With nw (bf16 [K]; x bf16,
+ * K <= 16384): of the rows' RMSNorm x / sqrt(mean(x^2) + eps) * nw, in float64, so that a value beside the border of two codes takes its
+ * own; there byte is at least 10, and magnitudes from 2^128 on count as the largest below. */
 int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M,
                      int K, void* stream);
 
 /* The values of M rows of K as bf16 or float32 (type; 16-byte aligned): exact but where they pass that type's range. */
 int scmx_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int type, int M, int K, void* stream);
 
-/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values (K <= 2^23, M and N < 2^31 - 511; N <= 2^26 where M <= 16 or M times K is below 512), on the scaled matrix instructions, sums in float32, each result rounded
- * once to bf16: epi 1: out [M, N]; 2: + res [M, N]; 3: silu(gate) * up of w rows in the order of the SwiGLU epilogue of scmx.h (two gates,
- * their two ups; N a multiple of 4), out [M, N / 2]. */
+/* x w^T of MXFP4 operands, x of M rows and w of N rows of K values, on the scaled matrix instructions, sums in float32, each result rounded
+ * once to bf16.  epi 1: out [M, N]; 2: + res [M, N]; 3: silu(gate) * up of w rows in the order of the SwiGLU epilogue of scmx.h (two gates,
+ * their two ups; N a multiple of 4), out [M, N / 2].
+ * K <= 2^23; M and N below 2^31 - 511 (any M where N times K is below 512); N <= 2^26 where M <= 16 or M times K is below 512; fewer than
+ * 2^31 groups of 16 x 16 results.  What is beyond is refused. */
 int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const uint8_t* wcodes, const uint8_t* wscales, const uint16_t* res,
                uint16_t* out, int epi, int M, int N, int K, void* stream);
 
-/* scmx_mx_quantize (bf16, with nw or without) and scmx_mx_mm in one call.  workspace: scmx_mx_linear_workspace(M, N, K, nw != NULL) bytes (0: none), 16-byte
- * aligned; it holds the rows' codes and scales between the call's launches. */
+/* scmx_mx_quantize (bf16, with nw or without) and scmx_mx_mm in one call.  workspace: scmx_mx_linear_workspace(M, N, K, nw != NULL) bytes
+ * (0: none), 16-byte aligned; it holds the rows' codes and scales between the call's launches. */
 size_t scmx_mx_linear_workspace(int M, int N, int K, int norm);
 int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw, float eps, const uint8_t* wcodes, const uint8_t* wscales,
                    const uint16_t* res, uint16_t* out, int epi, int M, int N, int K, void* workspace, size_t workspace_bytes,
@@ -63,10 +65,10 @@ int scmx_cache4_keep(const uint64_t* caches, int layers, int hk, int d, int cach
                      const int64_t* pos_dev, int64_t pos0, void* stream);
 
 /* scmx_attn_tree over such a cache.  q . K^T is taken to float32: q as two E4M3 parts a block of 32, whose sum differs from q by at most
- * 2^-23 of the block's largest value, times K as it is held.  The probabilities are held in 16 bits, as two bf16 parts, in the sum
- * and in the denominator alike (2^-15 of sum p |v| at most).  Values of any size: sums of 6 * 2^125 over 2^31 rows stay in float32; where a
- * query meets p |v| from 2^90 on, probabilities below 2^-80 of its largest may count as none.  A row's NaN reaches the nodes that see it and no other.  Scale bytes of rows that are read are at most 252, as
- * the append's are, or 255. */
+ * 2^-23 of the block's largest value, times K as it is held.  The probabilities are held in 16 bits, as two bf16 parts, in the sum and in
+ * the denominator alike (2^-15 of sum p |v| at most).  Values of any size: sums of 6 * 2^125 over 2^31 rows stay in float32; where a query
+ * meets p |v| from 2^90 on, probabilities below 2^-80 of its largest may count as none.  A row's NaN reaches the nodes that see it and no
+ * other.  Scale bytes of rows that are read are at most 252, as the append's are, or 255. */
 int scmx_attn_tree4_splits(int T, int n, int hq, int hk, int d);
 int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const uint8_t* vcache, const uint8_t* kscale, const uint8_t* vscale,
                     const int64_t* mask, const int64_t* pos_dev, int64_t pos0, uint16_t* out, int T, int hq, int hk, int d,

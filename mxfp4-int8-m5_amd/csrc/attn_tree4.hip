@@ -1,19 +1,20 @@
-// Attention of a tree of drafted tokens (1..64 of them, one: a decode step) against a KV cache in 4 bits (include/scmx_mx.h, scmx_attn_tree4).
+// Attention of a tree of drafted tokens (1..64 of them, one: a decode step) against a KV cache in 4 bits (include/scmx_mx.h,
+// scmx_attn_tree4).
 //
 // As over bf16 and 8-bit caches (attn_tree.hip): the query heads of a KV head and their tokens are the rows of one matrix product, a wave
-// owns 16 or 32 of them and walks tiles of 32 keys with a running reference, both products are transposed so that a query is a lane column in both
-// and the scores' accumulators are the second product's operand where they are, and nothing is staged.
+// owns 16 or 32 of them and walks tiles of 32 keys with a running reference, both products are transposed so that a query is a lane
+// column in both and the scores' accumulators are the second product's operand where they are, and nothing is staged.
 //
 // S^T = K Q^T runs on the scaled matrix instruction 16x16x128, the K codes and their bytes as they lie in the cache: no conversion.  The
-// queries are its other operand in E4M3, as two parts: hi, rounded to four bits, with the block's exponent, and lo, what is left
-// (exact in four bits more: q has eight), with an exponent 5 lower.  Both are exact for values down to 2^-14 of the block's largest, below that
+// queries are its other operand in E4M3, as two parts: hi, rounded to four bits, with the block's exponent, and lo, what is left (exact
+// in four bits more: q has eight), with an exponent 5 lower.  Both are exact for values down to 2^-14 of the block's largest, below that
 // their sum is off by at most 2^-23 of it.  64 dimensions take both parts in one instruction (K twice), 128 an instruction each, 256 two.
-// The instruction's E2M1 operand is 32 consecutive values a lane (lane group g: 32 g ..), its E4M3 operand 16 g .. and 64 + 16 g ..; a byte
-// belongs to the 32 values from 32 g on in both.
+// The instruction's E2M1 operand is 32 consecutive values a lane (lane group g: 32 g ..), its E4M3 operand 16 g .. and 64 + 16 g ..; a
+// byte belongs to the 32 values from 32 g on in both.
 // O^T = V^T P^T in bf16: a lane reads DPL = d / 16 consecutive codes of eight V rows, the conversion applies the row's block scale (exact
-// in bf16), byte permutes pair the rows.  The weights are two bf16 parts, what rounds to bf16 and what is left, 16 bits in all, and each product
-// is two: in one part (2^-8) the weights' rounding was as large as the result's, and larger where values cancel.  One token over 300 / 40000 rows
-// of 16:8 x 128 6.3 / 13.1 us, 64 tokens over 6000 of 32:8 x 128 20.6 (in one part 6.0 / 12.6 / 18.6).
+// in bf16), byte permutes pair the rows.  The weights are two bf16 parts, what rounds to bf16 and what is left, 16 bits in all, and each
+// product is two: in one part (2^-8) the weights' rounding was as large as the result's, and larger where values cancel.  One token over
+// 300 / 40000 rows of 16:8 x 128 6.3 / 13.1 us, 64 tokens over 6000 of 32:8 x 128 20.6 (in one part 6.0 / 12.6 / 18.6).
 #include <math.h>
 
 #include <type_traits>
@@ -59,7 +60,8 @@ __device__ __forceinline__ uint32_t split_e4m3(const u32x4 (&q)[2], uint32_t (&h
         h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[4 * i], x[4 * i + 1], s, false);
         h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[4 * i + 2], x[4 * i + 3], s, true);
         hi[i] = __builtin_bit_cast(uint32_t, h);
-        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, true);
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, false);
+        const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, true);
         l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[4 * i] - a[0], x[4 * i + 1] - a[1], sl, false);
         l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[4 * i + 2] - b[0], x[4 * i + 3] - b[1], sl, true);
         lo[i] = __builtin_bit_cast(uint32_t, l);
@@ -205,9 +207,9 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             }
         }
     }
-    // Sums of weights up to 2^8 times values up to 6 * 2^125 pass float32.  Of fewer than 2^room rows they do not while a weight times a value's
-    // scale is below 2^(122 - room); a query that meets more has its reference 2^(10 + room) higher (lift), until its scores pass even that.
-    // (Not before: weights below 2^(room - 116) are lost then, which count where no other row's product is large.)
+    // Sums of weights up to 2^8 times values up to 6 * 2^125 pass float32.  Of fewer than 2^room rows they do not while a weight times a
+    // value's scale is below 2^(122 - room); a query that meets more has its reference 2^(10 + room) higher (lift), until its scores pass
+    // even that.  (Not before: weights below 2^(room - 116) are lost then, which count where no other row's product is large.)
     const int room = 32 - __builtin_clz(unsigned(n));
     f32x4 o[RT][DPL], ones[RT];   // ones: sums of the rounded weights
     float m[RT], lift[RT];
@@ -236,8 +238,8 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
                 const i32x8 kf = {int(c[0]), int(c[1]), int(c[2]), int(c[3]), 0, 0, 0, 0};
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    s[rt][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[rt][qn], s[rt][h], FP4, FP8, 0, int(ks[h][qn / 2]), 0,
-                                                                                 qs[rt][qn]);
+                    s[rt][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qf[rt][qn], s[rt][h], FP4, FP8, 0,
+                                                                                 int(ks[h][qn / 2]), 0, qs[rt][qn]);
             }
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
@@ -389,7 +391,8 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
             u32x4 w0, w1;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t lo = mx_bf16x2<B % 4>(vr[2 * e][B / 4], sv[2 * e]), hi = mx_bf16x2<B % 4>(vr[2 * e + 1][B / 4], sv[2 * e + 1]);
+                const uint32_t lo = mx_bf16x2<B % 4>(vr[2 * e][B / 4], sv[2 * e]);
+                const uint32_t hi = mx_bf16x2<B % 4>(vr[2 * e + 1][B / 4], sv[2 * e + 1]);
                 w0[e] = perm(hi, lo, 0x05040100u);
                 w1[e] = perm(hi, lo, 0x07060302u);
             }
@@ -433,7 +436,8 @@ __global__ __launch_bounds__(TNT, 2) void attn_tree4_kernel(const Tree4Args a) {
         float f = ones[rt][0] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - mx);
         if (whole) f *= sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);   // (0: nothing was seen)
         else if (wave == 0 && g == 0 && row0 + r < rows_all)
-            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) = float2{mx, sum};
+            *reinterpret_cast<float2*>(a.part + size_t(a.T) * a.hq * a.splits * D + 2 * (out_row(row0 + r) * a.splits + range)) =
+                float2{mx, sum};
         if (row0 + r < rows_all) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
@@ -478,19 +482,20 @@ extern "C" int scmx_attn_tree4_splits(int T, int n, int hq, int hk, int d) {
     if (T < 1 || T > 64 || n < 1 || hq < 1 || hk < 1 || hq > 65535 || hq % hk || (d != 64 && d != 128 && d != 256)) return 1;
     const int qrows = T * (hq / hk), rt = tree4_blocks(qrows, d), tiles = tiles_of(n);
     if (tiles <= TONE) return 1;
-    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, whose join reads half as much.  Two workgroups a
-    // CU where a wave has eight tiles and more: one token of 16:8 x 128, 16 / 32 / 64 ranges, 3000 rows 7.6 / 8.0 / -, 10000 9.8 / 9.0 / 9.1, 40000
-    // 25.3 / 16.9 / 14.3 us; 64 tokens of 32:8 x 128, 6000 rows, 4 / 8 / 16 ranges 18.7 / 18.2 / 28.8.  Eight waves a workgroup: 40000 rows 14.4 with
-    // 32 ranges, 15.2 with 64, 16 tokens of 3000 rows 12.1 (four 10.8), one range of 300 rows 5.9 (6.1), of 500 6.9 (6.6).
+    // A workgroup a CU, a tile a wave; up to 32 ranges of one tile a wave are 16 of two instead, whose join reads half as much.  Two
+    // workgroups a CU where a wave has eight tiles and more.  us in a graph: one token of 16:8 x 128, 16 / 32 / 64 ranges, 3000 rows 7.9 /
+    // 8.2 / -, 10000 9.7 / 8.9 / 9.3, 40000 23.2 / 16.1 / 13.8; 64 tokens of 32:8 x 128, 6000 rows, 4 / 8 / 16 ranges 21.4 / 21.6 / 32.0.
+    // Eight waves a workgroup (with weights in one part, where four took a few per cent less than now): 40000 rows 14.4 with 32 ranges,
+    // 15.2 with 64, 16 tokens of 3000 rows 12.1 (four 10.8), one range of 300 rows 5.9 (6.1), of 500 6.9 (6.6).
     const int64_t groups = int64_t(hk) * ((qrows + 16 * rt - 1) / (16 * rt)), one = 256 / groups;
     const int64_t most = tiles >= 8 * TWAVES * one ? 512 / groups : one;
     const int even = (tiles + TWAVES - 1) / TWAVES, ranges = even > 16 && even <= 32 ? 16 : even < 64 ? even : 64;
     return most < 1 ? 1 : ranges < most ? ranges : int(most);
 }
 
-extern "C" int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const uint8_t* vcache, const uint8_t* kscale, const uint8_t* vscale,
-                               const int64_t* mask, const int64_t* pos_dev, int64_t pos0, uint16_t* out, int T, int hq, int hk, int d,
-                               int cache_rows, float scale, float* workspace, int splits, void* stream) {
+extern "C" int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const uint8_t* vcache, const uint8_t* kscale,
+                               const uint8_t* vscale, const int64_t* mask, const int64_t* pos_dev, int64_t pos0, uint16_t* out, int T,
+                               int hq, int hk, int d, int cache_rows, float scale, float* workspace, int splits, void* stream) {
     if (!q || !kcache || !vcache || !out || !kscale || !vscale) {
         set_error("attn_tree4: null pointer argument");
         return SCMX_ERR_ARG;
@@ -512,7 +517,8 @@ extern "C" int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const u
         set_error("attn_tree4: scale must be finite, times log2 e too");
         return SCMX_ERR_ARG;
     }
-    if ((uintptr_t(q) | uintptr_t(kcache) | uintptr_t(vcache) | uintptr_t(out)) % 16 || (uintptr_t(kscale) | uintptr_t(vscale)) % (d / 32)) {
+    if ((uintptr_t(q) | uintptr_t(kcache) | uintptr_t(vcache) | uintptr_t(out)) % 16 ||
+        (uintptr_t(kscale) | uintptr_t(vscale)) % (d / 32)) {
         set_error("attn_tree4: q, out and the caches must be 16-byte aligned, scales to a row's bytes");
         return SCMX_ERR_ARG;
     }
@@ -523,8 +529,8 @@ extern "C" int scmx_attn_tree4(const uint16_t* q, const uint8_t* kcache, const u
     const int qrows = T * (hq / hk), rt = tree4_blocks(qrows, d);
     const uint32_t by_group = uint32_t(((uint64_t(1) << 32) + hq / hk - 1) / uint64_t(hq / hk));
     Tree4Args a;
-    static_cast<TreeArgs&>(a) = TreeArgs{q, kcache, vcache, nullptr, nullptr, mask, pos_dev, pos0, out, workspace, T, hq, hk, cache_rows, splits,
-                                         (qrows + 16 * rt - 1) / (16 * rt), by_group, scale * 1.4426950408889634f};
+    static_cast<TreeArgs&>(a) = TreeArgs{q, kcache, vcache, nullptr, nullptr, mask, pos_dev, pos0, out, workspace, T, hq, hk, cache_rows,
+                                         splits, (qrows + 16 * rt - 1) / (16 * rt), by_group, scale * 1.4426950408889634f};
     a.ksb = kscale;
     a.vsb = vscale;
     const hipStream_t st = (hipStream_t)stream;

@@ -55,9 +55,9 @@ __device__ __forceinline__ float partner(float v) {   // of the lane half a head
     return __shfl_xor(v, 16, WAVE);
 }
 
-// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each: 16-byte loads, 16-byte
-// (bf16) or 8-byte (codes) stores, the norm's sum and the row's maximum over the lanes of the group, and the partner of a
-// rotation half a group away at the same place.  Per head (x: the row, n: its norm)
+// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each:
+// 16-byte loads, 16-byte (bf16) or 8-byte (codes) stores, the norm's sum and the row's maximum over the lanes of the group, and the
+// partner of a rotation half a group away at the same place.  Per head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
 // The angle is formed and reduced to one turn in float64: in float32 a position of 100000 is off by 4e-3 of a radian, as much as
 // the result's rounding.  Everything else is float32 and rounded once, to bf16 or to a code.

@@ -63,11 +63,12 @@ __device__ __forceinline__ float beside(float f, double v) {
     return !tie(f) || back == v ? f : __uint_as_float(fabs(back) > fabs(v) ? b - 1 : b + 1);
 }
 
-// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each; four lanes hold a block of 32.  Per
-// head (x: the row, n: its norm)
+// One token per blockIdx.x (and z, from WIDE tokens on).  A head of D values is held by D / 8 lanes, eight consecutive values each; four
+// lanes hold a block of 32.  Per head (x: the row, n: its norm)
 //     n = x / sqrt(mean(x^2) + eps) * w,  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq
 // in float64 throughout: a float32 rounding before a code's lands on the other side of a border once in a million values, and a third of
-// the block's largest value off (before a query's to bf16: once in a hundred thousand, by its last bit).  The angle in turns is off by 2^-53 of their number.
+// the block's largest value off (before a query's to bf16: once in a hundred thousand, by its last bit).  The angle in turns is off by
+// 2^-53 of their number.
 template <int D, bool ACC>
 __global__ __launch_bounds__(CNT) void cache4_write_kernel(const Write4Args a) {
     constexpr int LPH = D / 8, GROUPS = CNT / LPH;
@@ -245,7 +246,8 @@ extern "C" int scmx_cache4_write(const int32_t* acc, const float* xscale, const 
                                  const uint16_t* kn, float eps, uint16_t* q, uint8_t* kcache, uint8_t* vcache, uint8_t* kscale,
                                  uint8_t* vscale, int L, int hq, int hk, int d, const float* inv_freq, const int32_t* depth,
                                  const int64_t* pos_dev, int64_t pos0, int cache_rows, void* stream) {
-    if ((L && ((!acc && !y) || !q)) || (acc && (!xscale || !wscale)) || !qn || !kn || !kcache || !vcache || !inv_freq || !kscale || !vscale) {
+    if ((L && ((!acc && !y) || !q)) || (acc && (!xscale || !wscale)) || !qn || !kn || !kcache || !vcache || !inv_freq || !kscale ||
+        !vscale) {
         set_error("cache4_write: null pointer argument");
         return SCMX_ERR_ARG;
     }
@@ -260,8 +262,8 @@ extern "C" int scmx_cache4_write(const int32_t* acc, const float* xscale, const 
         return SCMX_ERR_ARG;
     }
     if (L == 0) return SCMX_OK;
-    const Write4Args a{acc, xscale, wscale, y, qn, kn, eps, q, {kcache, vcache}, {kscale, vscale}, L, hq, hk, inv_freq, depth, pos_dev, pos0,
-                       cache_rows};
+    const Write4Args a{acc, xscale,   wscale, y,     qn,      kn,   eps,       q, {kcache, vcache}, {kscale, vscale}, L, hq,
+                       hk,  inv_freq, depth,  pos_dev, pos0, cache_rows};
     const int groups = CNT / (d / 8), turns = (hq + 2 * hk + groups - 1) / groups;
     // a few tokens are spread over the CUs; a prompt fills them with a workgroup a token, which then takes the angles once
     const unsigned x = std::min(unsigned(L), WIDE);
@@ -296,8 +298,8 @@ extern "C" int scmx_cache4_read(const uint8_t* kcache, const uint8_t* vcache, co
     return check_launch("cache4_read");
 }
 
-extern "C" int scmx_cache4_keep(const uint64_t* caches, int layers, int hk, int d, int cache_rows, const int32_t* path, const int32_t* count,
-                                int T, const int64_t* pos_dev, int64_t pos0, void* stream) {
+extern "C" int scmx_cache4_keep(const uint64_t* caches, int layers, int hk, int d, int cache_rows, const int32_t* path,
+                                const int32_t* count, int T, const int64_t* pos_dev, int64_t pos0, void* stream) {
     if (!caches || !path || !count) {
         set_error("cache4_keep: null pointer argument");
         return SCMX_ERR_ARG;
@@ -326,7 +328,8 @@ extern "C" int scmx_cache4_keep(const uint64_t* caches, int layers, int hk, int 
         for (int l = 0; l < n; ++l)
             for (int i = 0; i < 4; ++i) a.t[l][i] = reinterpret_cast<uint8_t*>(uintptr_t(caches[size_t(l0 + l) * 4 + i]));
         const auto go = [&](auto dim) {
-            cache4_keep_kernel<decltype(dim)::value><<<dim3(hk, 2, n), dim3(CNT), 0, (hipStream_t)stream>>>(a, cache_rows, path, count, T, pos_dev, pos0);
+            cache4_keep_kernel<decltype(dim)::value>
+                <<<dim3(hk, 2, n), dim3(CNT), 0, (hipStream_t)stream>>>(a, cache_rows, path, count, T, pos_dev, pos0);
         };
         if (d == 64) go(std::integral_constant<int, 64>{});
         else if (d == 128) go(std::integral_constant<int, 128>{});

@@ -51,9 +51,9 @@ __device__ __forceinline__ uint32_t mx_codes_bf16(u32x4 x, uint32_t byte) {
     return byte == 255 ? 0 : w;
 }
 
-// Values in float64 (a norm's, a rotation's) go through a float rounded to odd (cut off, the last bit set if anything was), so that none lands
-// on the border of two codes that was beside it.  Magnitudes are held to 2^-120 .. 2^128 on the way, and the byte to 10 and above, below
-// which 2^-120 would count.
+// Values in float64 (a norm's, a rotation's) go through a float rounded to odd (cut off, the last bit set if anything was), so that none
+// lands on the border of two codes that was beside it.  Magnitudes are held to 2^-120 .. 2^128 on the way, and the byte to 10 and above,
+// below which 2^-120 would count.
 __device__ __forceinline__ uint32_t high(double v) { return uint32_t(__builtin_bit_cast(uint64_t, v) >> 32); }
 __device__ __forceinline__ float odd_float(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -62,8 +62,8 @@ __device__ __forceinline__ float odd_float(double v) {
     const uint32_t cut = ((m << 3) | (lo >> 29)) + 0x40000000u;   // the exponent less 896, to float's
     return __uint_as_float((hi & 0x80000000u) | cut | uint32_t((lo & 0x1FFFFFFFu) != 0));
 }
-// The byte for the largest magnitude's upper word: exponent fields, float64's less 1023, less 2, plus 127; at most 252 (2^125, of which 6 is
-// below 2^128).
+// The byte for the largest magnitude's upper word: exponent fields, float64's less 1023, less 2, plus 127; at most 252 (2^125, of which 6
+// is below 2^128).
 __device__ __forceinline__ uint32_t mx_byte_f64(uint32_t top) {
     return top >= 0x7FF00000u ? 255 : min(max(top >> 20, 898u + 10u) - 898u, 252u);
 }

@@ -1,6 +1,6 @@
-// Products of MXFP4 operands (include/scmx_mx.h, scmx_mx_mm and scmx_mx_linear) on the scaled matrix instructions: v_mfma_scale_f32_16x16x128,
-// both operands E2M1 with an E8M0 byte for 32 values, sums in float32.  The weights are the row operand, so that a lane's
-// accumulators are groups of four consecutive columns n of one row m, two gates and their two ups among them.
+// Products of MXFP4 operands (include/scmx_mx.h, scmx_mx_mm and scmx_mx_linear) on the scaled matrix instructions:
+// v_mfma_scale_f32_16x16x128, both operands E2M1 with an E8M0 byte for 32 values, sums in float32.  The weights are the row operand, so
+// that a lane's accumulators are groups of four consecutive columns n of one row m, two gates and their two ups among them.
 //
 // A lane's operand is 16 bytes of codes, one block of 32 values, with the block's byte beside it.  Which blocks
 // of K meet in an instruction is free, as long as both operands take the same.
@@ -36,15 +36,17 @@ template <int EPI>
 __device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
     if (m >= a.M) return;
     if constexpr (EPI == 3) {
-        if (n < a.N) *reinterpret_cast<uint32_t*>(a.out + (size_t(m) * a.N + n) / 2) = f32_to_bf16x2(silu_mul(v[0], v[2]), silu_mul(v[1], v[3]));
+        if (n < a.N)
+            *reinterpret_cast<uint32_t*>(a.out + (size_t(m) * a.N + n) / 2) = f32_to_bf16x2(silu_mul(v[0], v[2]), silu_mul(v[1], v[3]));
     } else {
         const size_t at = size_t(m) * a.N + n;
         if (a.N % 4 == 0) {
             if (n >= a.N) return;
-            u32x2 r = {0, 0};
-            if constexpr (EPI == 2) r = *reinterpret_cast<const u32x2*>(a.res + at);
-            *reinterpret_cast<u32x2*>(a.out + at) = EPI == 2 ? u32x2{f32_to_bf16x2(v[0] + bf16_lo(r[0]), v[1] + bf16_hi(r[0])), f32_to_bf16x2(v[2] + bf16_lo(r[1]), v[3] + bf16_hi(r[1]))}
-                                                             : u32x2{f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3])};
+            if constexpr (EPI == 2) {
+                const u32x2 r = *reinterpret_cast<const u32x2*>(a.res + at);
+                v = f32x4{v[0] + bf16_lo(r[0]), v[1] + bf16_hi(r[0]), v[2] + bf16_lo(r[1]), v[3] + bf16_hi(r[1])};
+            }
+            *reinterpret_cast<u32x2*>(a.out + at) = u32x2{f32_to_bf16x2(v[0], v[1]), f32_to_bf16x2(v[2], v[3])};
             return;
         }
 #pragma unroll
@@ -53,8 +55,8 @@ __device__ __forceinline__ void store4(const MxArgs& a, int m, int n, f32x4 v) {
     }
 }
 
-// Columns n .. n + 7 (SwiGLU: n + 15) of row m, all inside, in one store of eight values; a row starts at any even address (the hardware takes
-// vectors at them).
+// Columns n .. n + 7 (SwiGLU: n + 15) of row m, all inside, in one store of eight values; a row starts at any even address (the hardware
+// takes vectors at them).
 template <int EPI>
 __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float* v) {
     const size_t at = EPI == 3 ? (size_t(m) * a.N + n) / 2 : size_t(m) * a.N + n;
@@ -69,10 +71,11 @@ __device__ __forceinline__ void store(const MxArgs& a, int m, int n, const float
     *reinterpret_cast<u32x4u*>(a.out + at) = w;
 }
 
-// Few rows: a workgroup per 16 columns (8 where the workgroups would be too few: half of a fragment's columns are none then) and 16 rows.  BLOCKS
-// of K at a time, the rows' codes come to LDS, as they are or made of bf16 rows (a thread takes a block of 32, 64 bytes, and needs no other's
-// values), and the waves take steps of 128 side by side, the weights straight from memory, requested before the rows.  The waves meet in
-// LDS.  Bound by reading the weights where there are many (16384 x 8192 20.3 us, 3.5 TB/s), by the launch and a trip to memory where there are few.
+// Few rows: a workgroup per 16 columns (8 where the workgroups would be too few: half of a fragment's columns are none then) and 16
+// rows.  BLOCKS of K at a time, the rows' codes come to LDS, as they are or made of bf16 rows (a thread takes a block of 32, 64 bytes,
+// and needs no other's values), and the waves take steps of 128 side by side, the weights straight from memory, requested before the
+// rows.  The waves meet in LDS.  Bound by reading the weights where there are many (16384 x 8192 17.9-19.1 us, 3.7-4.0 TB/s), by the
+// launch and a trip to memory where there are few.
 constexpr int FEW_WAVES = 8;
 
 struct FewArgs : MxArgs {
@@ -139,7 +142,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void mx_few_kernel(const FewArgs a)
             if (u >= per) break;
             const int c = min(4 * (first + u) + g, blocks - 1);   // (behind the end: a block that meets zeros, its byte with them)
             const uint32_t sx = 4 * (first + u) + g < blocks ? s_xs[row][c] : 0;
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc[u]), operand(s_x[row][c]), acc, FP4, FP4, 0, int(sw[u]), 0, int(sx));
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(wc[u]), operand(s_x[row][c]), acc, FP4, FP4, 0, int(sw[u]), 0,
+                                                                   int(sx));
         }
     }
     s_acc[wave][lane] = acc;
@@ -185,11 +189,11 @@ __device__ __forceinline__ void multiply(f32x4& acc, u32x4 w, u32x4 x, int sw, i
 __device__ __forceinline__ void settle() { asm volatile("s_nop 1"); }
 __device__ __forceinline__ void done() { asm volatile("s_nop 15\n\ts_nop 3"); }
 
-// Many rows: workgroups of 2 x 2 waves take BM x BN tiles in turn.  A stage is 256 of K: BN + BM rows of 128 bytes of codes, loaded into LDS past
-// the registers, 16 bytes a lane; chunk c (a block of 32) of row r sits at chunk (c % 2 * 4 + c / 2) ^ (r / 2 % 8), so that a fragment's
-// lanes find theirs in different banks.  Rows and blocks behind the operands' ends are out of the buffers' bounds and come as zeros.  In
-// step s of a stage's two, lane group g takes block 2 g + s, so that its bytes lie side by side.  The bytes of four stages come together,
-// 32 a row.
+// Many rows: workgroups of 2 x 2 waves take BM x BN tiles in turn.  A stage is 256 of K: BN + BM rows of 128 bytes of codes, loaded into
+// LDS past the registers, 16 bytes a lane; chunk c (a block of 32) of row r sits at chunk (c % 2 * 4 + c / 2) ^ (r / 2 % 8), so that a
+// fragment's lanes find theirs in different banks.  Rows and blocks behind the operands' ends are out of the buffers' bounds and come as
+// zeros.  In step s of a stage's two, lane group g takes block 2 g + s, so that its bytes lie side by side.  The bytes of four stages
+// come together, 32 a row.
 //
 // Two stages: half way through one, its second step's fragments are in registers and the next stage has arrived (one barrier says both);
 // its place is loaded with the stage after the next, of the next tile too, while the second step multiplies, and the next stage's first
@@ -203,7 +207,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
     constexpr int TI = BN / 2 / 16, TJ = BM / 2 / 16;   // a wave's blocks of 16 columns n, of 16 rows m
     constexpr int SROWS = ROWS * 32, READS = TI + TJ, Q = EPI == 3 ? 4 : 2;
     constexpr int STORES = TI / Q * TJ;                 // a wave's stores of a whole tile
-    static_assert((BM == 32 || BM % 64 == 0) && BM <= 256 && BN % 128 == 0 && BN <= 256, "a wave loads whole pieces of one operand and holds 64 columns' fragments");
+    static_assert((BM == 32 || BM % 64 == 0) && BM <= 256 && BN % 128 == 0 && BN <= 256,
+                  "a wave loads whole pieces of one operand and holds 64 columns' fragments");
     static_assert(READS == LOADS && STORES < 64, "as many fragments a step as pieces a stage; a counter of six bits");
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE], s_scale[2 * SROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
@@ -211,8 +216,14 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
     // In a round of all workgroups a run of tiles to each XCD (workgroups are dealt to them in turn), in strips of eight tile rows
     const int all = tiles_m * tiles_n, grid = int(gridDim.x), b = int(blockIdx.x);
     const int mine = grid % 8 == 0 ? b % 8 * (grid / 8) + b / 8 : b;
-    const auto tile_m = [&](int o) { const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip); return (8 * strip + (o - strip * 8 * tiles_n) % high) * BM; };
-    const auto tile_n = [&](int o) { const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip); return (o - strip * 8 * tiles_n) / high * BN; };
+    const auto tile_m = [&](int o) {
+        const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip);
+        return (8 * strip + (o - strip * 8 * tiles_n) % high) * BM;
+    };
+    const auto tile_n = [&](int o) {
+        const int strip = o / (8 * tiles_n), high = min(8, tiles_m - 8 * strip);
+        return (o - strip * 8 * tiles_n) / high * BN;
+    };
     const int nb = a.K / 32, stages = (nb + 7) / 8;
     // row p of LDS: which row of its operand's part of the tile
     const auto source = [](int p) { return p < BN ? p / (16 * Q) * (16 * Q) + p % 16 / 4 * (4 * Q) + p / 16 % Q * 4 + p % 4 : p - BN; };
@@ -221,7 +232,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
     const unsigned codes_at = lds_offset(smem), scales_at = lds_offset(s_scale), row_bytes = unsigned(nb) * 16u;
     // pieces of eight rows, wave's wave + 4 i; the lane's 16 bytes in a row of each
     const int r8 = lane / 8, slot = (lane % 8) ^ (4 * (wave & 1) + r8 / 2), chunk = slot % 4 * 2 + slot / 4;
-    const unsigned wlane = unsigned(source(8 * wave + r8)) * row_bytes + 16u * chunk, xlane = unsigned(8 * wave + r8) * row_bytes + 16u * chunk;
+    const unsigned wlane = unsigned(source(8 * wave + r8)) * row_bytes + 16u * chunk;
+    const unsigned xlane = unsigned(8 * wave + r8) * row_bytes + 16u * chunk;
     // of scales waves 0 and 1 bring the weights', 2 and 3 the rows', 32 rows a piece
     const bool of_w = wave < 2;
     const int odd = of_w || BM > 32 ? wave & 1 : 0;
@@ -261,7 +273,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
                 load_lds16(sbuf, scales_at + to, (slane + 8u * l + part * 64u * unsigned(nb)) | behind(c));
             } else {
                 const int rows = of_w ? a.N : a.M, row = min((of_w ? tile_n(lo) : tile_m(lo)) + 64 * part + row0, rows - 1);
-                const int64_t first = int64_t(row) * nb + c, at = min(first, int64_t(rows) * nb - 16);   // (the last 16 hold the last bytes)
+                const int64_t first = int64_t(row) * nb + c;
+                const int64_t at = min(first, int64_t(rows) * nb - 16);   // (the last 16 hold the last bytes)
                 held[part] = *reinterpret_cast<const u32x4b*>((of_w ? a.ws : a.xs) + at);
                 over[part] = int(min(first - at, int64_t(16)));
             }
@@ -371,7 +384,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
             // the stage after it into this one's place; the next one's first fragments
             const int next = t + 1 < stages ? t + 1 : 0;
             if (next % 4 == 0) quad ^= 1;
-            step(std::integral_constant<int, 1>{}, std::integral_constant<int, LOADS + 1 + 2 * READS>{}, [&](int i) __attribute__((always_inline)) {
+            constexpr std::integral_constant<int, LOADS + 1 + 2 * READS> items;
+            step(std::integral_constant<int, 1>{}, items, [&](int i) __attribute__((always_inline)) {
                 if (i < 2 * LOADS) {
                     if (i % 2 == 0) load(place, i / 2);
                     else read(place ^ 1, i / 2, 0);
@@ -410,7 +424,8 @@ __global__ __launch_bounds__(256, 1) void mx_tile_kernel(const MxArgs a, int til
 #pragma unroll
             for (int j = 0; j < TJ; ++j) {
 #pragma unroll
-                for (int i = 0; i < TI; ++i) store4<EPI>(a, m0 + (wm * TJ + j) * 16 + ln, n0 + source((wn * TI + i) * 16 + 4 * g), acc[i][j]);
+                for (int i = 0; i < TI; ++i)
+                    store4<EPI>(a, m0 + (wm * TJ + j) * 16 + ln, n0 + source((wn * TI + i) * 16 + 4 * g), acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -429,16 +444,19 @@ static void few(const FewArgs& a, hipStream_t st) {
     const unsigned down = (unsigned(a.M) + 15) / 16, z = (down + 65534) / 65535;
     mx_few_kernel<COLS, BLOCKS><<<dim3((unsigned(a.N) + COLS - 1) / COLS, (down + z - 1) / z, z), dim3(64 * FEW_WAVES), 0, st>>>(a);
 }
-// Eight columns where that leaves no CU two workgroups.  us with 16 columns and 128 blocks / 16 and 256 / 8 and 256: one row of 12288 x 2048 4.9 / 6.9 /
-// 7.7, of 16384 x 8192 20.1 / 17.9 / 20.0, of 4096 x 4096 4.1 / 4.2 / 4.5, of 2944 x 6752 4.3 / 4.2 / 4.9, of 2048 x 8192 6.1 / 5.9 / 4.5, 16 rows of 12288 x
-// 2048 5.6 / 7.7 / 9.0, of 2048 x 8192 7.8 / 7.8 / 6.7.  16 waves: between these; 64 blocks: no better.
+// Eight columns where that leaves no CU two workgroups.  us with 16 columns and 128 blocks / 16 and 256 / 8 and 256: one row of 12288 x
+// 2048 4.9 / 6.9 / 7.7, of 16384 x 8192 20.1 / 17.9 / 20.0, of 4096 x 4096 4.1 / 4.2 / 4.5, of 2944 x 6752 4.3 / 4.2 / 4.9, of 2048 x
+// 8192 6.1 / 5.9 / 4.5, 16 rows of 12288 x 2048 5.6 / 7.7 / 9.0, of 2048 x 8192 7.8 / 7.8 / 6.7.  16 waves: between these; 64 blocks: no
+// better.
 static void launch_few(const FewArgs& a, hipStream_t st) {
     if ((int64_t(a.N) + 15) / 16 * ((int64_t(a.M) + 15) / 16) <= device_cus() / 2) few<8, 256>(a, st);
     else if (a.K > 4096) few<16, 256>(a, st);
     else few<16, 128>(a, st);
 }
 // Whether every row's bytes are whole words.
-static bool words(const MxArgs& a) { return a.K % 128 == 0 && (reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) % 4 == 0; }
+static bool words(const MxArgs& a) {
+    return a.K % 128 == 0 && (reinterpret_cast<uintptr_t>(a.xs) | reinterpret_cast<uintptr_t>(a.ws)) % 4 == 0;
+}
 
 template <int BM, int BN>
 static void launch_tile(const MxArgs& a, hipStream_t st) {
@@ -460,7 +478,8 @@ constexpr int FEW = 16;   // rows up to which they are few
 
 static int check_mm(const char* who, const void* w, const void* ws, const void* res, const void* out, int epi, int M, int N, int K) {
     if (M < 0 || N < 1 || K < 32 || K % 32 || K > (1 << 23) || epi < 1 || epi > 3 || (epi == 3 && N % 4)) {
-        set_error("%s: need epilogue 1..3, K a multiple of 32 up to 2^23 and for SwiGLU N a multiple of 4 (epi=%d M=%d N=%d K=%d)", who, epi, M, N, K);
+        set_error("%s: need epilogue 1..3, K a multiple of 32 up to 2^23 and for SwiGLU N a multiple of 4 (epi=%d M=%d N=%d K=%d)", who,
+                  epi, M, N, K);
         return SCMX_ERR_ARG;
     }
     if (M && (!w || !ws || !out || (epi == 2 && !res))) {
@@ -479,13 +498,15 @@ static int check_mm(const char* who, const void* w, const void* ws, const void* 
     return SCMX_OK;
 }
 
-// The tile that takes the least time, in us: alone on a CU a stage of 256 of K and a tile's beginning and end take so long, and so long for each
-// tile when every CU has some (a CU that holds several takes them in turn or side by side alike); measured from 17 to 8192 rows, 512 to 16384
-// columns, K from 256 to 8192, where the choice is half a per cent off the best on average.  us for 32x128 / 64x128 / 128x128 / 256x256: 100 rows
-// of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944 20.6 / 14.3 / 12.8 / 28.4, 6000 of 12288 x
-// 2048 180 / 124 / 92 / 89, of 2048 x 8192 114 / 70 / 74 / 56, 4000 of 16384 x 512 58 / 44 / 35 / 46.
-// Some rows go to the kernel of few, 16 at a time, where its workgroups are few too (us with tiles / with it: 17 rows of 2048 x 2048 5.9 / 3.5, of 4096 x
-// 4096 8.6 / 6.7, of 12288 x 2048 6.1 / 9.0, 64 rows of 2048 x 2048 6.1 / 4.5, of 2048 x 8192 14.2 / 11.9, of 4096 x 4096 8.8 / 12.2, 333 of 512 x 2048 6.0 / 5.7).
+// The tile that takes the least time, in us: alone on a CU a stage of 256 of K and a tile's beginning and end take so long, and so long
+// for each tile when every CU has some (a CU that holds several takes them in turn or side by side alike); measured from 17 to 8192 rows,
+// 512 to 16384 columns, K from 256 to 8192, where the choice is half a per cent off the best on average.  us for 32x128 / 64x128 /
+// 128x128 / 256x256: 100 rows of 12288 x 2048 7.8 / 7.2 / 8.5 / 16.9, 333 of 5120 x 2944 11.2 / 9.6 / 11.0 / 24.5, 700 of 5120 x 2944
+// 20.6 / 14.3 / 12.8 / 28.4, 6000 of 12288 x 2048 180 / 124 / 92 / 89, of 2048 x 8192 114 / 70 / 74 / 56, 4000 of 16384 x 512 58 / 44 /
+// 35 / 46.
+// Some rows go to the kernel of few, 16 at a time, where its workgroups are few too (us with tiles / with it: 17 rows of 2048 x 2048 5.9 /
+// 3.5, of 4096 x 4096 8.6 / 6.7, of 12288 x 2048 6.1 / 9.0, 64 rows of 2048 x 2048 6.1 / 4.5, of 2048 x 8192 14.2 / 11.9, of 4096 x 4096
+// 8.8 / 12.2, 333 of 512 x 2048 6.0 / 5.7).
 constexpr int NO_TILE = 4;
 static int tile_of(int M, int N, int K, bool words) {
     constexpr int BM[4] = {32, 64, 128, 256}, BN[4] = {128, 128, 128, 256};
@@ -498,7 +519,8 @@ static int tile_of(int M, int N, int K, bool words) {
     for (int i = 0; i < most; ++i) {
         const int64_t tiles = (int64_t(M) + BM[i] - 1) / BM[i] * ((int64_t(N) + BN[i] - 1) / BN[i]);
         const double load = tiles < cus ? double(tiles) / cus : double((tiles + cus - 1) / cus);
-        const double alone = (ALONE[i] + (words ? 0 : 0.13)) * stages + ALONE_ENDS[i], full = ((FULL[i] + (words ? 0 : 0.08)) * stages + FULL_ENDS[i]) * load;
+        const double alone = (ALONE[i] + (words ? 0 : 0.13)) * stages + ALONE_ENDS[i];
+        const double full = ((FULL[i] + (words ? 0 : 0.08)) * stages + FULL_ENDS[i]) * load;
         const double us = alone > full ? alone : full;
         if (us < least) {
             least = us;
@@ -542,10 +564,11 @@ extern "C" int scmx_mx_mm(const uint8_t* xcodes, const uint8_t* xscales, const u
     return check_launch("mx_mm");
 }
 
-// Whether a linear layer's rows are quantised in the product's own kernel, that of few: every workgroup of its columns does it for itself, which
-// costs a launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6, 16 rows of 4096 x 4096
-// (2^28) 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1 / 15.9, 64 rows of 2048 x 2048
-// (2^28) 6.3 / 7.4, 32 of 2048 x 8192 (2^29) 10.5 / 11.7, of 4096 x 4096 10.2 / 9.9, 64 of 2048 x 8192 (2^30) 18.3 / 15.5.
+// Whether a linear layer's rows are quantised in the product's own kernel, that of few: every workgroup of its columns does it for
+// itself, which costs a launch less and reads the rows N / 16 times.  us in one / in two: a row of 4096 x 4096 (2^24 products) 4.4 / 6.6,
+// 16 rows of 4096 x 4096 (2^28) 6.4 / 8.1, of 12288 x 2048 (2^28.6) 8.1 / 9.3, 8 rows of 16384 x 4096 (2^29) 14.0 / 14.1, 16 (2^30) 18.1
+// / 15.9, 64 rows of 2048 x 2048 (2^28) 6.3 / 7.4, 32 of 2048 x 8192 (2^29) 10.5 / 11.7, of 4096 x 4096 10.2 / 9.9, 64 of 2048 x 8192
+// (2^30) 18.3 / 15.5.
 static bool in_one(int M, int N, int K) {   // (bytes off a word only turn more to that kernel)
     return int64_t(M) * N <= (int64_t(1) << 29) / K && (M <= FEW || tile_of(M, N, K, K % 128 == 0) == NO_TILE);
 }
@@ -565,7 +588,8 @@ extern "C" int scmx_mx_linear(const uint16_t* x, int64_t ldx, const uint16_t* nw
         return SCMX_ERR_WORKSPACE;
     }
     if (M && (!x || uintptr_t(x) % 2 || uintptr_t(nw) % 2 || (M > 1 && (ldx < K || ldx > INT64_MAX / 8 / M)) || (nw && K > 16384))) {
-        set_error("mx_linear: need bf16 rows at least K apart, of up to 16384 values with a norm (M=%d K=%d ldx=%lld)", M, K, (long long)ldx);
+        set_error("mx_linear: need bf16 rows at least K apart, of up to 16384 values with a norm (M=%d K=%d ldx=%lld)", M, K,
+                  (long long)ldx);
         return SCMX_ERR_ARG;
     }
     if (M == 0) return SCMX_OK;

@@ -87,21 +87,25 @@ __device__ __forceinline__ double wave_sum(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     double sum = 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        sum += __builtin_bit_cast(double, uint64_t(uint32_t(__builtin_amdgcn_readlane(int(b >> 32), 16 * r))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(b), 16 * r)));
+    for (int r = 0; r < 4; ++r) {
+        const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(b >> 32), 16 * r));
+        const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(b), 16 * r));
+        sum += __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+    }
     return sum;
 }
 
-// RMSNorm first: WPR waves a row, NC pieces of 8 values a lane.  The codes are those of the float64 values: a product rounded to float32 lands on the
-// other side of a border between codes once in a million values, a third of the block's largest value off.  The sum of squares is in float64.  A
-// value times its gain is exact in float32; times the inverse less and more 2^-21 of it, which is rounded to within 3 * 2^-24, float64's result
-// lies between the two, and if both take the same code and byte, so does it.  If not, once in some thousand pieces, or where a product leaves
-// float32's range, the wave takes its piece in float64.  8192 rows of 2048 take 11.4 us, 32768 33.5 (without the norm 6.5, 25.0: memory); all in float64 16.8, its
-// instructions.
+// RMSNorm first: WPR waves a row, NC pieces of 8 values a lane.  The codes are those of the float64 values: a product rounded to float32
+// lands on the other side of a border between codes once in a million values, a third of the block's largest value off.  The sum of
+// squares is in float64.  A value times its gain is exact in float32; times the inverse less and more 2^-21 of it, which is rounded to
+// within 3 * 2^-24, float64's result lies between the two, and if both take the same code and byte, so does it.  If not, once in some
+// thousand pieces, or where a product leaves float32's range, the wave takes its piece in float64.  In a graph 8192 rows of 2048 take
+// 11.4-11.8 us, 32768 33.5-33.9 (without the norm 6.5-7.0, 25.0-25.7: memory); all in float64 16.8, its instructions.
 template <int NC, int WPR, bool ALIGNED>
-__global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ nw,
-                                                               float eps, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int M,
-                                                               int K) {
+__global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(const uint16_t* __restrict__ x, int64_t ldx,
+                                                                               const uint16_t* __restrict__ nw, float eps,
+                                                                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                               int M, int K) {
     __shared__ double s_sum[QNT / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = wave % WPR * 64 + lane;
     const uint64_t unit = block_index() * (QNT / 64 / WPR) + wave / WPR;
@@ -131,7 +135,8 @@ __global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(c
     }
     const double inv = 1.0 / sqrt(ss / double(K) + double(eps));
     const float inv32 = float(inv), less = inv32 * (1.0f - 0x1p-21f), more = inv32 * (1.0f + 0x1p-21f);
-    // (not for an infinity or a NaN in the row; a product with a gain that float32 cannot hold, below 2^-126, is then a zero of blocks from 2^-58 on)
+    // (not for an infinity or a NaN in the row; a product with a gain that float32 cannot hold, below 2^-126, is then a zero of blocks from
+    // 2^-58 on)
     const bool plain = inv32 > 0x1p-120f && inv32 < 0x1p60f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(QNT, NC > 4 ? 2 : 4) void mx_norm_quantize_kernel(c
     }
 }
 
-// 32 values a lane, a block: 16 bytes of codes read.
+// Eight values a lane, a word of codes; four lanes share a block's byte.
 template <bool F32>
 __global__ __launch_bounds__(QNT) void mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             void* __restrict__ out, uint64_t words) {
@@ -189,7 +194,8 @@ template <int NC, bool ALIGNED>
 static void launch_norm(const void* x, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M, int K, int wpr,
                         hipStream_t st) {
     const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<grid_of((uint64_t(M) + 3) / 4), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
+    const dim3 fours = grid_of((uint64_t(M) + 3) / 4);
+    if (wpr == 1) mx_norm_quantize_kernel<NC, 1, ALIGNED><<<fours, dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
     else mx_norm_quantize_kernel<NC, 4, ALIGNED><<<grid_of(M), dim3(QNT), 0, st>>>(p, ldx, nw, eps, codes, scales, M, K);
 }
 
@@ -200,7 +206,8 @@ using namespace scmx;
 extern "C" int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint16_t* nw, float eps, uint8_t* codes, uint8_t* scales, int M,
                                 int K, void* stream) {
     if (M < 0 || K < 32 || K % 32 || K > (1 << 30) || (type != SCMX_MX_BF16 && type != SCMX_MX_F16 && type != SCMX_MX_F32)) {
-        set_error("mx_quantize: need rows of a multiple of 32 values, up to 2^30, in bf16, fp16 or float32 (M=%d K=%d type=%d)", M, K, type);
+        set_error("mx_quantize: need rows of a multiple of 32 values, up to 2^30, in bf16, fp16 or float32 (M=%d K=%d type=%d)", M, K,
+                  type);
         return SCMX_ERR_ARG;
     }
     if (M && (!x || !codes || !scales)) {
@@ -225,8 +232,8 @@ extern "C" int scmx_mx_quantize(const void* x, int type, int64_t ldx, const uint
     const hipStream_t st = (hipStream_t)stream;
     const bool aligned = (uintptr_t(x) | uintptr_t(nw)) % 16 == 0 && (M == 1 || ldx * size % 16 == 0);
     if (nw) {
-        // a wave a row where the rows are many and short enough for its registers, else four: 1024 / 2048 / 8192 rows of 2048 3.8 / 4.5 / 11.4 us,
-        // with four waves 3.3 / 4.7 / 12.8, 4096 rows of 1024 4.0 and 6.8
+        // a wave a row where the rows are many and short enough for its registers, else four: 1024 / 2048 / 8192 rows of 2048 3.8 / 4.5 /
+        // 11.4 us, with four waves 3.3 / 4.7 / 12.8, 4096 rows of 1024 4.0 and 6.8
         const int wpr = K <= 2048 && M >= 2048 ? 1 : 4, pieces = (K / 8 + 64 * wpr - 1) / (64 * wpr);
         const auto go = [&](auto nc) {
             constexpr int NC = decltype(nc)::value;
