@@ -55,3 +55,21 @@ def test_large_values_behind_scores_that_grow_and_fall(C):   # noqa: F811
                 out = C.attn_tree(q, *c[:2], pos, None, *c[2:], splits=splits)
                 assert torch.isfinite(out).all()
                 check_attention(out, q, c, chain, pos, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_values_of_rows_that_a_node_does_not_see(C, d):   # noqa: F811
+    """The nodes that do not see them give the bits they give without."""
+    T, hq, hk, pos = 37, 6, 2, 290
+    rnd = gen(d)
+    c = make_cache(rnd, hk, pos + T, d)
+    q = rnd(T, hq, d).to(BF).transpose(0, 1)
+    masks = O.line_masks(tree(T, 3))
+    for splits in (1, 3):
+        clean = C.attn_tree(q, *c[:2], pos, bits(masks), *c[2:], splits=splits)
+        large = [t.clone() for t in c]
+        large[3][:, pos + 4], large[3][:, pos + 11] = 252, 250
+        out = C.attn_tree(q, *large[:2], pos, bits(masks), *large[2:], splits=splits)
+        check_attention(out, q, large, masks, pos, d ** -0.5)
+        unseen = [i for i in range(T) if not (masks[i] >> 4 & 1 or masks[i] >> 11 & 1)]
+        assert unseen and torch.equal(out[unseen], clean[unseen])
